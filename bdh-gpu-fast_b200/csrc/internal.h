@@ -307,4 +307,60 @@ size_t state_decode_partial_bytes(int64_t B, int64_t H, int64_t N, int64_t D);
 size_t state_decode_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D);
 int launch_state_decode(const StateDecodeArgs& a, float* partial, float* qrot, cudaStream_t stream);
 
+// Operators on logits (token_logprobs.cu, distill_topk.cu). Rows are (outer, inner) pairs; strides
+// are in elements, {outer, inner} and, for lists, {outer, inner, entry}.
+struct TokenLogprobsArgs {
+  const void* logits = nullptr;  // (outer, inner, V), unit stride over V
+  int dtype = BDH_DTYPE_F32;
+  int64_t l_strides[2] = {0, 0};
+  const int64_t* tokens = nullptr;  // null: no token's figures
+  int64_t t_strides[2] = {0, 0};
+  int64_t ignore_index = -100;
+  int64_t outer = 0, inner = 0, V = 0, K = 0;
+  float temperature = 1.0f;
+  // forward outputs, one per row in row order; top_* K per row; any but stats may be null
+  float* logprob = nullptr;
+  float* lse = nullptr;
+  float* entropy = nullptr;
+  float* stats = nullptr;  // 2 per row: the largest logit, ln of the sum of exp((x - it) / temperature)
+  float* top_logprob = nullptr;
+  int64_t* top_index = nullptr;
+};
+int launch_token_logprobs(const TokenLogprobsArgs& a, cudaStream_t stream);
+
+// An upstream gradient per row (null: none), strided so that an expanded scalar is read in place.
+struct RowGrad {
+  const float* p = nullptr;
+  int64_t strides[2] = {0, 0};
+};
+struct TokenLogprobsBwdArgs {
+  TokenLogprobsArgs f;  // logits, tokens, sizes; stats, entropy and top_index as the forward wrote them
+  RowGrad g_logprob, g_lse, g_entropy;
+  const float* g_top = nullptr;  // K per row in row order
+  void* dlogits = nullptr;       // (outer, inner, V) in the logits' dtype
+  int64_t d_strides[2] = {0, 0};
+};
+int launch_token_logprobs_bwd(const TokenLogprobsBwdArgs& a, cudaStream_t stream);
+
+struct DistillTopkArgs {
+  const void* logits = nullptr;  // (outer, inner, V), unit stride over V
+  int dtype = BDH_DTYPE_F32;
+  int64_t l_strides[2] = {0, 0};
+  const int64_t* index = nullptr;  // (outer, inner, K)
+  int64_t i_strides[3] = {0, 0, 0};
+  const float* teacher = nullptr;  // (outer, inner, K)
+  int64_t t_strides[3] = {0, 0, 0};
+  RowGrad weight;  // null: 1
+  int64_t outer = 0, inner = 0, V = 0, K = 0;
+  float temperature = 1.0f;
+  int tail = 0;
+  float* loss = nullptr;   // one per row; null in the backward form
+  float* stats = nullptr;  // 4 per row (written by the forward when not null, read by the backward)
+  void* dlogits = nullptr;  // null: the loss alone
+  int64_t d_strides[2] = {0, 0};
+  RowGrad g_loss;  // backward form only
+};
+int launch_distill_topk(const DistillTopkArgs& a, cudaStream_t stream);
+int launch_distill_topk_bwd(const DistillTopkArgs& a, cudaStream_t stream);
+
 }  // namespace bdh

@@ -509,6 +509,247 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> residual_layer_norm(const at::
   return {out, out16};
 }
 
+// ------------------------------------------------------------------ operators on logits ----
+// Logits (..., V) as (outer, inner) rows of V with unit stride: the last leading dimension is
+// the inner one and the rest the outer, in place for up to two leading dimensions (and for more
+// where they flatten), else a copy.
+struct LogitRows {
+  at::Tensor t;
+  int64_t outer = 1, inner = 1, V = 0;
+  int64_t strides[2] = {0, 0};
+  std::vector<int64_t> lead;  // the caller's leading shape
+
+  LogitRows(const at::Tensor& x, const char* what) : t(x) {
+    if (x.dim() < 1) TORCH_CHECK_VALUE(false, std::string(what) + ": logits must be (..., V)");
+    require_cuda({&x});
+    if (x.scalar_type() != at::kFloat && x.scalar_type() != at::kBFloat16)
+      TORCH_CHECK_TYPE(false, std::string(what) + ": logits must be float32 or bfloat16, got " +
+                                  c10::toString(x.scalar_type()));
+    V = x.size(-1);
+    if (V < 1) TORCH_CHECK_VALUE(false, std::string(what) + ": the vocabulary is empty");
+    lead.assign(x.sizes().begin(), x.sizes().end() - 1);
+    for (size_t d = 0; d + 1 < lead.size(); ++d) outer *= lead[d];
+    if (!lead.empty()) inner = lead.back();
+    if (V > 1 && t.stride(-1) != 1) t = t.contiguous();
+    if (t.dim() > 3) t = t.numel() == 0 ? t : t.reshape({outer, inner, V});
+    if (t.dim() == 3) strides[0] = t.stride(0);
+    if (t.dim() >= 2) strides[1] = t.stride(-2);
+  }
+  int64_t rows() const { return outer * inner; }
+};
+
+// A tensor of one value per row (or, with entries, `extra` values per row) beside the logits'
+// leading shape, as its {outer, inner[, entry]} strides.
+struct BesideRows {
+  at::Tensor t;
+  int64_t strides[3] = {0, 0, 0};
+
+  BesideRows(const LogitRows& x, const at::Tensor& v, at::ScalarType dtype, int64_t extra,
+             const char* what)
+      : t(v) {
+    if (!t.is_cuda() || t.device() != x.t.device())
+      TORCH_CHECK(false, std::string(what) + " must be on the logits' device");
+    const int64_t lists = extra >= 0 ? 1 : 0;
+    const int64_t n = static_cast<int64_t>(x.lead.size());
+    bool ok = t.dim() == n + lists && (lists == 0 || t.size(-1) == extra);
+    for (int64_t d = 0; ok && d < n; ++d) ok = t.size(d) == x.lead[d];
+    if (!ok)
+      TORCH_CHECK_VALUE(false, std::string(what) + " has shape " + shape_str(t) +
+                                   ", which does not go with logits of " + shape_str(x.t));
+    if (t.scalar_type() != dtype) t = t.to(dtype);
+    if (n > 2 && t.numel() > 0)
+      t = lists ? t.reshape({x.outer, x.inner, extra}) : t.reshape({x.outer, x.inner});
+    const int64_t r = t.dim() - lists;
+    if (r >= 2) strides[0] = t.stride(r - 2);
+    if (r >= 1) strides[1] = t.stride(r - 1);
+    if (lists) strides[2] = t.stride(-1);
+  }
+};
+
+bool whole(const at::Tensor& t) { return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt; }
+
+// One upstream gradient or weight per row; a 0-dimensional or broadcast one is read in place.
+std::optional<BesideRows> per_row(const LogitRows& x, const std::optional<at::Tensor>& v,
+                                  const char* what) {
+  if (!v.has_value()) return std::nullopt;
+  if (!v->is_floating_point())
+    TORCH_CHECK_TYPE(false, std::string(what) + " must be a floating point tensor");
+  at::Tensor t = *v;
+  if (t.dim() == 0) t = t.expand(x.lead);
+  return BesideRows(x, t, at::kFloat, -1, what);
+}
+const float* data_of(const std::optional<BesideRows>& v) {
+  return v.has_value() ? v->t.data_ptr<float>() : nullptr;
+}
+const int64_t* strides_of(const std::optional<BesideRows>& v) {
+  static const int64_t none[2] = {0, 0};
+  return v.has_value() ? v->strides : none;
+}
+
+std::optional<BesideRows> token_rows(const LogitRows& x, const std::optional<at::Tensor>& tokens,
+                                     const char* what) {
+  if (!tokens.has_value()) return std::nullopt;
+  if (!whole(*tokens)) TORCH_CHECK_TYPE(false, std::string(what) + ": tokens must be int64 or int32");
+  return BesideRows(x, *tokens, at::kLong, -1, "tokens");
+}
+
+void check_temperature(double temperature, const char* what) {
+  if (!(temperature > 0.0) || !(temperature < 1e30) || !(temperature > 1e-30))
+    TORCH_CHECK_VALUE(false, std::string(what) + ": temperature must be positive and finite, got " +
+                                 std::to_string(temperature));
+}
+
+std::vector<int64_t> with_entries(const LogitRows& x, int64_t k) {
+  std::vector<int64_t> s = x.lead;
+  s.push_back(k);
+  return s;
+}
+
+using MaybeTensor = std::optional<at::Tensor>;
+
+// (logprob, entropy, lse, top_logprob, top_index, stats) per row; None where not asked for.
+std::tuple<MaybeTensor, at::Tensor, at::Tensor, MaybeTensor, MaybeTensor, MaybeTensor>
+token_logprobs(const at::Tensor& logits, const MaybeTensor& tokens, int64_t top_k,
+               double temperature, int64_t ignore_index, bool want_stats) {
+  const LogitRows x(logits, "token_logprobs");
+  if (top_k < 0 || top_k > BDH_TOP_MAX || top_k > x.V)
+    TORCH_CHECK_VALUE(false, "token_logprobs: top_k must be 0 to min(V, " +
+                                 std::to_string(BDH_TOP_MAX) + "), got " + std::to_string(top_k));
+  check_temperature(temperature, "token_logprobs");
+  const std::optional<BesideRows> tok = token_rows(x, tokens, "token_logprobs");
+  const c10::cuda::CUDAGuard guard(x.t.device());
+  const auto f32 = x.t.options().dtype(at::kFloat);
+  MaybeTensor logprob, top_logprob, top_index, stats;
+  if (tok.has_value()) logprob = at::empty(x.lead, f32);
+  at::Tensor entropy = at::empty(x.lead, f32), lse = at::empty(x.lead, f32);
+  if (top_k > 0) {
+    top_logprob = at::empty(with_entries(x, top_k), f32);
+    top_index = at::empty(with_entries(x, top_k), f32.dtype(at::kLong));
+  }
+  if (want_stats) stats = at::empty({x.rows(), 2}, f32);
+  auto fp = [](const MaybeTensor& t) { return t.has_value() ? t->data_ptr<float>() : nullptr; };
+  check_rc(bdh_token_logprobs(
+               x.t.data_ptr(), dtype_code(x.t), x.strides,
+               tok.has_value() ? tok->t.data_ptr<int64_t>() : nullptr, strides_of(tok),
+               ignore_index, fp(logprob), lse.data_ptr<float>(), entropy.data_ptr<float>(),
+               fp(stats), fp(top_logprob),
+               top_index.has_value() ? top_index->data_ptr<int64_t>() : nullptr, x.outer, x.inner,
+               x.V, top_k, static_cast<float>(temperature), stream_of(x.t)),
+           "token_logprobs");
+  return {logprob, entropy, lse, top_logprob, top_index, stats};
+}
+
+at::Tensor token_logprobs_bwd(const at::Tensor& logits, const MaybeTensor& tokens,
+                              const at::Tensor& stats, const MaybeTensor& entropy,
+                              const MaybeTensor& top_index, const MaybeTensor& g_logprob,
+                              const MaybeTensor& g_entropy, const MaybeTensor& g_lse,
+                              const MaybeTensor& g_top, double temperature, int64_t ignore_index) {
+  const LogitRows x(logits, "token_logprobs_bwd");
+  check_temperature(temperature, "token_logprobs_bwd");
+  const std::optional<BesideRows> tok = token_rows(x, tokens, "token_logprobs_bwd"),
+                                  glp = per_row(x, g_logprob, "g_logprob"),
+                                  gen = per_row(x, g_entropy, "g_entropy"),
+                                  gls = per_row(x, g_lse, "g_lse");
+  const int64_t k = g_top.has_value() && top_index.has_value() ? top_index->size(-1) : 0;
+  if (k > BDH_TOP_MAX || k > x.V)
+    TORCH_CHECK_VALUE(false, "token_logprobs_bwd: a list of " + std::to_string(k) + " is too long");
+  const c10::cuda::CUDAGuard guard(x.t.device());
+  auto rowmajor = [&](const MaybeTensor& v, at::ScalarType dtype, int64_t n, const char* what) {
+    if (!v->is_cuda() || v->device() != x.t.device() || v->scalar_type() != dtype || v->numel() != n)
+      TORCH_CHECK_VALUE(false, std::string("token_logprobs_bwd: bad ") + what);
+    return v->contiguous();
+  };
+  const at::Tensor st = rowmajor(stats, at::kFloat, 2 * x.rows(), "stats");
+  at::Tensor en, ti, gt;
+  if (gen.has_value()) {
+    if (!entropy.has_value()) TORCH_CHECK_VALUE(false, "token_logprobs_bwd: g_entropy needs entropy");
+    en = rowmajor(entropy, at::kFloat, x.rows(), "entropy");
+  }
+  if (k > 0) {
+    ti = rowmajor(top_index, at::kLong, k * x.rows(), "top_index");
+    gt = rowmajor(g_top, at::kFloat, k * x.rows(), "g_top");
+  }
+  at::Tensor d = at::empty(logits.sizes(), x.t.options());
+  const int64_t ds[2] = {x.inner * x.V, x.V};
+  check_rc(bdh_token_logprobs_bwd(
+               x.t.data_ptr(), dtype_code(x.t), x.strides,
+               tok.has_value() ? tok->t.data_ptr<int64_t>() : nullptr, strides_of(tok),
+               ignore_index, st.data_ptr<float>(), gen.has_value() ? en.data_ptr<float>() : nullptr,
+               k > 0 ? ti.data_ptr<int64_t>() : nullptr, data_of(glp), strides_of(glp),
+               data_of(gls), strides_of(gls), data_of(gen), strides_of(gen),
+               k > 0 ? gt.data_ptr<float>() : nullptr, d.data_ptr(), ds, x.outer, x.inner, x.V, k,
+               static_cast<float>(temperature), stream_of(x.t)),
+           "token_logprobs_bwd");
+  return d;
+}
+
+struct DistillList {
+  BesideRows index, teacher;
+  std::optional<BesideRows> weight;
+  int64_t k;
+};
+DistillList distill_list(const LogitRows& x, const at::Tensor& index, const at::Tensor& teacher,
+                         const MaybeTensor& weight, double temperature) {
+  if (!whole(index)) TORCH_CHECK_TYPE(false, "distill_topk: teacher_index must be int64 or int32");
+  if (!teacher.is_floating_point())
+    TORCH_CHECK_TYPE(false, "distill_topk: teacher_logprob must be a floating point tensor");
+  const int64_t k = index.dim() > 0 ? index.size(-1) : 0;
+  if (k < 1 || k > BDH_TOP_MAX)
+    TORCH_CHECK_VALUE(false, "distill_topk: the list must have 1 to " + std::to_string(BDH_TOP_MAX) +
+                                 " slots, got " + std::to_string(k));
+  check_temperature(temperature, "distill_topk");
+  return {BesideRows(x, index, at::kLong, k, "teacher_index"),
+          BesideRows(x, teacher, at::kFloat, k, "teacher_logprob"), per_row(x, weight, "weight"), k};
+}
+
+// (loss per row, dlogits or None, stats or None)
+std::tuple<at::Tensor, MaybeTensor, MaybeTensor> distill_topk(
+    const at::Tensor& logits, const at::Tensor& index, const at::Tensor& teacher,
+    const MaybeTensor& weight, double temperature, bool tail, bool want_grad, bool want_stats) {
+  const LogitRows x(logits, "distill_topk");
+  const c10::cuda::CUDAGuard guard(x.t.device());
+  const DistillList l = distill_list(x, index, teacher, weight, temperature);
+  const auto f32 = x.t.options().dtype(at::kFloat);
+  at::Tensor loss = at::empty(x.lead, f32);
+  MaybeTensor d, stats;
+  if (want_grad) d = at::empty(logits.sizes(), x.t.options());
+  if (want_stats) stats = at::empty({x.rows(), 4}, f32);
+  const int64_t ds[2] = {x.inner * x.V, x.V};
+  check_rc(bdh_distill_topk(x.t.data_ptr(), dtype_code(x.t), x.strides,
+                            l.index.t.data_ptr<int64_t>(), l.index.strides,
+                            l.teacher.t.data_ptr<float>(), l.teacher.strides, data_of(l.weight),
+                            strides_of(l.weight), loss.data_ptr<float>(),
+                            want_stats ? stats->data_ptr<float>() : nullptr,
+                            want_grad ? d->data_ptr() : nullptr, ds, x.outer, x.inner, x.V, l.k,
+                            static_cast<float>(temperature), tail ? 1 : 0, stream_of(x.t)),
+           "distill_topk");
+  return {loss, d, stats};
+}
+
+at::Tensor distill_topk_bwd(const at::Tensor& logits, const at::Tensor& index,
+                            const at::Tensor& teacher, const MaybeTensor& weight,
+                            const at::Tensor& stats, const at::Tensor& g_loss, double temperature,
+                            bool tail) {
+  const LogitRows x(logits, "distill_topk_bwd");
+  const c10::cuda::CUDAGuard guard(x.t.device());
+  const DistillList l = distill_list(x, index, teacher, weight, temperature);
+  const std::optional<BesideRows> g = per_row(x, g_loss, "g_loss");
+  if (!stats.is_cuda() || stats.device() != x.t.device() || stats.scalar_type() != at::kFloat ||
+      stats.numel() != 4 * x.rows())
+    TORCH_CHECK_VALUE(false, "distill_topk_bwd: bad stats");
+  const at::Tensor st = stats.contiguous();
+  at::Tensor d = at::empty(logits.sizes(), x.t.options());
+  const int64_t ds[2] = {x.inner * x.V, x.V};
+  check_rc(bdh_distill_topk_bwd(x.t.data_ptr(), dtype_code(x.t), x.strides,
+                                l.index.t.data_ptr<int64_t>(), l.index.strides,
+                                l.teacher.t.data_ptr<float>(), l.teacher.strides, data_of(l.weight),
+                                strides_of(l.weight), st.data_ptr<float>(), data_of(g),
+                                strides_of(g), d.data_ptr(), ds, x.outer, x.inner, x.V, l.k,
+                                static_cast<float>(temperature), tail ? 1 : 0, stream_of(x.t)),
+           "distill_topk_bwd");
+  return d;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -548,6 +789,23 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("residual_layer_norm", &residual_layer_norm,
         "(LN(x + LN(y)), its bf16 copy or None): the BDH layer's residual double LayerNorm",
         py::arg("x"), py::arg("y"), py::arg("eps") = 1e-5, py::arg("want_bf16") = false);
+  m.def("token_logprobs", &token_logprobs,
+        "(logprob, entropy, lse, top_logprob, top_index, stats) of every row of logits",
+        py::arg("logits"), py::arg("tokens") = py::none(), py::arg("top_k") = 0,
+        py::arg("temperature") = 1.0, py::arg("ignore_index") = -100, py::arg("want_stats") = false);
+  m.def("token_logprobs_bwd", &token_logprobs_bwd, "gradient of token_logprobs by the logits",
+        py::arg("logits"), py::arg("tokens"), py::arg("stats"), py::arg("entropy") = py::none(),
+        py::arg("top_index") = py::none(), py::arg("g_logprob") = py::none(),
+        py::arg("g_entropy") = py::none(), py::arg("g_lse") = py::none(),
+        py::arg("g_top") = py::none(), py::arg("temperature") = 1.0, py::arg("ignore_index") = -100);
+  m.def("distill_topk", &distill_topk,
+        "(loss, dlogits or None, stats or None) against a teacher's list of top tokens",
+        py::arg("logits"), py::arg("teacher_index"), py::arg("teacher_logprob"),
+        py::arg("weight") = py::none(), py::arg("temperature") = 1.0, py::arg("tail") = false,
+        py::arg("want_grad") = false, py::arg("want_stats") = false);
+  m.def("distill_topk_bwd", &distill_topk_bwd, "gradient of distill_topk's loss by the logits",
+        py::arg("logits"), py::arg("teacher_index"), py::arg("teacher_logprob"), py::arg("weight"),
+        py::arg("stats"), py::arg("g_loss"), py::arg("temperature") = 1.0, py::arg("tail") = false);
   m.def("abi_version", &bdh_abi_version, "ABI version of the loaded libbdh_sm100.so");
   m.attr("has_cuda") = true;
 }

@@ -378,6 +378,73 @@ int bdh_decoder_f32(const float* x, int64_t ldx, const float* w, int64_t ldw, fl
                     int64_t ldo, float* partial, int64_t M, int64_t K, int64_t D, void* stream);
 
 /*
+ * Operators on a language model's logits (no counterpart in the reference, which computes its
+ * loss and its sampling with torch: bdh.py:680-728, :1066-1072). Rows are (outer, inner) pairs of
+ * V logits with unit stride over V and any {outer, inner} strides in elements (a shifted view
+ * [:, :-1] is read in place); statistics are fp32 whatever the logits' dtype (f32 or bf16). Rows
+ * start at any element: nothing needs to be aligned beyond the element size.
+ *
+ * bdh_token_logprobs: with z = x / temperature and lse = ln sum_i exp(z_i), per row
+ *   logprob = z[token] - lse (0 for token == ignore_index, NaN for any other token outside
+ *   [0, V)), entropy = - sum p ln p, and the K <= BDH_TOP_MAX largest logits in falling order
+ *   (an equal value's lower index first, NaN before everything): top_logprob = z_i - lse, top_index.
+ * A row with no logit above -inf: lse = logprob = top_logprob = -inf, entropy = 0. NaN or +inf in
+ * a row makes its figures NaN. Outputs are in row order; lse, entropy and stats may be null, logprob
+ * and tokens are given together or not at all. stats (2 floats per row) is what the backward reads.
+ *
+ * bdh_token_logprobs_bwd: dlogits of the same row for upstream gradients g_* (null: none; strides
+ * {outer, inner}, 0 for a broadcast scalar; g_top: K per row in row order), in the logits' dtype:
+ *   dx_i = 1/temperature [ p_i (g_lse - g_logprob - sum_j g_top_j - g_entropy (ln p_i + entropy))
+ *                          + [i = token] g_logprob + sum_j [i = top_index_j] g_top_j ]
+ * Zero for a row with no logit above -inf.
+ */
+#define BDH_TOP_MAX 128
+int bdh_token_logprobs(const void* logits, int dtype, const int64_t l_strides[2],
+                       const int64_t* tokens, const int64_t t_strides[2], int64_t ignore_index,
+                       float* logprob, float* lse, float* entropy, float* stats,
+                       float* top_logprob, int64_t* top_index, int64_t outer, int64_t inner,
+                       int64_t V, int64_t K, float temperature, void* stream);
+int bdh_token_logprobs_bwd(const void* logits, int dtype, const int64_t l_strides[2],
+                           const int64_t* tokens, const int64_t t_strides[2], int64_t ignore_index,
+                           const float* stats, const float* entropy, const int64_t* top_index,
+                           const float* g_logprob, const int64_t glp_strides[2],
+                           const float* g_lse, const int64_t gls_strides[2],
+                           const float* g_entropy, const int64_t gen_strides[2],
+                           const float* g_top, void* dlogits, const int64_t d_strides[2],
+                           int64_t outer, int64_t inner, int64_t V, int64_t K, float temperature,
+                           void* stream);
+
+/*
+ * Distillation from a teacher's list of K <= BDH_TOP_MAX (token, log probability) slots per row
+ * against the student's p = softmax(x / temperature):
+ *   tail = 0: q = softmax of the slots' values (log probabilities or logits / temperature);
+ *   tail = 1: q_j = exp(value_j), and "every other token" is one more class with
+ *             r = max(0, 1 - sum_j q_j) against s = the sum of p over unlisted tokens
+ *   loss = w [ sum_j q_j (ln q_j - ln p[index_j]) + r (ln r - ln s) ]
+ *   dx_i = w/temperature [ p_i (sum_j q_j + r) - r p_i / s [i unlisted] - sum_j q_j [i = index_j] ]
+ * index < 0: an empty slot; index >= V: the row's loss and gradient are NaN; a repeated token's
+ * masses add. weight null: 1; a row of weight 0 gives exact zeros and its logits are not read.
+ * When the list holds every token there is no other class (r = 0). A row with no logit above -inf
+ * has loss +inf and gradient 0.
+ * bdh_distill_topk writes the loss per row and, with dlogits, the gradient of the sum of the losses
+ * in the same call (the logits are read from memory once); stats (4 floats per row, may be null) is
+ * what bdh_distill_topk_bwd reads, which multiplies the gradient of each row by g_loss.
+ */
+int bdh_distill_topk(const void* logits, int dtype, const int64_t l_strides[2],
+                     const int64_t* index, const int64_t i_strides[3], const float* teacher,
+                     const int64_t t_strides[3], const float* weight, const int64_t w_strides[2],
+                     float* loss, float* stats, void* dlogits, const int64_t d_strides[2],
+                     int64_t outer, int64_t inner, int64_t V, int64_t K, float temperature,
+                     int tail, void* stream);
+int bdh_distill_topk_bwd(const void* logits, int dtype, const int64_t l_strides[2],
+                         const int64_t* index, const int64_t i_strides[3], const float* teacher,
+                         const int64_t t_strides[3], const float* weight,
+                         const int64_t w_strides[2], const float* stats, const float* g_loss,
+                         const int64_t g_strides[2], void* dlogits, const int64_t d_strides[2],
+                         int64_t outer, int64_t inner, int64_t V, int64_t K, float temperature,
+                         int tail, void* stream);
+
+/*
  * Launch timing for benchmarks (no counterpart in the reference, which timed whole calls with
  * perf_counter, benchmarks/bench_gpu_attn.py:263-280). Between begin and end, every kernel of
  * this library is bracketed by CUDA events on its own stream; end synchronises them and
@@ -386,6 +453,7 @@ int bdh_decoder_f32(const float* x, int64_t ldx, const float* w, int64_t ldw, fl
  *   7 gated product (bdh_relu_mul), 8 state pass of the chunked forward,
  *   9 latent encode (bdh_latent_encode), 10 latent gate (bdh_latent_gate), 11 LayerNorms,
  *   12 fp32 decoder product of a decode step (bdh_decoder_f32).
+ * The operators on logits are not among the kinds and are not bracketed.
  */
 #define BDH_PROF_KINDS 13
 int bdh_profile_begin(void);
