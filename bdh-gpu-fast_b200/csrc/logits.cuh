@@ -53,6 +53,82 @@ __device__ __forceinline__ void logit_put(uint16_t* p, int64_t i, float v) {
   p[i] = static_cast<uint16_t>(f32_to_bf16_bits(v));
 }
 
+// ------------------------------------------------------------------------ vectors ----
+// A row is read as 16-byte vectors of kVec<T> elements between its first and last 16-byte
+// boundary, and element by element before and after them (rows start at any element, so the
+// vectors of two rows may lie differently). Nothing outside the row is read.
+template <typename T>
+constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+
+struct RowSpan {
+  int head, vecs, tail;  // elements, vectors, elements
+};
+template <typename T>
+__device__ __forceinline__ RowSpan row_span(const T* p, int n) {
+  RowSpan r;
+  r.head = static_cast<int>(((16u - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / sizeof(T));
+  if (r.head > n) r.head = n;
+  r.vecs = (n - r.head) / kVec<T>;
+  r.tail = n - r.head - r.vecs * kVec<T>;
+  return r;
+}
+
+// Two fp32 in a register pair: sm_100's packed arithmetic does both with one instruction, each
+// rounded as its scalar form.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_split(const F2& x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+}
+__device__ __forceinline__ F2 f2_add(const F2& a, const F2& b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_mul(const F2& a, const F2& b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_fma(const F2& a, const F2& b, const F2& c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// The elements of a 16-byte vector as fp32.
+__device__ __forceinline__ void unpack(const uint4& u, float (&x)[4]) {
+  x[0] = __uint_as_float(u.x);
+  x[1] = __uint_as_float(u.y);
+  x[2] = __uint_as_float(u.z);
+  x[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void unpack(const uint4& u, float (&x)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = bf16x2_lo(w[i]);
+    x[2 * i + 1] = bf16x2_hi(w[i]);
+  }
+}
+// A vector of -inf: what a place past the end of a row counts as.
+template <typename T>
+__device__ __forceinline__ uint4 void_vec();
+template <>
+__device__ __forceinline__ uint4 void_vec<float>() {
+  return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+}
+template <>
+__device__ __forceinline__ uint4 void_vec<uint16_t>() {
+  return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+}
+
 // Offset of row r of a two-level layout (outer stride, inner stride) in elements.
 struct RowLayout {
   int64_t so = 0, si = 0;
@@ -99,6 +175,40 @@ __device__ __forceinline__ SoftState soft_warp(SoftState st, float c) {
   return st;
 }
 
+// Raise the state's maximum to m (not below it; NaN stays).
+__device__ __forceinline__ void soft_raise(SoftState& st, float m, float c) {
+  const float d = max_nan((st.m - m) * c, kExpFloor);
+  const float f = ex2(d);
+  st.a = f * fmaf(d, st.s, st.a);
+  st.s *= f;
+  st.m = m;
+}
+// Add N elements none of which is above the state's maximum, which is not -inf.
+template <bool ENTROPY, int N>
+__device__ __forceinline__ void soft_sum(SoftState& st, const float (&x)[N], float c) {
+  const F2 nm = f2(-st.m, -st.m), cc = f2(c, c);
+  F2 s = f2(0.0f, 0.0f), a = f2(0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    float t0, t1;
+    f2_split(f2_mul(f2_add(f2(x[i], x[i + 1]), nm), cc), t0, t1);
+    if (ENTROPY) {
+      t0 = max_nan(t0, kExpFloor);
+      t1 = max_nan(t1, kExpFloor);
+    }
+    const F2 e = f2(ex2(t0), ex2(t1));
+    s = f2_add(s, e);
+    if (ENTROPY) a = f2_fma(e, f2(t0, t1), a);
+  }
+  float s0, s1, a0, a1;
+  f2_split(s, s0, s1);
+  st.s += s0 + s1;
+  if (ENTROPY) {
+    f2_split(a, a0, a1);
+    st.a += a0 + a1;
+  }
+}
+
 // Order of a row's top list: larger values first, an equal value's lower index first; -0 equals
 // +0, and NaN comes before everything (as torch.sort places it). Larger key, earlier place;
 // key 0 stands for "no element" and is below every element's, ~0 is above.
@@ -115,6 +225,31 @@ __device__ __forceinline__ uint64_t top_key(float x, uint32_t i) {
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t k) {
   return 0xffffffffu - static_cast<uint32_t>(k);
+}
+
+// ------------------------------------------------------------------------ clusters ----
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Address of the local shared variable at `p` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_smem(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void peer_store(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void peer_store(uint32_t addr, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
 }  // namespace bdh

@@ -5,8 +5,13 @@
 //   dx_i = 1/temperature [ p_i (g_lse - g_logprob - sum_j g_top_j - g_entropy (ln p_i + entropy))
 //                          + [i = token] g_logprob + sum_j [i = top_j] g_top_j ]
 //
-// One CTA per row; the row's softmax state in one pass (logits.cuh), the top list by K rounds of
-// "the largest below the last one" over the row.
+// The forward reads a row once. A group of threads (a warp for short rows and lists, else a CTA of
+// 256 threads, else a cluster of up to 8 CTAs with a slice of the row each) keeps a softmax state
+// per thread and joins them at the end, through distributed shared memory in a cluster. For the top
+// list it keeps the maximum of every batch of vectors that a thread reads (a cell); the K-th largest
+// of the threads' own maxima bounds the K-th largest logit from below, so that only cells above it
+// are looked at again, a few cache lines, and the few candidates are put in order by counting.
+#include <algorithm>
 #include <string>
 
 #include "bdh_sm100.h"
@@ -19,10 +24,39 @@ namespace bdh {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kUnroll = 4;       // vectors that a thread has in flight (a batch)
+constexpr int kWarpTop = 16;     // longest list of the warp form: half of its threads' maxima
+constexpr int kMaxCells = 48;    // cells per thread; longer rows put more batches into a cell
+constexpr int kMaxCluster = 8;
 
-struct Shared {
-  SoftState part[kThreads / 32];
-  uint64_t key[kThreads / 32];
+// Threads' maxima that may lie above the bound besides the K wanted: the search for it ends early.
+__host__ __device__ constexpr int top_slack(int K) { return K / 4 + 4; }
+// Room for candidates: every element of the vectors that hold the maxima (a row of equal values),
+// and of the row's ends.
+template <typename T>
+constexpr int candidate_room(int K) {
+  return (K + top_slack(K)) * kVec<T> + 16;
+}
+
+struct ForwardPlan {
+  int cells, cell_batches;  // per thread; batches in a cell
+  int cluster;
+};
+
+template <int G>
+struct Group;
+template <>
+struct Group<32> {
+  static __device__ __forceinline__ void sync() { __syncwarp(); }
+  static __device__ __forceinline__ int count(bool p, int*) {
+    return __popc(__ballot_sync(0xffffffffu, p));
+  }
+};
+template <>
+struct Group<kThreads> {
+  static __device__ __forceinline__ void sync() { __syncthreads(); }
+  static __device__ __forceinline__ int count(bool p, int*) { return __syncthreads_count(p); }
 };
 
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
@@ -34,58 +68,303 @@ __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
   return k;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsArgs a, RowLayout ll,
-                                                                  RowLayout tl) {
-  __shared__ Shared sh;
-  const int64_t row = blockIdx.x;
+// Shared memory of one group; cells and candidates follow it (forward_smem).
+struct GroupShared {
+  SoftState part[kMaxCluster];
+  uint64_t best[kWarps];
+  SoftState warp_part[kWarps];
+  uint32_t lo[kWarps], hi[kWarps];
+  int found;
+};
+
+template <typename T, int G>
+__host__ __device__ constexpr size_t group_smem(int K, int cells, int cluster) {
+  size_t n = sizeof(GroupShared);
+  if (K > 0) {
+    n += (static_cast<size_t>(cells) * G * sizeof(float) + 7) & ~size_t(7);
+    n += static_cast<size_t>(candidate_room<T>(K)) * sizeof(uint64_t);
+    n += static_cast<size_t>(cluster) * K * sizeof(uint64_t);
+  }
+  return (n + 15) & ~size_t(15);
+}
+
+template <typename T, int G, int U, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsArgs a,
+                                                                  ForwardPlan plan) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  using Gr = Group<G>;
+  constexpr int kV = kVec<T>;
+  const int K = static_cast<int>(a.K), V = static_cast<int>(a.V);
+  const int C = G == 32 ? 1 : plan.cluster;
+  const uint32_t rank = C > 1 ? cta_rank() : 0;
+  const int tid = threadIdx.x % G, group = threadIdx.x / G;
+  uint8_t* base = smem + group * group_smem<T, G>(K, plan.cells, C);
+  GroupShared& sh = *reinterpret_cast<GroupShared*>(base);
+  float* cells = reinterpret_cast<float*>(base + sizeof(GroupShared));
+  uint64_t* cand = reinterpret_cast<uint64_t*>(
+      base + sizeof(GroupShared) + ((static_cast<size_t>(plan.cells) * G * 4 + 7) & ~size_t(7)));
+  uint64_t* lists = cand + candidate_room<T>(K);
+  const int64_t rows = a.outer * a.inner;
+  const int64_t row = G == 32 ? static_cast<int64_t>(blockIdx.x) * (kThreads / G) + group
+                              : static_cast<int64_t>(blockIdx.x) / C;
+  if (row >= rows) return;  // whole warps of the warp form
+  if (C > 1) cluster_arrive();  // every CTA's shared memory may be written once all have started
   const int64_t o = row / a.inner, i = row - o * a.inner;
-  const T* x = static_cast<const T*>(a.logits) + ll.at(o, i);
-  const int V = static_cast<int>(a.V);
+  const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
   const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
+
+  // This CTA's slice of the vectors; the row's head goes with the first slice, its tail with the last.
+  const RowSpan span = row_span(x, V);
+  const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
+  const int per = (span.vecs + C - 1) / C;
+  const int v0 = min(static_cast<int>(rank) * per, span.vecs), v1 = min(v0 + per, span.vecs);
   SoftState st = soft_empty();
-  for (int v = threadIdx.x; v < V; v += kThreads) soft_add(st, logit_at<T>(x, v), c);
+  int edge = -1;  // this thread's element of the row's ends
+  if (rank == 0 && tid < span.head) edge = tid;
+  if (rank == C - 1 && tid >= 8 && tid - 8 < span.tail) edge = V - span.tail + tid - 8;
+  float edge_x = neg_inf();
+  if (edge >= 0) {
+    edge_x = logit_at<T>(x, edge);
+    soft_add(st, edge_x, c);
+  }
+  // For the list: an index that the first occurrence of the thread's maximum is not above.
+  int at_most = edge >= 0 ? edge : span.head + (v0 + tid) * kV + kV - 1;
+  const bool any = edge >= 0 || v0 + tid < v1;
+
+  int cell = 0, in_cell = 0;
+  float cell_max = neg_inf();
+  for (int b = v0; b < v1; b += G * U) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = b + u * G + tid;
+      w[u] = v < v1 ? __ldg(vec + v) : void_vec<T>();
+    }
+    float xs[U * kV], vmax[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float part[kV];
+      unpack(w[u], part);
+      vmax[u] = part[0];
+#pragma unroll
+      for (int e = 0; e < kV; ++e) {
+        xs[u * kV + e] = part[e];
+        if (e > 0) vmax[u] = max_nan(vmax[u], part[e]);
+      }
+    }
+    float m = vmax[0];
+#pragma unroll
+    for (int u = 1; u < U; ++u) m = max_nan(m, vmax[u]);
+    if (!(m <= st.m)) {  // a larger one, or a NaN here or before (at_most may then rise further)
+      if (TOP) {
+        int u_first = U - 1;
+        if (m == m) {
+#pragma unroll
+          for (int u = U - 2; u >= 0; --u)
+            if (vmax[u] == m) u_first = u;
+        }
+        at_most = span.head + (b + u_first * G + tid) * kV + kV - 1;
+      }
+      soft_raise(st, max_nan(m, st.m), c);
+    }
+    if (st.m != neg_inf()) soft_sum<true>(st, xs, c);
+    if (TOP) {
+      cell_max = max_nan(cell_max, m);
+      if (++in_cell == plan.cell_batches) {
+        cells[cell++ * G + tid] = cell_max;
+        in_cell = 0;
+        cell_max = neg_inf();
+      }
+    }
+  }
+  if (TOP && in_cell > 0) cells[cell++ * G + tid] = cell_max;
+  const float own_max = st.m;
+
   st = soft_warp(st, c);
-  if ((threadIdx.x & 31) == 0) sh.part[threadIdx.x >> 5] = st;
-  __syncthreads();
-  st = sh.part[0];
-  for (int w = 1; w < kThreads / 32; ++w) st = soft_merge(st, sh.part[w], c);
-  const bool none = st.m == neg_inf();  // nothing finite in the row
+  if (G > 32) {
+    if ((threadIdx.x & 31) == 0) sh.warp_part[threadIdx.x >> 5] = st;
+    __syncthreads();
+    st = sh.warp_part[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) st = soft_merge(st, sh.warp_part[w], c);
+  }
+
+  if (TOP) {
+    // A bound below K elements of the slice: value key lo, and an index among elements of that value.
+    const uint32_t key = any ? value_key(own_max) : 0u;
+    at_most = min(at_most, V - 1);
+    if (tid == 0) sh.found = 0;
+    uint64_t bound = 0;
+    if (Gr::count(any, nullptr) >= K) {
+      uint32_t lo = __reduce_min_sync(0xffffffffu, any ? key : 0xffffffffu);
+      uint32_t hi = __reduce_max_sync(0xffffffffu, key);
+      if (G > 32) {
+        if ((threadIdx.x & 31) == 0) {
+          sh.lo[threadIdx.x >> 5] = lo;
+          sh.hi[threadIdx.x >> 5] = hi;
+        }
+        __syncthreads();
+        for (int w = 0; w < kWarps; ++w) {
+          lo = min(lo, sh.lo[w]);
+          hi = max(hi, sh.hi[w]);
+        }
+      }
+      ++hi;  // at least K maxima at or above lo, fewer than K at or above hi
+      int above = 0, at_lo = G;
+      while (hi - lo > 1 && at_lo > K + top_slack(K)) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        const int n = Gr::count(key >= mid, nullptr);
+        if (n >= K) {
+          lo = mid;
+          at_lo = n;
+        } else {
+          hi = mid;
+          above = n;
+        }
+      }
+      uint32_t last = 0xffffffffu;  // of equal values, those up to this index
+      if (hi - lo == 1 && at_lo > K + top_slack(K)) {
+        // count again: the search may have ended on its first interval
+        above = Gr::count(key > lo, nullptr);
+        uint32_t left = 0, right = static_cast<uint32_t>(V);  // fewer than wanted at left - 1, enough at right
+        int n = G;
+        while (left < right && n > K - above + top_slack(K)) {
+          const uint32_t mid = left + (right - left) / 2;
+          const int now = Gr::count(key == lo && static_cast<uint32_t>(at_most) <= mid, nullptr);
+          if (now >= K - above) {
+            right = mid;
+            n = now;
+          } else {
+            left = mid + 1;
+          }
+        }
+        last = right;
+      }
+      bound = (static_cast<uint64_t>(lo) << 32) |
+              (last == 0xffffffffu ? 0u : 0xffffffffu - last);
+    }
+    Gr::sync();  // sh.found is set
+    const uint32_t bound_value = static_cast<uint32_t>(bound >> 32);
+    const int room = candidate_room<T>(K);
+    auto offer = [&](float v, int at) {
+      const uint64_t k = top_key(v, at);
+      if (k >= bound) {
+        const int n = atomicAdd(&sh.found, 1);
+        if (n < room) cand[n] = k;
+      }
+    };
+    if (edge >= 0) offer(edge_x, edge);
+    if (value_key(own_max) >= bound_value) {
+      for (int q = 0; q < cell; ++q) {
+        if (value_key(cells[q * G + tid]) < bound_value) continue;
+        const int b0 = v0 + q * plan.cell_batches * G * U;
+        for (int b = b0; b < min(b0 + plan.cell_batches * G * U, v1); b += G) {
+          const int v = b + tid;
+          if (v >= v1) break;
+          float part[kV];
+          unpack(__ldg(vec + v), part);
+#pragma unroll
+          for (int e = 0; e < kV; ++e) offer(part[e], span.head + v * kV + e);
+        }
+      }
+    }
+    Gr::sync();
+    const int found = sh.found;
+    uint64_t* list = C > 1 ? lists + rank * K : lists;  // this slice's K largest in order
+    for (int k = tid; k < K; k += G) list[k] = 0;
+    Gr::sync();
+    if (found <= room) {
+      for (int n = tid; n < found; n += G) {
+        const uint64_t mine = cand[n];
+        int place = 0;
+        for (int q = 0; q < found; ++q) place += cand[q] > mine ? 1 : 0;
+        if (place < K) list[place] = mine;
+      }
+    } else {
+      // More elements above the bound than there is room for: large values that keep to few
+      // threads' cells. K rounds of "the largest below the last one" over the slice.
+      uint64_t last = ~0ull;
+      for (int k = 0; k < K; ++k) {
+        uint64_t best = 0;
+        auto look = [&](float v, int at) {
+          const uint64_t q = top_key(v, at);
+          if (q < last && q > best) best = q;
+        };
+        if (edge >= 0) look(edge_x, edge);
+        for (int v = v0 + tid; v < v1; v += G) {
+          float part[kV];
+          unpack(__ldg(vec + v), part);
+#pragma unroll
+          for (int e = 0; e < kV; ++e) look(part[e], span.head + v * kV + e);
+        }
+        best = warp_max_key(best);
+        if (G > 32) {
+          __syncthreads();
+          if ((threadIdx.x & 31) == 0) sh.best[threadIdx.x >> 5] = best;
+          __syncthreads();
+          for (int w = 0; w < kWarps; ++w) best = sh.best[w] > best ? sh.best[w] : best;
+        }
+        if (tid == 0) list[k] = best;
+        last = best;
+      }
+    }
+    Gr::sync();
+  }
+
+  if (C > 1) {
+    cluster_wait();
+    if (tid == 0) {
+      const uint32_t to = peer_smem(&sh.part[rank], 0);
+      peer_store(to, st.m);
+      peer_store(to + 4, st.s);
+      peer_store(to + 8, st.a);
+    }
+    if (TOP && rank != 0)
+      for (int k = tid; k < K; k += G) peer_store(peer_smem(lists + rank * K + k, 0), lists[rank * K + k]);
+    cluster_arrive();
+    cluster_wait();
+    if (rank != 0) return;
+    st = sh.part[0];
+    for (int r = 1; r < C; ++r) st = soft_merge(st, sh.part[r], c);
+  }
+
+  const bool none = st.m == neg_inf();  // nothing above -inf in the row
   const float ln_s = none ? neg_inf() : logf(st.s);
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     if (a.lse != nullptr) a.lse[row] = none ? neg_inf() : fmaf(st.m, inv_t, ln_s);
     if (a.entropy != nullptr) a.entropy[row] = none ? 0.0f : ln_s - kLn2 * st.a / st.s;
     if (a.stats != nullptr) {
       a.stats[2 * row] = st.m;
       a.stats[2 * row + 1] = ln_s;
     }
-    if (a.tokens != nullptr && a.logprob != nullptr) {
-      const int64_t tok = a.tokens[tl.at(o, i)];
+    if (a.tokens != nullptr) {
+      const int64_t tok = a.tokens[o * a.t_strides[0] + i * a.t_strides[1]];
       float lp = quiet_nan();
       if (tok == a.ignore_index) lp = 0.0f;
       else if (tok >= 0 && tok < V) lp = none ? neg_inf() : (logit_at<T>(x, tok) - st.m) * inv_t - ln_s;
       a.logprob[row] = lp;
     }
   }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < a.K; ++k) {
-    uint64_t best = 0;
-    for (int v = threadIdx.x; v < V; v += kThreads) {
-      const uint64_t key = top_key(logit_at<T>(x, v), v);
-      if (key < last && key > best) best = key;
-    }
-    best = warp_max_key(best);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh.key[threadIdx.x >> 5] = best;
-    __syncthreads();
-    for (int w = 0; w < kThreads / 32; ++w) best = sh.key[w] > best ? sh.key[w] : best;
-    last = best;
-    if (threadIdx.x == 0) {
-      const uint32_t at = key_index(best);
-      if (a.top_index != nullptr) a.top_index[row * a.K + k] = at;
-      if (a.top_logprob != nullptr)
-        a.top_logprob[row * a.K + k] =
-            none ? neg_inf() : (logit_at<T>(x, at) - st.m) * inv_t - ln_s;
+  if (TOP) {
+    for (int n = tid; n < C * K; n += G) {
+      const uint64_t mine = lists[n];
+      if (mine == 0) continue;  // a slice shorter than K
+      int place = n % K;
+      for (int r = 0; r < C; ++r) {  // and how many of the other slices' lists come before it
+        if (r == n / K) continue;
+        int lo = 0, hi = K;
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (lists[r * K + mid] > mine) lo = mid + 1;
+          else hi = mid;
+        }
+        place += lo;
+      }
+      if (place < K) {
+        a.top_index[row * K + place] = key_index(mine);
+        a.top_logprob[row * K + place] =
+            none ? neg_inf() : (key_value(static_cast<uint32_t>(mine >> 32)) - st.m) * inv_t - ln_s;
+      }
     }
   }
 }
@@ -164,17 +443,69 @@ int launch_check(const char* what) {
   return BDH_OK;
 }
 
+int sm_count_here() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return sm_count(dev);
+}
+
+template <typename T, int G, int U>
+int launch_forward(const TokenLogprobsArgs& a, int cluster, cudaStream_t stream) {
+  const int64_t rows = a.outer * a.inner;
+  ForwardPlan plan;
+  plan.cluster = cluster;
+  const int64_t vecs = (a.V / kVec<T> + cluster - 1) / cluster;
+  const int64_t batches = std::max<int64_t>(1, (vecs + G * U - 1) / (G * U));
+  plan.cell_batches = static_cast<int>((batches + kMaxCells - 1) / kMaxCells);
+  plan.cells = static_cast<int>((batches + plan.cell_batches - 1) / plan.cell_batches);
+  constexpr int kGroups = kThreads / G;
+  const size_t smem = kGroups * group_smem<T, G>(static_cast<int>(a.K), plan.cells, cluster);
+  auto* kern = a.K > 0 ? token_logprobs_kernel<T, G, U, true> : token_logprobs_kernel<T, G, U, false>;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(smem));
+    if (e != cudaSuccess) {
+      set_error(std::string("token_logprobs shared memory: ") + cudaGetErrorString(e));
+      return BDH_ERR_CUDA;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(G == 32 ? (rows + kGroups - 1) / kGroups : rows * cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kern, a, plan);
+  return launch_check("token_logprobs launch");
+}
+
+template <typename T>
+int forward_by_size(const TokenLogprobsArgs& a, cudaStream_t stream) {
+  const int64_t rows = a.outer * a.inner, vecs = a.V / kVec<T>;
+  if (a.V <= 1024 && a.K <= kWarpTop) {
+    if (vecs <= 32) return launch_forward<T, 32, 1>(a, 1, stream);
+    if (vecs <= 64) return launch_forward<T, 32, 2>(a, 1, stream);
+    return launch_forward<T, 32, kUnroll>(a, 1, stream);
+  }
+  // Few rows: split each until there are some CTAs for every SM or a slice is one batch.
+  int cluster = 1;
+  while (cluster < kMaxCluster && rows * cluster < 4 * sm_count_here() &&
+         vecs / (2 * cluster) >= kThreads * kUnroll)
+    cluster *= 2;
+  return launch_forward<T, kThreads, kUnroll>(a, cluster, stream);
+}
+
 }  // namespace
 
 int launch_token_logprobs(const TokenLogprobsArgs& a, cudaStream_t stream) {
-  const unsigned rows = static_cast<unsigned>(a.outer * a.inner);
-  if (rows == 0) return BDH_OK;
-  const RowLayout ll = {a.l_strides[0], a.l_strides[1]}, tl = {a.t_strides[0], a.t_strides[1]};
-  if (a.dtype == BDH_DTYPE_F32)
-    token_logprobs_kernel<float><<<rows, kThreads, 0, stream>>>(a, ll, tl);
-  else
-    token_logprobs_kernel<uint16_t><<<rows, kThreads, 0, stream>>>(a, ll, tl);
-  return launch_check("token_logprobs launch");
+  if (a.outer * a.inner == 0) return BDH_OK;
+  return a.dtype == BDH_DTYPE_F32 ? forward_by_size<float>(a, stream)
+                                  : forward_by_size<uint16_t>(a, stream);
 }
 
 int launch_token_logprobs_bwd(const TokenLogprobsBwdArgs& a, cudaStream_t stream) {
