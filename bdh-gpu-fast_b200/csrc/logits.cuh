@@ -117,6 +117,14 @@ __device__ __forceinline__ void unpack(const uint4& u, float (&x)[8]) {
     x[2 * i + 1] = bf16x2_hi(w[i]);
   }
 }
+// The other way, to a 16-byte aligned place.
+__device__ __forceinline__ void store_vec(float* p, const float (&x)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void store_vec(uint16_t* p, const float (&x)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(cvt_bf16x2(x[0], x[1]), cvt_bf16x2(x[2], x[3]),
+                                            cvt_bf16x2(x[4], x[5]), cvt_bf16x2(x[6], x[7]));
+}
 // A vector of -inf: what a place past the end of a row counts as.
 template <typename T>
 __device__ __forceinline__ uint4 void_vec();
@@ -129,13 +137,51 @@ __device__ __forceinline__ uint4 void_vec<uint16_t>() {
   return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
 }
 
-// Offset of row r of a two-level layout (outer stride, inner stride) in elements.
-struct RowLayout {
-  int64_t so = 0, si = 0;
-  __host__ __device__ __forceinline__ int64_t at(int64_t outer, int64_t inner) const {
-    return outer * so + inner * si;
+constexpr int kUnroll = 4;  // vectors that a thread has in flight (a batch)
+
+// d[i] = f(x[i]) for n elements by a group of G threads: `pair` on two elements, `single` on one,
+// or zeros. Vectors where x and d lie alike; else vectors are read and elements written.
+template <typename T, int G, typename Single, typename Pair>
+__device__ __forceinline__ void map_row(const T* x, T* d, int n, int tid, bool zero, Single single,
+                                        Pair pair) {
+  constexpr int kV = kVec<T>;
+  const RowSpan span = row_span(x, n);
+  const bool aligned = (reinterpret_cast<uintptr_t>(d + span.head) & 15u) == 0;
+  const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
+  T* out = d + span.head;
+  for (int e = tid; e < span.head + span.tail; e += G) {
+    const int at = e < span.head ? e : n - span.tail + (e - span.head);
+    logit_put(d, at, zero ? 0.0f : single(logit_at<T>(x, at)));
   }
-};
+  for (int b = 0; b < span.vecs; b += G * kUnroll) {
+    uint4 w[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int v = b + u * G + tid;
+      if (v < span.vecs && !zero) w[u] = __ldg(vec + v);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int v = b + u * G + tid;
+      if (v >= span.vecs) break;
+      float xs[kV], ds[kV];
+      if (zero) {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) ds[e] = 0.0f;
+      } else {
+        unpack(w[u], xs);
+#pragma unroll
+        for (int e = 0; e < kV; e += 2) pair(xs[e], xs[e + 1], ds[e], ds[e + 1]);
+      }
+      if (aligned) {
+        store_vec(out + static_cast<int64_t>(v) * kV, ds);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) logit_put(out, static_cast<int64_t>(v) * kV + e, ds[e]);
+      }
+    }
+  }
+}
 
 // Softmax state of a part of a row: maximum, sum, and exponent-weighted sum (see above).
 struct SoftState {

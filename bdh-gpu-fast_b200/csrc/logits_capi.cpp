@@ -121,6 +121,8 @@ int bdh_distill_topk(const void* logits, int dtype, const int64_t l_strides[2],
                      int tail, void* stream) {
   if (int rc = check_rows("distill_topk", dtype, outer, inner, V, K, temperature)) return rc;
   if (K < 1) return refuse("distill_topk", "the list needs at least one slot");
+  if (V > BDH_DISTILL_VOCAB_MAX)
+    return refuse("distill_topk", "the vocabulary is wider than BDH_DISTILL_VOCAB_MAX");
   if (outer * inner == 0) return BDH_OK;
   if (logits == nullptr || index == nullptr || teacher == nullptr || loss == nullptr)
     return refuse("distill_topk", "logits, index, teacher or loss is null");
@@ -149,6 +151,8 @@ int bdh_distill_topk_bwd(const void* logits, int dtype, const int64_t l_strides[
                          int tail, void* stream) {
   if (int rc = check_rows("distill_topk_bwd", dtype, outer, inner, V, K, temperature)) return rc;
   if (K < 1) return refuse("distill_topk_bwd", "the list needs at least one slot");
+  if (V > BDH_DISTILL_VOCAB_MAX)
+    return refuse("distill_topk_bwd", "the vocabulary is wider than BDH_DISTILL_VOCAB_MAX");
   if (outer * inner == 0) return BDH_OK;
   if (logits == nullptr || index == nullptr || teacher == nullptr || stats == nullptr ||
       g_loss == nullptr || dlogits == nullptr)

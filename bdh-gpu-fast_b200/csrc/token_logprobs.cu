@@ -25,7 +25,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kUnroll = 4;       // vectors that a thread has in flight (a batch)
 constexpr int kWarpTop = 16;     // longest list of the warp form: half of its threads' maxima
 constexpr int kMaxCells = 48;    // cells per thread; longer rows put more batches into a cell
 constexpr int kMaxCluster = 8;
@@ -109,7 +108,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
                               : static_cast<int64_t>(blockIdx.x) / C;
   if (row >= rows) return;  // whole warps of the warp form
   if (C > 1) cluster_arrive();  // every CTA's shared memory may be written once all have started
-  const int64_t o = row / a.inner, i = row - o * a.inner;
+  const int64_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
   const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
   const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
 
@@ -369,68 +368,96 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
   }
 }
 
+// The gradient writes as many bytes as it reads and needs nothing of a row but its two statistics, so
+// a row is cut into pieces of kPiece elements for the CTAs (short rows: a warp each). The token and
+// the list get their own terms in the CTA whose piece they lie in: the element is computed again with
+// its term added, so that it is rounded once.
+constexpr int kPiece = 16384;
+
 struct GradShared {
   int index[kTopMax + 1];
   float add[kTopMax + 1];
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(TokenLogprobsBwdArgs a) {
-  __shared__ GradShared sh;
-  const int64_t row = blockIdx.x;
-  const int64_t o = row / a.f.inner, i = row - o * a.f.inner;
-  const RowLayout ll = {a.f.l_strides[0], a.f.l_strides[1]}, dl = {a.d_strides[0], a.d_strides[1]};
-  const T* x = static_cast<const T*>(a.f.logits) + ll.at(o, i);
-  T* d = static_cast<T*>(a.dlogits) + dl.at(o, i);
+template <typename T, int G>
+__global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(TokenLogprobsBwdArgs a,
+                                                                      int pieces, int piece) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int tid = threadIdx.x % G, group = threadIdx.x / G;
+  GradShared& sh = *(reinterpret_cast<GradShared*>(smem) + group);  // with a list only
+  const uint32_t unit = blockIdx.x * (kThreads / G) + group;
+  const int64_t row = unit / static_cast<uint32_t>(pieces);
+  if (row >= a.f.outer * a.f.inner) return;  // whole warps of the warp form
+  const int64_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.f.inner), i = row - o * a.f.inner;
   const int V = static_cast<int>(a.f.V), K = a.g_top != nullptr ? static_cast<int>(a.f.K) : 0;
-  const float inv_t = 1.0f / a.f.temperature;
+  const int from = static_cast<int>(unit - static_cast<uint32_t>(row) * pieces) * piece, n = min(piece, V - from);
+  const T* x = static_cast<const T*>(a.f.logits) + o * a.f.l_strides[0] + i * a.f.l_strides[1];
+  T* d = static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1];
+  const float inv_t = 1.0f / a.f.temperature, c = kLog2e * inv_t;
   const float m = a.f.stats[2 * row], ln_s = a.f.stats[2 * row + 1];
+  const bool none = m == neg_inf();
   auto up = [&](const RowGrad& g) {
     return g.p != nullptr ? g.p[o * g.strides[0] + i * g.strides[1]] : 0.0f;
   };
-  float g_tok = up(a.g_logprob);
+  float g_tok = a.f.tokens != nullptr ? up(a.g_logprob) : 0.0f;
   const float g_ent = up(a.g_entropy);
   const float ent = a.g_entropy.p != nullptr ? a.f.entropy[row] : 0.0f;
   float sum = up(a.g_lse);
-  int64_t tok = -1;
+  int tok = -1;
   if (a.g_logprob.p != nullptr && a.f.tokens != nullptr) {
-    tok = a.f.tokens[o * a.f.t_strides[0] + i * a.f.t_strides[1]];
-    if (tok == a.f.ignore_index) {
-      tok = -1;
-      g_tok = 0.0f;
-    } else if (tok < 0 || tok >= V) {  // no such token: its log probability is NaN, and so is this
-      tok = -1;
-      sum = quiet_nan();
-    }
-  } else {
-    g_tok = 0.0f;
+    const int64_t t = a.f.tokens[o * a.f.t_strides[0] + i * a.f.t_strides[1]];
+    if (t == a.f.ignore_index) g_tok = 0.0f;
+    else if (t >= 0 && t < V) tok = static_cast<int>(t);
+    else sum = quiet_nan();  // no such token: its log probability is NaN, and so is this
   }
   sum -= g_tok;
-  for (int k = 0; k < K; ++k) sum -= a.g_top[row * K + k];
-  for (int k = threadIdx.x; k <= K; k += kThreads) {
-    sh.index[k] = k == 0 ? static_cast<int>(tok) : static_cast<int>(a.f.top_index[row * K + k - 1]);
-    sh.add[k] = k == 0 ? g_tok : a.g_top[row * K + k - 1];
+  if (K > 0) {
+    for (int k = tid; k <= K; k += G) {
+      sh.index[k] = k == 0 ? tok : static_cast<int>(a.f.top_index[row * K + k - 1]);
+      sh.add[k] = k == 0 ? g_tok : a.g_top[row * K + k - 1];
+    }
+    if (G == 32) __syncwarp();
+    else __syncthreads();
+    for (int k = 1; k <= K; ++k) sum -= sh.add[k];
   }
-  __syncthreads();
-  const bool none = m == neg_inf();
+  // With y = log2 p: p (sum - g_entropy (ln p + entropy)) / temperature = 2^y (k0 + k1 y)
+  const float shift = none ? 0.0f : -ln_s * kLog2e, m0 = none ? 0.0f : m;
+  const float k0 = (sum - g_ent * ent) * inv_t, k1 = -g_ent * kLn2 * inv_t;
+  const bool with_y = g_ent != 0.0f;  // NaN counts
+  const F2 nm2 = f2(-m0, -m0), c2 = f2(c, c), shift2 = f2(shift, shift);
   auto dense = [&](float v) {
-    const float t = (v - m) * inv_t - ln_s;
-    const float p = ex2(t * kLog2e);
-    return p * (sum - g_ent * (max_nan(t, kExpFloor) + ent));
+    const float y = fmaf(v - m0, c, shift);
+    return with_y ? ex2(y) * fmaf(k1, max_nan(y, kExpFloor), k0) : ex2(y) * k0;
   };
-  for (int v = threadIdx.x; v < V; v += kThreads)
-    logit_put(d, v, none ? 0.0f : dense(logit_at<T>(x, v)) * inv_t);
-  __syncthreads();
-  for (int k = threadIdx.x; k <= K; k += kThreads) {
+  auto pair = [&](float x0, float x1, float& d0, float& d1) {
+    float y0, y1;
+    f2_split(f2_fma(f2_add(f2(x0, x1), nm2), c2, shift2), y0, y1);
+    const F2 p = f2(ex2(y0), ex2(y1));
+    F2 w = f2(k0, k0);
+    if (with_y) w = f2_fma(f2(k1, k1), f2(max_nan(y0, kExpFloor), max_nan(y1, kExpFloor)), w);
+    f2_split(f2_mul(p, w), d0, d1);
+  };
+  map_row<T, G>(x + from, d + from, n, tid, none, dense, pair);
+  if (none) return;
+  if (K == 0) {
+    if (tok < from || tok >= from + n) return;
+    if (G == 32) __syncwarp();
+    else __syncthreads();
+    if (tid == 0) logit_put(d, tok, fmaf(g_tok, inv_t, dense(logit_at<T>(x, tok))));
+    return;
+  }
+  if (G == 32) __syncwarp();
+  else __syncthreads();
+  for (int k = tid; k <= K; k += G) {
     const int at = sh.index[k];
-    bool mine = at >= 0 && at < V && !none;
+    bool mine = at >= from && at < from + n;
     float add = sh.add[k];
     for (int j = 0; mine && j <= K; ++j)
-      if (j != k && sh.index[j] == at) {
+      if (j != k && sh.index[j] == at) {  // the token is in the list too: once, with both terms
         mine = j > k;
         add += sh.add[j];
       }
-    if (mine) logit_put(d, at, (dense(logit_at<T>(x, at)) + add) * inv_t);
+    if (mine) logit_put(d, at, fmaf(add, inv_t, dense(logit_at<T>(x, at))));
   }
 }
 
@@ -500,6 +527,25 @@ int forward_by_size(const TokenLogprobsArgs& a, cudaStream_t stream) {
   return launch_forward<T, kThreads, kUnroll>(a, cluster, stream);
 }
 
+template <typename T>
+int backward_by_size(const TokenLogprobsBwdArgs& a, cudaStream_t stream) {
+  const int64_t rows = a.f.outer * a.f.inner;
+  const size_t lists = a.g_top != nullptr && a.f.K > 0 ? sizeof(GradShared) : 0;
+  if (a.f.V <= 1024) {
+    const unsigned grid = static_cast<unsigned>((rows + kWarps - 1) / kWarps);
+    token_logprobs_bwd_kernel<T, 32><<<grid, kThreads, kWarps * lists, stream>>>(a, 1, static_cast<int>(a.f.V));
+  } else {
+    const int64_t pieces = (a.f.V + kPiece - 1) / kPiece;
+    if (rows * pieces >= int64_t(1) << 31) {
+      set_error("token_logprobs_bwd: too many rows for this vocabulary");
+      return BDH_ERR_INVALID;
+    }
+    token_logprobs_bwd_kernel<T, kThreads><<<static_cast<unsigned>(rows * pieces), kThreads, lists, stream>>>(
+        a, static_cast<int>(pieces), kPiece);
+  }
+  return launch_check("token_logprobs_bwd launch");
+}
+
 }  // namespace
 
 int launch_token_logprobs(const TokenLogprobsArgs& a, cudaStream_t stream) {
@@ -509,13 +555,9 @@ int launch_token_logprobs(const TokenLogprobsArgs& a, cudaStream_t stream) {
 }
 
 int launch_token_logprobs_bwd(const TokenLogprobsBwdArgs& a, cudaStream_t stream) {
-  const unsigned rows = static_cast<unsigned>(a.f.outer * a.f.inner);
-  if (rows == 0) return BDH_OK;
-  if (a.f.dtype == BDH_DTYPE_F32)
-    token_logprobs_bwd_kernel<float><<<rows, kThreads, 0, stream>>>(a);
-  else
-    token_logprobs_bwd_kernel<uint16_t><<<rows, kThreads, 0, stream>>>(a);
-  return launch_check("token_logprobs_bwd launch");
+  if (a.f.outer * a.f.inner == 0) return BDH_OK;
+  return a.f.dtype == BDH_DTYPE_F32 ? backward_by_size<float>(a, stream)
+                                    : backward_by_size<uint16_t>(a, stream);
 }
 
 }  // namespace bdh
