@@ -14,6 +14,10 @@
 // gradient from it, so that the logits cross HBM once. A warp takes a short row; else a CTA, or a
 // cluster whose CTAs hold a slice each and exchange their sums through distributed shared memory.
 // The backward from stored statistics has nothing to sum and streams.
+//
+// Repeated tokens are found while striking out: every slot writes its number in place of its token's
+// logit and reads it back, and where one finds another's number the masses are added up by a search
+// (K^2 comparisons, which as a rule cost more than the row itself and are seldom needed).
 #include <algorithm>
 #include <string>
 
@@ -31,122 +35,19 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kPiece = 16384;             // elements of a row per CTA of the streaming backward
 constexpr int kSliceBytes = 48 * 1024;    // of a row per CTA, while the cluster may grow
-static_assert(kThreads >= kTopMax, "one thread per slot");
+static_assert(kThreads - 32 >= kTopMax, "one thread per slot, and a warp beside them");
 
-template <int G>
-__device__ __forceinline__ void group_sync() {
-  if (G == 32) __syncwarp();
-  else __syncthreads();
-}
+constexpr int kStats = 8;  // floats per row: see RowStats
 
-// A row's list in shared memory, K entries each (rounded up to a warp).
-struct List {
-  int* index;    // -1: empty slot; V: a token past the vocabulary
-  float* lnq;
-  float* q;
-  float* z;      // the student's logit
-  float* mass;   // q summed over the slots of the same token; below 0: not the token's first slot
+// What the forward leaves for the gradient.
+struct RowStats {
+  float m, ln_s;            // largest logit, ln of the sum of exp((x - m) / temperature)
+  float rest_m, ln_rest;    // the same of the unlisted tokens
+  float total, r;           // mass of the list, and of the class beside it
+  float shift;              // ln q = teacher's value - shift
+  float repeated;           // 1: a token is in the list twice
 };
-struct GroupShared {
-  SoftState part[kMaxCluster];
-  SoftState warp_part[kWarps];
-  SoftState top;       // softmax state of the listed tokens
-  float total, r;      // mass of the list, of the class beside it
-};
-
-__host__ __device__ constexpr int list_room(int K) { return (K + 31) / 32 * 32; }
-__host__ __device__ constexpr size_t list_smem(int K) {
-  return sizeof(GroupShared) + 5 * sizeof(float) * static_cast<size_t>(list_room(K));
-}
-static_assert(sizeof(GroupShared) % 4 == 0, "lists follow");
-__host__ __device__ constexpr size_t group_smem(int K, size_t slice_bytes) {
-  return ((list_smem(K) + 15) & ~size_t(15)) + ((slice_bytes + 15) & ~size_t(15));
-}
-__device__ __forceinline__ List list_at(uint8_t* base, int K) {
-  float* p = reinterpret_cast<float*>(base + sizeof(GroupShared));
-  const int n = list_room(K);
-  return {reinterpret_cast<int*>(p), p + n, p + 2 * n, p + 3 * n, p + 4 * n};
-}
-
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, d));
-  return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  return v;
-}
-
-// The row's list: q, its mass and the other class's, the student's logits of the listed tokens and
-// their softmax state. Ends in a barrier of the group.
-template <typename T, int G>
-__device__ __forceinline__ void load_list(const DistillTopkArgs& a, const T* x, int64_t o, int64_t i,
-                                          int tid, float c, GroupShared& sh, const List& l) {
-  const int K = static_cast<int>(a.K), V = static_cast<int>(a.V);
-  for (int j = tid; j < K; j += G) {
-    const int64_t at = a.index[o * a.i_strides[0] + i * a.i_strides[1] + j * a.i_strides[2]];
-    const float t = a.teacher[o * a.t_strides[0] + i * a.t_strides[1] + j * a.t_strides[2]];
-    l.index[j] = at < 0 ? -1 : at < V ? static_cast<int>(at) : V;
-    l.lnq[j] = at < 0 ? neg_inf() : t;
-    l.z[j] = at >= 0 && at < V ? logit_at<T>(x, at) : neg_inf();
-  }
-  group_sync<G>();
-  if (tid < 32) {
-    float m = neg_inf();
-    for (int j = tid; j < K; j += 32) m = max_nan(m, l.lnq[j]);
-    m = warp_max(m);
-    float shift = 0.0f;
-    if (!a.tail && m != neg_inf()) {
-      float s = 0.0f;
-      for (int j = tid; j < K; j += 32) s += expf(l.lnq[j] - m);
-      shift = m + logf(warp_sum(s));
-    }
-    float total = 0.0f;
-    bool bad = false;
-    for (int j = tid; j < K; j += 32) {
-      const float v = l.lnq[j] - shift, q = expf(v);
-      l.lnq[j] = v;
-      l.q[j] = q;
-      total += q;
-      bad |= l.index[j] == V;
-    }
-    total = warp_sum(total);
-    __syncwarp();
-    // the masses of a repeated token go to its first slot
-    SoftState top = soft_empty();
-    int distinct = 0;
-    for (int j = tid; j < K; j += 32) {
-      const int at = l.index[j];
-      float mass = at >= 0 ? 0.0f : -1.0f;
-      if (at >= 0)
-        for (int k = 0; k < K; ++k)
-          if (l.index[k] == at) {
-            if (k < j) {
-              mass = -1.0f;
-              break;
-            }
-            mass += l.q[k];
-          }
-      l.mass[j] = mass;
-      if (!(mass < 0.0f)) {
-        soft_add(top, l.z[j], c);
-        ++distinct;
-      }
-    }
-    top = soft_warp(top, c);
-    distinct = __reduce_add_sync(0xffffffffu, distinct);
-    bad = __any_sync(0xffffffffu, bad);
-    if (tid == 0) {
-      sh.top = top;
-      sh.total = bad ? quiet_nan() : total;  // a token past the vocabulary: NaN throughout
-      // where every token is listed there is no other class
-      sh.r = a.tail && distinct < V ? max_nan(0.0f, 1.0f - total) : 0.0f;
-    }
-  }
-  group_sync<G>();
-}
+static_assert(sizeof(RowStats) == kStats * sizeof(float), "stored as it is");
 
 // What the gradient needs of a row: dx_i = 2^(c (x_i - m) + shift) coef for unlisted tokens.
 struct RowGradient {
@@ -155,64 +56,326 @@ struct RowGradient {
   float scale, total;          // listed: scale (p total - mass)
   bool none;                   // no logit above -inf in the row
 };
-__device__ __forceinline__ RowGradient row_gradient(const DistillTopkArgs& a, const GroupShared& sh,
-                                                    float m, float ln_s, float rest_m, float ln_rest,
+__device__ __forceinline__ RowGradient row_gradient(const RowStats& st, int tail, float inv_t,
                                                     float scale) {
-  const float inv_t = 1.0f / a.temperature;
   RowGradient g;
-  g.none = m == neg_inf();
+  g.none = st.m == neg_inf();
   g.scale = scale * inv_t;
-  g.total = sh.total + sh.r;
-  g.top_m = m;
-  g.top_shift = -ln_s * kLog2e;
-  g.m = m;
+  g.total = st.total + st.r;
+  g.top_m = st.m;
+  g.top_shift = -st.ln_s * kLog2e;
+  g.m = st.m;
   g.shift = g.top_shift;
   g.coef = g.scale * g.total;
-  if (a.tail) {
+  if (tail) {
     // p_i (total - r / s) = (p_i / s) (total s - r); nothing is unlisted and above -inf: all zeros
-    const float s = expf((rest_m - m) * inv_t + ln_rest - ln_s);
-    const bool empty = rest_m == neg_inf();
-    g.m = empty ? 0.0f : rest_m;
-    g.shift = empty ? neg_inf() : -ln_rest * kLog2e;
-    g.coef = empty ? 0.0f : g.scale * (g.total * s - sh.r);
+    const float s = expf((st.rest_m - st.m) * inv_t + st.ln_rest - st.ln_s);
+    const bool empty = st.rest_m == neg_inf();
+    g.m = empty ? 0.0f : st.rest_m;
+    g.shift = empty ? neg_inf() : -st.ln_rest * kLog2e;
+    g.coef = empty ? 0.0f : g.scale * (g.total * s - st.r);
     if (g.total != g.total) g.coef = g.total;
   }
   return g;
 }
-// The gradient of the listed tokens of [from, to), over what the unlisted ones' formula left there.
-template <typename T, int G>
-__device__ __forceinline__ void write_listed(const RowGradient& g, const List& l, int K, int V, T* d,
-                                             int from, int to, int tid, float c) {
-  for (int j = tid; j < K; j += G) {
-    const int at = l.index[j];
-    if (at < from || at >= to || at >= V || l.mass[j] < 0.0f) continue;
-    const float p = ex2(fmaf(l.z[j] - g.top_m, c, g.top_shift));
-    logit_put(d, at, g.scale * (p * g.total - l.mass[j]));
-  }
+__device__ __forceinline__ float listed_gradient(const RowGradient& g, float z, float mass, float c) {
+  return g.scale * (ex2(fmaf(z - g.top_m, c, g.top_shift)) * g.total - mass);
 }
+// The formula for unlisted tokens, on one element and on two.
+struct Unlisted {
+  RowGradient g;
+  float c;
+  F2 nm2, c2, shift2, coef2;
+  __device__ __forceinline__ Unlisted(const RowGradient& g_, float c_)
+      : g(g_), c(c_), nm2(f2(-g_.m, -g_.m)), c2(f2(c_, c_)), shift2(f2(g_.shift, g_.shift)),
+        coef2(f2(g_.coef, g_.coef)) {}
+  __device__ __forceinline__ float operator()(float x) const {
+    return ex2(fmaf(x - g.m, c, g.shift)) * g.coef;
+  }
+  __device__ __forceinline__ void operator()(float x0, float x1, float& d0, float& d1) const {
+    float y0, y1;
+    f2_split(f2_fma(f2_add(f2(x0, x1), nm2), c2, shift2), y0, y1);
+    f2_split(f2_mul(f2(ex2(y0), ex2(y1)), coef2), d0, d1);
+  }
+};
+struct Nothing {
+  __device__ __forceinline__ float operator()(float) const { return 0.0f; }
+  __device__ __forceinline__ void operator()(float, float, float& a, float& b) const { a = b = 0.0f; }
+};
+
+// Loss of a row from its list (one warp; `slot(f)` calls f(ln q, q, z) for the lane's slots).
+template <typename Slots>
+__device__ __forceinline__ float warp_loss(const RowStats& st, float inv_t, Slots slots) {
+  const bool none = st.m == neg_inf();
+  float loss = 0.0f;
+  slots([&](float lnq, float q, float z) {
+    const float lp = none || z == neg_inf() ? neg_inf() : (z - st.m) * inv_t - st.ln_s;
+    if (!(q <= 0.0f)) loss = fmaf(q, lnq - lp, loss);
+  });
+  loss = warp_sum(loss);
+  if (st.r > 0.0f) {
+    const float ls = st.rest_m == neg_inf() ? neg_inf()
+                                            : (st.rest_m - st.m) * inv_t + st.ln_rest - st.ln_s;
+    loss = fmaf(st.r, logf(st.r) - ls, loss);
+  }
+  return st.total != st.total ? quiet_nan() : loss;
+}
+
+// A slot's token: -1 for an empty one, V for one past the vocabulary.
+__device__ __forceinline__ int slot_token(int64_t at, int V) {
+  return at < 0 ? -1 : at < V ? static_cast<int>(at) : V;
+}
+// A slot's number in place of a logit, and back.
+__device__ __forceinline__ void put_slot(float* p, int64_t at, int slot) {
+  reinterpret_cast<int*>(p)[at] = slot;
+}
+__device__ __forceinline__ void put_slot(uint16_t* p, int64_t at, int slot) {
+  p[at] = static_cast<uint16_t>(slot);
+}
+__device__ __forceinline__ int get_slot(const float* p, int64_t at) {
+  return reinterpret_cast<const int*>(p)[at];
+}
+__device__ __forceinline__ int get_slot(const uint16_t* p, int64_t at) { return p[at]; }
 
 template <typename T>
 __device__ __forceinline__ float row_weight(const DistillTopkArgs& a, int64_t o, int64_t i) {
   return a.weight.p != nullptr ? a.weight.p[o * a.weight.strides[0] + i * a.weight.strides[1]] : 1.0f;
 }
-struct NoSingle {
-  __device__ __forceinline__ float operator()(float) const { return 0.0f; }
-};
-struct NoPair {
-  __device__ __forceinline__ void operator()(float, float, float& a, float& b) const { a = b = 0.0f; }
-};
+// ------------------------------------------------------------------ a warp for a short row
+// Rows of at most kShort elements: the slots and the row's elements stay in the lanes' registers
+// (S slots, E elements and one of the row's unaligned ends); the row passes through shared memory
+// for the slots to find their logits.
+constexpr int kShort = 1024;
 
-template <typename T, int G>
-__global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillTopkArgs a, int C,
-                                                                size_t slice_bytes) {
+template <typename T, int E, int S>
+__global__ void __launch_bounds__(kThreads, E <= 16 && S == 1 ? 4 : 3) distill_short_kernel(DistillTopkArgs a) {
+  constexpr int kV = kVec<T>, kVecs = E / kV;
+  __shared__ __align__(16) T rows_held[kWarps][(kVecs * 32 + 2) * kV];
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  if (row >= a.outer * a.inner) return;
+  const int64_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
+  const int V = static_cast<int>(a.V), K = static_cast<int>(a.K);
+  const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
+  T* d = a.dlogits != nullptr
+             ? static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1]
+             : nullptr;
+  const float w = row_weight<T>(a, o, i);
+  if (w == 0.0f) {
+    if (d != nullptr) map_row<T, 32>(x, d, V, lane, true, Nothing(), Nothing());
+    if (lane == 0) a.loss[row] = 0.0f;
+    return;
+  }
+  // the row on its way to shared memory, the list to registers
+  const RowSpan span = row_span(x, V);
+  T* held = rows_held[threadIdx.x >> 5] + (kV - span.head) % kV;
+  const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
+  uint4* hvec = reinterpret_cast<uint4*>(held + span.head);
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const int v = u * 32 + lane;
+    if (v < span.vecs)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hvec + v)), "l"(vec + v)
+                   : "memory");
+  }
+  int edge = -1;  // this lane's element of the row's ends
+  if (lane < span.head) edge = lane;
+  if (lane >= 8 && lane - 8 < span.tail) edge = V - span.tail + lane - 8;
+  if (edge >= 0) held[edge] = x[edge];
+  int at[S];
+  float lnq[S], q[S], z[S], mass[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const int j = s * 32 + lane;
+    at[s] = -1;
+    lnq[s] = neg_inf();
+    if (j < K) {
+      at[s] = slot_token(a.index[o * a.i_strides[0] + i * a.i_strides[1] + j * a.i_strides[2]], V);
+      const float t = a.teacher[o * a.t_strides[0] + i * a.t_strides[1] + j * a.t_strides[2]];
+      if (at[s] >= 0) lnq[s] = t;
+    }
+  }
+  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
+  RowStats st;
+  st.shift = 0.0f;
+  if (!a.tail) {
+    float m = lnq[0], sum = 0.0f;
+#pragma unroll
+    for (int s = 1; s < S; ++s) m = max_nan(m, lnq[s]);
+    m = warp_max(m);
+    if (m != neg_inf()) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) sum += expf(lnq[s] - m);
+      st.shift = m + logf(warp_sum(sum));
+    }
+  }
+  st.total = 0.0f;
+  bool bad = false;
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    lnq[s] -= st.shift;
+    q[s] = expf(lnq[s]);
+    st.total += q[s];
+    bad |= at[s] == V;
+    if (at[s] == V) at[s] = -1;  // no token to find
+    mass[s] = at[s] >= 0 ? q[s] : -1.0f;
+  }
+  st.total = warp_sum(st.total);
+  st.r = a.tail ? max_nan(0.0f, 1.0f - st.total) : 0.0f;
+  if (__any_sync(0xffffffffu, bad)) st.total = quiet_nan();
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();
+#pragma unroll
+  for (int s = 0; s < S; ++s) z[s] = at[s] >= 0 ? logit_at<T>(held, at[s]) : neg_inf();
+  __syncwarp();
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+    if (at[s] >= 0) put_slot(held, at[s], s * 32 + lane);
+  __syncwarp();
+  bool other = false;
+#pragma unroll
+  for (int s = 0; s < S; ++s) other |= at[s] >= 0 && get_slot(held, at[s]) != s * 32 + lane;
+  st.repeated = __any_sync(0xffffffffu, other) ? 1.0f : 0.0f;  // and all have read
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+    if (at[s] >= 0) logit_put(held, at[s], neg_inf());
+  __syncwarp();
+  if (st.repeated != 0.0f) {  // masses to the first slot of each token
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      float sum = 0.0f;
+      bool first = at[s] >= 0;
+#pragma unroll
+      for (int t = 0; t < S; ++t)
+        for (int k = 0; k < 32; ++k) {
+          const int other_at = __shfl_sync(0xffffffffu, at[t], k);
+          const float other_q = __shfl_sync(0xffffffffu, q[t], k);
+          if (other_at != at[s]) continue;
+          sum += other_q;
+          if (t * 32 + k < s * 32 + lane) first = false;
+        }
+      mass[s] = first ? sum : -1.0f;
+    }
+  }
+  int distinct = 0;
+  float zs[S < 2 ? 2 : S];
+  if (S < 2) zs[1] = neg_inf();
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const bool own = !(mass[s] < 0.0f);
+    zs[s] = own ? z[s] : neg_inf();
+    distinct += own ? 1 : 0;
+  }
+  if (K >= V && a.tail) {  // where every token is listed there is no other class
+    if (__reduce_add_sync(0xffffffffu, distinct) >= V) st.r = 0.0f;
+  }
+
+  float xs[E];
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const int v = u * 32 + lane;
+    float part[kV];
+    unpack(v < span.vecs ? hvec[v] : void_vec<T>(), part);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) xs[u * kV + e] = part[e];
+  }
+  const float edge_x = edge >= 0 ? logit_at<T>(held, edge) : neg_inf();
+  const SoftState rest = soft_of_warp<false>(xs, edge_x, c);
+  const SoftState all = soft_merge(rest, soft_of_warp<false>(zs, neg_inf(), c), c);
+  st.m = all.m;
+  st.ln_s = all.m == neg_inf() ? neg_inf() : logf(all.s);
+  st.rest_m = rest.m;
+  st.ln_rest = rest.m == neg_inf() ? neg_inf() : logf(rest.s);
+  const float loss = warp_loss(st, inv_t, [&](auto f) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) f(lnq[s], q[s], z[s]);
+  });
+  if (lane == 0) {
+    a.loss[row] = w * loss;
+    if (a.stats != nullptr) *reinterpret_cast<RowStats*>(a.stats + kStats * row) = st;
+  }
+  if (d == nullptr) return;
+
+  const RowGradient g = row_gradient(st, a.tail, inv_t, w);
+  const Unlisted f(g, c);
+  if (edge >= 0) logit_put(d, edge, g.none ? 0.0f : f(edge_x));
+  T* out = d + span.head;
+  const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const int v = u * 32 + lane;
+    if (v >= span.vecs) continue;
+    float ds[kV];
+#pragma unroll
+    for (int e = 0; e < kV; e += 2) {
+      f(xs[u * kV + e], xs[u * kV + e + 1], ds[e], ds[e + 1]);
+      if (g.none) ds[e] = ds[e + 1] = 0.0f;
+    }
+    if (aligned) {
+      store_vec(out + v * kV, ds);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kV; ++e) logit_put(out, v * kV + e, ds[e]);
+    }
+  }
+  if (g.none) return;
+  __syncwarp();
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+    if (!(mass[s] < 0.0f)) logit_put(d, at[s], listed_gradient(g, z[s], mass[s], c));
+}
+
+// ------------------------------------------------------------ a CTA or a cluster for a row
+struct CtaShared {
+  SoftState part[kMaxCluster];
+  int part_repeated[kMaxCluster];
+  SoftState warp_part[kWarps];
+  SoftState top;  // softmax state of the listed tokens
+  float total, r, shift;
+  int index[kTopMax];  // -1: empty slot (or one past the vocabulary)
+  float lnq[kTopMax], q[kTopMax], z[kTopMax];
+  float mass[kTopMax];  // q summed over the slots of the same token; below 0: not its first slot
+};
+static_assert(sizeof(CtaShared) % 4 == 0, "the slice follows, aligned");
+constexpr size_t kCtaShared = (sizeof(CtaShared) + 15) & ~size_t(15);
+
+// Masses of repeated tokens to the first slot of each, and the listed tokens' softmax state
+// (one warp).
+__device__ __forceinline__ void list_state(CtaShared& sh, int K, int lane, float c, bool repeated) {
+  float zs[kTopMax / 32];
+#pragma unroll
+  for (int s = 0; s < kTopMax / 32; ++s) {
+    const int j = s * 32 + lane;
+    zs[s] = neg_inf();
+    if (j >= K) continue;
+    const int at = sh.index[j];
+    float mass = at >= 0 ? sh.q[j] : -1.0f;
+    if (repeated && at >= 0) {
+      mass = 0.0f;
+      bool first = true;
+      for (int k = 0; k < K; ++k)
+        if (sh.index[k] == at) {
+          mass += sh.q[k];
+          if (k < j) first = false;
+        }
+      if (!first) mass = -1.0f;
+    }
+    sh.mass[j] = mass;
+    if (!(mass < 0.0f)) zs[s] = sh.z[j];
+  }
+  const SoftState top = soft_of_warp<false>(zs, neg_inf(), c);
+  if (lane == 0) sh.top = top;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillTopkArgs a, int C) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int kV = kVec<T>;
-  const int tid = threadIdx.x % G, group = threadIdx.x / G;
+  CtaShared& sh = *reinterpret_cast<CtaShared*>(smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int V = static_cast<int>(a.V), K = static_cast<int>(a.K);
-  const uint32_t rank = G > 32 && C > 1 ? cta_rank() : 0;
-  const int64_t row = G == 32 ? static_cast<int64_t>(blockIdx.x) * (kThreads / G) + group
-                              : static_cast<int64_t>(blockIdx.x) / C;
-  if (row >= a.outer * a.inner) return;  // whole warps of the warp form
+  const uint32_t rank = C > 1 ? cta_rank() : 0;
+  const int64_t row = blockIdx.x / static_cast<uint32_t>(C);
   const int64_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
   const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
   T* d = a.dlogits != nullptr
@@ -220,55 +383,83 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillTopkArgs 
              : nullptr;
 
   // This CTA's slice: vectors [v0, v1) between the row's 16-byte boundaries, the row's head with
-  // the first slice and its tail with the last; elements [from, to).
+  // the first slice and its tail with the last; n elements from `from`.
   const RowSpan span = row_span(x, V);
   const int per = (span.vecs + C - 1) / C;
   const int v0 = min(static_cast<int>(rank) * per, span.vecs), v1 = min(v0 + per, span.vecs);
   const int head = rank == 0 ? span.head : 0, tail = rank == C - 1 ? span.tail : 0;
-  const int from = span.head + v0 * kV - head, to = span.head + v1 * kV + tail;
-  const int n = to - from;
+  const int from = span.head + v0 * kV - head, vecs = v1 - v0, n = head + vecs * kV + tail;
 
   const float w = row_weight<T>(a, o, i);
   if (w == 0.0f) {  // the whole cluster
-    if (d != nullptr) map_row<T, G>(x + from, d + from, n, tid, true, NoSingle(), NoPair());
+    if (d != nullptr) map_row<T, kThreads>(x + from, d + from, n, tid, true, Nothing(), Nothing());
     if (tid == 0 && rank == 0) a.loss[row] = 0.0f;
     return;
   }
-  if (G > 32 && C > 1) cluster_arrive();  // shared memory may be written once all CTAs have started
+  if (C > 1) cluster_arrive();  // shared memory may be written once all CTAs have started
 
-  uint8_t* base = smem + group * group_smem(K, slice_bytes);
-  GroupShared& sh = *reinterpret_cast<GroupShared*>(base);
-  const List l = list_at(base, K);
-  T* buf = reinterpret_cast<T*>(base + ((list_smem(K) + 15) & ~size_t(15)));
-  T* held = buf + (kV - head) % kV;  // held[e] is element from + e; vectors keep their alignment
+  T* held = reinterpret_cast<T*>(smem + kCtaShared) + (kV - head) % kV;  // element from + e: held[e]
   const uint4* vec = reinterpret_cast<const uint4*>(x + span.head) + v0;
   uint4* hvec = reinterpret_cast<uint4*>(held + head);
-  const int vecs = v1 - v0;
-  for (int v = tid; v < vecs; v += G)
+  for (int v = tid; v < vecs; v += kThreads)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hvec + v)), "l"(vec + v)
                  : "memory");
-  for (int e = tid; e < head + tail; e += G) {
-    const int at = e < head ? e : n - tail + (e - head);
-    held[at] = x[from + at];
+  const int edge = tid < head ? tid : tid - head < tail ? n - tail + tid - head : -1;
+  if (edge >= 0) held[edge] = x[from + edge];
+  int at = -1;  // this thread's slot: its token, where it lies in the slice
+  bool bad = false;
+  if (tid < K) {
+    at = slot_token(a.index[o * a.i_strides[0] + i * a.i_strides[1] + tid * a.i_strides[2]], V);
+    const float t = a.teacher[o * a.t_strides[0] + i * a.t_strides[1] + tid * a.t_strides[2]];
+    sh.lnq[tid] = at >= 0 ? t : neg_inf();
+    bad = at == V;
+    if (bad) at = -1;
+    sh.z[tid] = at >= 0 ? logit_at<T>(x, at) : neg_inf();
+    sh.index[tid] = at;
+    at = at >= from && at < from + n ? at - from : -1;
   }
   const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
-  load_list<T, G>(a, x, o, i, tid, c, sh, l);
   asm volatile("cp.async.wait_all;" ::: "memory");
-  group_sync<G>();
-  for (int j = tid; j < K; j += G) {
-    const int at = l.index[j];
-    if (at >= from && at < to) logit_put(held, at - from, neg_inf());
+  bad = __syncthreads_or(bad);
+  if (at >= 0) put_slot(held, at, tid);
+  if (warp == kWarps - 1) {  // (the slots are the first warps')
+    float m = neg_inf(), shift = 0.0f, total = 0.0f;
+    if (!a.tail) {
+      for (int j = lane; j < K; j += 32) m = max_nan(m, sh.lnq[j]);
+      m = warp_max(m);
+      if (m != neg_inf()) {
+        float s = 0.0f;
+        for (int j = lane; j < K; j += 32) s += expf(sh.lnq[j] - m);
+        shift = m + logf(warp_sum(s));
+      }
+    }
+    for (int j = lane; j < K; j += 32) {
+      const float l = sh.lnq[j] - shift, q = expf(l);
+      sh.lnq[j] = l;
+      sh.q[j] = q;
+      total += q;
+    }
+    total = warp_sum(total);
+    if (lane == 0) {
+      sh.total = bad ? quiet_nan() : total;  // a token past the vocabulary: NaN throughout
+      sh.r = a.tail ? max_nan(0.0f, 1.0f - total) : 0.0f;
+      sh.shift = shift;
+    }
+    __syncwarp();
+    list_state(sh, K, lane, c, false);
   }
-  group_sync<G>();
+  __syncthreads();
+  bool repeated = __syncthreads_or(at >= 0 && get_slot(held, at) != tid);
+  if (at >= 0) logit_put(held, at, neg_inf());
+  __syncthreads();
 
   SoftState rest = soft_empty();
-  for (int e = tid; e < head + tail; e += G)
-    soft_add(rest, logit_at<T>(held, e < head ? e : n - tail + (e - head)), c);
-  for (int b = 0; b < vecs; b += G * kUnroll) {
+  if (edge >= 0) soft_add(rest, logit_at<T>(held, edge), c);
+  for (int b = 0; b < vecs; b += kThreads * kUnroll) {
     float xs[kUnroll * kV];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int v = b + u * G + tid;
+      const int v = b + u * kThreads + tid;
       float part[kV];
       unpack(v < vecs ? hvec[v] : void_vec<T>(), part);
 #pragma unroll
@@ -280,94 +471,96 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillTopkArgs 
     if (!(m <= rest.m)) soft_raise(rest, max_nan(m, rest.m), c);
     if (rest.m != neg_inf()) soft_sum<false>(rest, xs, c);
   }
-  rest = soft_warp(rest, c);
-  if (G > 32) {
-    if ((threadIdx.x & 31) == 0) sh.warp_part[threadIdx.x >> 5] = rest;
-    __syncthreads();
-    rest = sh.warp_part[0];
-#pragma unroll
-    for (int k = 1; k < kWarps; ++k) rest = soft_merge(rest, sh.warp_part[k], c);
-    if (C > 1) {
-      cluster_wait();
-      if (tid < C) {
-        const uint32_t at = peer_smem(&sh.part[rank], tid);
-        peer_store(at, rest.m);
-        peer_store(at + 4, rest.s);
-      }
-      cluster_arrive();
-      cluster_wait();
-      rest = {sh.part[0].m, sh.part[0].s, 0.0f};
-      for (int k = 1; k < C; ++k) rest = soft_merge(rest, {sh.part[k].m, sh.part[k].s, 0.0f}, c);
+  {
+    const float m = warp_max(rest.m);
+    if (m != neg_inf()) soft_raise(rest, m, c);
+    rest.s = warp_sum(rest.s);
+  }
+  if (lane == 0) sh.warp_part[warp] = rest;
+  __syncthreads();
+  if (C > 1) cluster_wait();
+  if (warp == 0) {  // the CTA's state, to every CTA of the cluster
+    SoftState mine = lane < kWarps ? sh.warp_part[lane] : soft_empty();
+    const float m = warp_max(mine.m);
+    if (m != neg_inf()) soft_raise(mine, m, c);
+    mine.s = warp_sum(mine.s);
+    if (C == 1 && lane == 0) {
+      sh.part[0] = mine;
+      sh.part_repeated[0] = repeated ? 1 : 0;
+    } else if (C > 1 && lane < C) {
+      const uint32_t to = peer_smem(&sh.part[rank], lane);
+      peer_store(to, m);
+      peer_store(to + 4, mine.s);
+      peer_store(peer_smem(&sh.part_repeated[rank], lane), __int_as_float(repeated ? 1 : 0));
     }
   }
-  rest.a = 0.0f;
+  if (C > 1) {
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  rest = {sh.part[0].m, sh.part[0].s, 0.0f};
+  repeated = sh.part_repeated[0] != 0;
+  for (int k = 1; k < C; ++k) {
+    rest = soft_merge(rest, {sh.part[k].m, sh.part[k].s, 0.0f}, c);
+    repeated |= sh.part_repeated[k] != 0;
+  }
+  if (repeated) {
+    __syncthreads();
+    if (warp == 0) list_state(sh, K, lane, c, true);
+    __syncthreads();
+  }
   const SoftState all = soft_merge(rest, {sh.top.m, sh.top.s, 0.0f}, c);
-  const bool none = all.m == neg_inf(), rest_none = rest.m == neg_inf();
-  const float ln_s = none ? neg_inf() : logf(all.s);
-  const float ln_rest = rest_none ? neg_inf() : logf(rest.s);
-
-  if (rank == 0 && tid < 32) {
-    float loss = 0.0f;
-    for (int j = tid; j < K; j += 32) {
-      const float q = l.q[j], z = l.z[j];
-      const float lp = none || z == neg_inf() ? neg_inf() : (z - all.m) * inv_t - ln_s;
-      if (!(q <= 0.0f)) loss = fmaf(q, l.lnq[j] - lp, loss);
-    }
-    loss = warp_sum(loss);
-    if (tid == 0) {
-      if (sh.r > 0.0f) {
-        const float ls = rest_none ? neg_inf() : (rest.m - all.m) * inv_t + ln_rest - ln_s;
-        loss = fmaf(sh.r, logf(sh.r) - ls, loss);
-      }
-      a.loss[row] = sh.total != sh.total ? quiet_nan() : w * loss;
-      if (a.stats != nullptr) {
-        a.stats[4 * row] = all.m;
-        a.stats[4 * row + 1] = ln_s;
-        a.stats[4 * row + 2] = rest.m;
-        a.stats[4 * row + 3] = ln_rest;
-      }
+  RowStats st;
+  st.m = all.m;
+  st.ln_s = all.m == neg_inf() ? neg_inf() : logf(all.s);
+  st.rest_m = rest.m;
+  st.ln_rest = rest.m == neg_inf() ? neg_inf() : logf(rest.s);
+  st.total = sh.total;
+  st.r = sh.r;
+  st.shift = sh.shift;
+  st.repeated = repeated ? 1.0f : 0.0f;
+  if (rank == 0 && warp == 0) {
+    const float loss = warp_loss(st, inv_t, [&](auto f) {
+      for (int j = lane; j < K; j += 32) f(sh.lnq[j], sh.q[j], sh.z[j]);
+    });
+    if (lane == 0) {
+      a.loss[row] = w * loss;
+      if (a.stats != nullptr) *reinterpret_cast<RowStats*>(a.stats + kStats * row) = st;
     }
   }
   if (d == nullptr) return;
 
-  const RowGradient g = row_gradient(a, sh, all.m, ln_s, rest.m, ln_rest, w);
-  auto dense = [&](float v) { return ex2(fmaf(v - g.m, c, g.shift)) * g.coef; };
-  const F2 nm2 = f2(-g.m, -g.m), c2 = f2(c, c), shift2 = f2(g.shift, g.shift), coef2 = f2(g.coef, g.coef);
-  auto pair = [&](float x0, float x1, float& d0, float& d1) {
-    float y0, y1;
-    f2_split(f2_fma(f2_add(f2(x0, x1), nm2), c2, shift2), y0, y1);
-    f2_split(f2_mul(f2(ex2(y0), ex2(y1)), coef2), d0, d1);
-  };
+  const RowGradient g = row_gradient(st, a.tail, inv_t, w);
+  const Unlisted f(g, c);
   T* out = d + from + head;
   if ((reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
-    for (int e = tid; e < head + tail; e += G) {
-      const int at = e < head ? e : n - tail + (e - head);
-      logit_put(d, from + at, g.none ? 0.0f : dense(logit_at<T>(held, at)));
-    }
-    for (int v = tid; v < vecs; v += G) {
+    if (edge >= 0) logit_put(d, from + edge, g.none ? 0.0f : f(logit_at<T>(held, edge)));
+    for (int v = tid; v < vecs; v += kThreads) {
       float xs[kV], ds[kV];
       unpack(hvec[v], xs);
 #pragma unroll
-      for (int e = 0; e < kV; e += 2) pair(xs[e], xs[e + 1], ds[e], ds[e + 1]);
-      if (g.none) {
-#pragma unroll
-        for (int e = 0; e < kV; ++e) ds[e] = 0.0f;
+      for (int e = 0; e < kV; e += 2) {
+        f(xs[e], xs[e + 1], ds[e], ds[e + 1]);
+        if (g.none) ds[e] = ds[e + 1] = 0.0f;
       }
       store_vec(out + static_cast<int64_t>(v) * kV, ds);
     }
   } else {  // x and d lie differently in their vectors
-    for (int e = tid; e < n; e += G)
-      logit_put(d, from + e, g.none ? 0.0f : dense(logit_at<T>(held, e)));
+    for (int e = tid; e < n; e += kThreads)
+      logit_put(d, from + e, g.none ? 0.0f : f(logit_at<T>(held, e)));
   }
   if (g.none) return;
-  group_sync<G>();
-  write_listed<T, G>(g, l, K, V, d, from, to, tid, c);
+  __syncthreads();
+  if (at >= 0 && !(sh.mass[tid] < 0.0f))
+    logit_put(d, from + at, listed_gradient(g, sh.z[tid], sh.mass[tid], c));
 }
 
+// --------------------------------------------------- the gradient from the forward's statistics
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads) distill_topk_bwd_kernel(DistillTopkArgs a, int pieces,
                                                                     int piece) {
-  extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x % G, group = threadIdx.x / G;
   const int V = static_cast<int>(a.V), K = static_cast<int>(a.K);
   const uint32_t unit = blockIdx.x * (kThreads / G) + group;
@@ -380,28 +573,37 @@ __global__ void __launch_bounds__(kThreads) distill_topk_bwd_kernel(DistillTopkA
   T* d = static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1];
   const float w = row_weight<T>(a, o, i);
   if (w == 0.0f) {
-    map_row<T, G>(x + from, d + from, n, tid, true, NoSingle(), NoPair());
+    map_row<T, G>(x + from, d + from, n, tid, true, Nothing(), Nothing());
     return;
   }
-  uint8_t* base = smem + group * group_smem(K, 0);
-  GroupShared& sh = *reinterpret_cast<GroupShared*>(base);
-  const List l = list_at(base, K);
-  const float c = kLog2e / a.temperature;
-  load_list<T, G>(a, x, o, i, tid, c, sh, l);
-  const float* st = a.stats + 4 * row;
+  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
+  const RowStats st = *reinterpret_cast<const RowStats*>(a.stats + kStats * row);
   const float up = a.g_loss.p[o * a.g_loss.strides[0] + i * a.g_loss.strides[1]];
-  const RowGradient g = row_gradient(a, sh, st[0], st[1], st[2], st[3], w * up);
-  auto dense = [&](float v) { return ex2(fmaf(v - g.m, c, g.shift)) * g.coef; };
-  const F2 nm2 = f2(-g.m, -g.m), c2 = f2(c, c), shift2 = f2(g.shift, g.shift), coef2 = f2(g.coef, g.coef);
-  auto pair = [&](float x0, float x1, float& d0, float& d1) {
-    float y0, y1;
-    f2_split(f2_fma(f2_add(f2(x0, x1), nm2), c2, shift2), y0, y1);
-    f2_split(f2_mul(f2(ex2(y0), ex2(y1)), coef2), d0, d1);
-  };
-  map_row<T, G>(x + from, d + from, n, tid, g.none, dense, pair);
+  const RowGradient g = row_gradient(st, a.tail, inv_t, w * up);
+  const Unlisted f(g, c);
+  map_row<T, G>(x + from, d + from, n, tid, g.none, f, f);
   if (g.none) return;
-  group_sync<G>();
-  write_listed<T, G>(g, l, K, V, d, from, from + n, tid, c);
+  if (G == 32) __syncwarp();
+  else __syncthreads();
+  // the listed tokens of this piece, over what the formula for the others left there
+  const int64_t* index = a.index + o * a.i_strides[0] + i * a.i_strides[1];
+  const float* teacher = a.teacher + o * a.t_strides[0] + i * a.t_strides[1];
+  for (int j = tid; j < K; j += G) {
+    const int64_t at = index[j * a.i_strides[2]];
+    if (at < from || at >= from + n) continue;
+    float mass = expf(teacher[j * a.t_strides[2]] - st.shift);
+    if (st.repeated != 0.0f) {
+      bool first = true;
+      mass = 0.0f;
+      for (int k = 0; first && k < K; ++k)
+        if (index[k * a.i_strides[2]] == at) {
+          mass += expf(teacher[k * a.t_strides[2]] - st.shift);
+          first = k >= j;
+        }
+      if (!first) continue;
+    }
+    logit_put(d, at, listed_gradient(g, logit_at<T>(x, at), mass, c));
+  }
 }
 
 int launch_check(const char* what, cudaError_t e) {
@@ -413,36 +615,19 @@ int launch_check(const char* what, cudaError_t e) {
   return BDH_OK;
 }
 
-template <typename T, int G>
-int launch_forward(const DistillTopkArgs& a, int cluster, cudaStream_t stream) {
-  const int64_t rows = a.outer * a.inner;
-  constexpr int kGroups = kThreads / G;
-  // a slice's vectors, and one more for the row's head and one for its tail
-  const size_t slice = (static_cast<size_t>((a.V / kVec<T> + cluster - 1) / cluster) + 2) * 16;
-  const size_t smem = kGroups * group_smem(static_cast<int>(a.K), slice);
-  auto* kern = distill_topk_kernel<T, G>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem));
-    if (e != cudaSuccess) return launch_check("distill_topk shared memory", e);
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(G == 32 ? (rows + kGroups - 1) / kGroups : rows * cluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return launch_check("distill_topk launch", cudaLaunchKernelEx(&cfg, kern, a, cluster, slice));
+template <typename T, int E>
+int launch_short(const DistillTopkArgs& a, cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>((a.outer * a.inner + kWarps - 1) / kWarps);
+  if (a.K <= 32) distill_short_kernel<T, E, 1><<<grid, kThreads, 0, stream>>>(a);
+  else distill_short_kernel<T, E, kTopMax / 32><<<grid, kThreads, 0, stream>>>(a);
+  return launch_check("distill_topk launch", cudaSuccess);
 }
 
 template <typename T>
 int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
-  if (a.V <= 1024) return launch_forward<T, 32>(a, 1, stream);
+  if (a.V <= 256) return launch_short<T, 8>(a, stream);
+  if (a.V <= 512) return launch_short<T, 16>(a, stream);
+  if (a.V <= kShort) return launch_short<T, 32>(a, stream);
   int dev = 0;
   cudaGetDevice(&dev);
   const int64_t rows = a.outer * a.inner, bytes = a.V * static_cast<int64_t>(sizeof(T));
@@ -455,23 +640,41 @@ int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
     set_error("distill_topk: too many rows for this vocabulary");
     return BDH_ERR_INVALID;
   }
-  return launch_forward<T, kThreads>(a, cluster, stream);
+  // a slice's vectors, and one more for the row's head and one for its tail
+  const size_t smem = kCtaShared + (static_cast<size_t>((a.V / kVec<T> + cluster - 1) / cluster) + 2) * 16;
+  auto* kern = distill_topk_kernel<T>;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(smem));
+    if (e != cudaSuccess) return launch_check("distill_topk shared memory", e);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  return launch_check("distill_topk launch", cudaLaunchKernelEx(&cfg, kern, a, cluster));
 }
 
 template <typename T>
 int backward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
-  const size_t lists = group_smem(static_cast<int>(a.K), 0);
-  if (a.V <= 1024) {
+  if (a.V <= kShort) {
     const unsigned grid = static_cast<unsigned>((rows + kWarps - 1) / kWarps);
-    distill_topk_bwd_kernel<T, 32><<<grid, kThreads, kWarps * lists, stream>>>(a, 1, static_cast<int>(a.V));
+    distill_topk_bwd_kernel<T, 32><<<grid, kThreads, 0, stream>>>(a, 1, static_cast<int>(a.V));
   } else {
     const int64_t pieces = (a.V + kPiece - 1) / kPiece;
     if (rows * pieces >= int64_t(1) << 31) {
       set_error("distill_topk_bwd: too many rows for this vocabulary");
       return BDH_ERR_INVALID;
     }
-    distill_topk_bwd_kernel<T, kThreads><<<static_cast<unsigned>(rows * pieces), kThreads, lists, stream>>>(
+    distill_topk_bwd_kernel<T, kThreads><<<static_cast<unsigned>(rows * pieces), kThreads, 0, stream>>>(
         a, static_cast<int>(pieces), kPiece);
   }
   return launch_check("distill_topk_bwd launch", cudaSuccess);

@@ -355,7 +355,7 @@ struct DistillTopkArgs {
   float temperature = 1.0f;
   int tail = 0;
   float* loss = nullptr;   // one per row; null in the backward form
-  float* stats = nullptr;  // 4 per row (written by the forward when not null, read by the backward)
+  float* stats = nullptr;  // 8 per row (written by the forward when not null, read by the backward)
   void* dlogits = nullptr;  // null: the loss alone
   int64_t d_strides[2] = {0, 0};
   RowGrad g_loss;  // backward form only

@@ -255,6 +255,31 @@ __device__ __forceinline__ void soft_sum(SoftState& st, const float (&x)[N], flo
   }
 }
 
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+// Softmax state of a row that a warp holds N elements a lane of: the maximum first, then the sums.
+template <bool ENTROPY, int N>
+__device__ __forceinline__ SoftState soft_of_warp(const float (&x)[N], float edge, float c) {
+  float m = edge;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = max_nan(m, x[i]);
+  SoftState st = {warp_max(m), 0.0f, 0.0f};
+  if (st.m == neg_inf()) return st;
+  soft_sum<ENTROPY>(st, x, c);
+  const float t = max_nan((edge - st.m) * c, kExpFloor), e = ex2(t);
+  st.s = warp_sum(st.s + e);
+  if (ENTROPY) st.a = warp_sum(fmaf(e, t, st.a));
+  return st;
+}
+
 // Order of a row's top list: larger values first, an equal value's lower index first; -0 equals
 // +0, and NaN comes before everything (as torch.sort places it). Larger key, earlier place;
 // key 0 stands for "no element" and is below every element's, ~0 is above.

@@ -38,6 +38,46 @@ constexpr int candidate_room(int K) {
   return (K + top_slack(K)) * kVec<T> + 16;
 }
 
+// A key that at least K of a group's items are at or above, and as a rule few more, by bisection:
+// first over the values' keys, [lo, hi] holding all of them, then, where more items share the value
+// found than may be taken, over the index up to which they count. from(v): items with value key >= v;
+// tied(v, i): items with value key v and an index up to i.
+template <typename From, typename Tied>
+__device__ __forceinline__ uint64_t list_bound(int K, uint32_t lo, uint32_t hi, int V, From from,
+                                               Tied tied) {
+  const int most = K + top_slack(K);
+  int n = 0x7fffffff;
+  ++hi;  // at least K items from lo, fewer than K from hi
+  while (hi - lo > 1 && n > most) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    const int now = from(mid);
+    if (now >= K) {
+      lo = mid;
+      n = now;
+    } else {
+      hi = mid;
+    }
+  }
+  uint32_t last = 0xffffffffu;
+  if (n > most) {
+    const int above = from(lo + 1);
+    uint32_t left = 0, right = static_cast<uint32_t>(V);
+    n = 0x7fffffff;
+    while (left < right && n > most - above) {
+      const uint32_t mid = left + (right - left) / 2;
+      const int now = tied(lo, mid);
+      if (now >= K - above) {
+        right = mid;
+        n = now;
+      } else {
+        left = mid + 1;
+      }
+    }
+    last = right;
+  }
+  return (static_cast<uint64_t>(lo) << 32) | (0xffffffffu - last);
+}
+
 struct ForwardPlan {
   int cells, cell_batches;  // per thread; batches in a cell
   int cluster;
@@ -48,14 +88,14 @@ struct Group;
 template <>
 struct Group<32> {
   static __device__ __forceinline__ void sync() { __syncwarp(); }
-  static __device__ __forceinline__ int count(bool p, int*) {
+  static __device__ __forceinline__ int count(bool p) {
     return __popc(__ballot_sync(0xffffffffu, p));
   }
 };
 template <>
 struct Group<kThreads> {
   static __device__ __forceinline__ void sync() { __syncthreads(); }
-  static __device__ __forceinline__ int count(bool p, int*) { return __syncthreads_count(p); }
+  static __device__ __forceinline__ int count(bool p) { return __syncthreads_count(p); }
 };
 
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
@@ -73,7 +113,7 @@ struct GroupShared {
   uint64_t best[kWarps];
   SoftState warp_part[kWarps];
   uint32_t lo[kWarps], hi[kWarps];
-  int found;
+  int found, queued;
 };
 
 template <typename T, int G>
@@ -81,7 +121,7 @@ __host__ __device__ constexpr size_t group_smem(int K, int cells, int cluster) {
   size_t n = sizeof(GroupShared);
   if (K > 0) {
     n += (static_cast<size_t>(cells) * G * sizeof(float) + 7) & ~size_t(7);
-    n += static_cast<size_t>(candidate_room<T>(K)) * sizeof(uint64_t);
+    n += static_cast<size_t>(candidate_room<T>(K)) * (sizeof(uint64_t) + sizeof(int));
     n += static_cast<size_t>(cluster) * K * sizeof(uint64_t);
   }
   return (n + 15) & ~size_t(15);
@@ -103,6 +143,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
   uint64_t* cand = reinterpret_cast<uint64_t*>(
       base + sizeof(GroupShared) + ((static_cast<size_t>(plan.cells) * G * 4 + 7) & ~size_t(7)));
   uint64_t* lists = cand + candidate_room<T>(K);
+  int* queue = reinterpret_cast<int*>(lists + C * K);  // cells to look at again
   const int64_t rows = a.outer * a.inner;
   const int64_t row = G == 32 ? static_cast<int64_t>(blockIdx.x) * (kThreads / G) + group
                               : static_cast<int64_t>(blockIdx.x) / C;
@@ -192,9 +233,9 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
     // A bound below K elements of the slice: value key lo, and an index among elements of that value.
     const uint32_t key = any ? value_key(own_max) : 0u;
     at_most = min(at_most, V - 1);
-    if (tid == 0) sh.found = 0;
+    if (tid == 0) sh.found = sh.queued = 0;
     uint64_t bound = 0;
-    if (Gr::count(any, nullptr) >= K) {
+    if (Gr::count(any) >= K) {
       uint32_t lo = __reduce_min_sync(0xffffffffu, any ? key : 0xffffffffu);
       uint32_t hi = __reduce_max_sync(0xffffffffu, key);
       if (G > 32) {
@@ -208,39 +249,11 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
           hi = max(hi, sh.hi[w]);
         }
       }
-      ++hi;  // at least K maxima at or above lo, fewer than K at or above hi
-      int above = 0, at_lo = G;
-      while (hi - lo > 1 && at_lo > K + top_slack(K)) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        const int n = Gr::count(key >= mid, nullptr);
-        if (n >= K) {
-          lo = mid;
-          at_lo = n;
-        } else {
-          hi = mid;
-          above = n;
-        }
-      }
-      uint32_t last = 0xffffffffu;  // of equal values, those up to this index
-      if (hi - lo == 1 && at_lo > K + top_slack(K)) {
-        // count again: the search may have ended on its first interval
-        above = Gr::count(key > lo, nullptr);
-        uint32_t left = 0, right = static_cast<uint32_t>(V);  // fewer than wanted at left - 1, enough at right
-        int n = G;
-        while (left < right && n > K - above + top_slack(K)) {
-          const uint32_t mid = left + (right - left) / 2;
-          const int now = Gr::count(key == lo && static_cast<uint32_t>(at_most) <= mid, nullptr);
-          if (now >= K - above) {
-            right = mid;
-            n = now;
-          } else {
-            left = mid + 1;
-          }
-        }
-        last = right;
-      }
-      bound = (static_cast<uint64_t>(lo) << 32) |
-              (last == 0xffffffffu ? 0u : 0xffffffffu - last);
+      bound = list_bound(
+          K, lo, hi, V, [&](uint32_t v) { return Gr::count(key >= v); },
+          [&](uint32_t v, uint32_t at) {
+            return Gr::count(key == v && static_cast<uint32_t>(at_most) <= at);
+          });
     }
     Gr::sync();  // sh.found is set
     const uint32_t bound_value = static_cast<uint32_t>(bound >> 32);
@@ -254,21 +267,31 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
     };
     if (edge >= 0) offer(edge_x, edge);
     if (value_key(own_max) >= bound_value) {
+      const uint32_t last = 0xffffffffu - static_cast<uint32_t>(bound);
       for (int q = 0; q < cell; ++q) {
-        if (value_key(cells[q * G + tid]) < bound_value) continue;
-        const int b0 = v0 + q * plan.cell_batches * G * U;
-        for (int b = b0; b < min(b0 + plan.cell_batches * G * U, v1); b += G) {
-          const int v = b + tid;
-          if (v >= v1) break;
-          float part[kV];
-          unpack(__ldg(vec + v), part);
-#pragma unroll
-          for (int e = 0; e < kV; ++e) offer(part[e], span.head + v * kV + e);
-        }
+        const uint32_t k = value_key(cells[q * G + tid]);
+        const uint32_t first = span.head + (v0 + q * plan.cell_batches * G * U + tid) * kV;
+        if (k < bound_value || (k == bound_value && first > last)) continue;
+        const int n = atomicAdd(&sh.queued, 1);
+        if (n < room) queue[n] = q * G + tid;
       }
     }
     Gr::sync();
-    const int found = sh.found;
+    // All threads on the queued cells' vectors, one each, so that their loads are under way together.
+    const int in_cell_vecs = plan.cell_batches * U;
+    if (sh.queued <= room) {
+      for (int n = tid; n < sh.queued * in_cell_vecs; n += G) {
+        const int item = queue[n / in_cell_vecs], q = item / G;
+        const int v = v0 + (q * in_cell_vecs + n % in_cell_vecs) * G + item % G;
+        if (v >= v1) continue;
+        float part[kV];
+        unpack(__ldg(vec + v), part);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) offer(part[e], span.head + v * kV + e);
+      }
+    }
+    Gr::sync();
+    const int found = sh.queued <= room ? sh.found : room + 1;
     uint64_t* list = C > 1 ? lists + rank * K : lists;  // this slice's K largest in order
     for (int k = tid; k < K; k += G) list[k] = 0;
     Gr::sync();

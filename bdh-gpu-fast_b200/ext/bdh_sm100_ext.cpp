@@ -713,7 +713,7 @@ std::tuple<at::Tensor, MaybeTensor, MaybeTensor> distill_topk(
   at::Tensor loss = at::empty(x.lead, f32);
   MaybeTensor d, stats;
   if (want_grad) d = at::empty(logits.sizes(), x.t.options());
-  if (want_stats) stats = at::empty({x.rows(), 4}, f32);
+  if (want_stats) stats = at::empty({x.rows(), 8}, f32);
   const int64_t ds[2] = {x.inner * x.V, x.V};
   check_rc(bdh_distill_topk(x.t.data_ptr(), dtype_code(x.t), x.strides,
                             l.index.t.data_ptr<int64_t>(), l.index.strides,
@@ -735,7 +735,7 @@ at::Tensor distill_topk_bwd(const at::Tensor& logits, const at::Tensor& index,
   const DistillList l = distill_list(x, index, teacher, weight, temperature);
   const std::optional<BesideRows> g = per_row(x, g_loss, "g_loss");
   if (!stats.is_cuda() || stats.device() != x.t.device() || stats.scalar_type() != at::kFloat ||
-      stats.numel() != 4 * x.rows())
+      stats.numel() != 8 * x.rows())
     TORCH_CHECK_VALUE(false, "distill_topk_bwd: bad stats");
   const at::Tensor st = stats.contiguous();
   at::Tensor d = at::empty(logits.sizes(), x.t.options());

@@ -188,7 +188,7 @@ def distill_topk(logits, teacher_index, teacher_logprob, weight=None, temperatur
     k, (idx, si), (val, sv), (w, sw) = _list(x, teacher_index, teacher_logprob, weight, temperature)
     lib, dev = _lib(), x.t.device
     loss = torch.empty(x.lead, dtype=torch.float32, device=dev)
-    stats = torch.empty(x.rows, 4, dtype=torch.float32, device=dev) if want_stats else None
+    stats = torch.empty(x.rows, 8, dtype=torch.float32, device=dev) if want_stats else None
     d, ds = x.grad() if want_grad else (None, (_i64 * 2)(0, 0))
     with torch.cuda.device(dev):
         rc = lib.bdh_distill_topk(
@@ -205,7 +205,7 @@ def distill_topk_bwd(logits, teacher_index, teacher_logprob, weight, stats, g_lo
     x = _Rows(logits, "distill_topk_bwd")
     k, (idx, si), (val, sv), (w, sw) = _list(x, teacher_index, teacher_logprob, weight, temperature)
     g, sg = x.per_row(g_loss, "g_loss")
-    if stats.device != x.t.device or stats.dtype != torch.float32 or stats.numel() != 4 * x.rows:
+    if stats.device != x.t.device or stats.dtype != torch.float32 or stats.numel() != 8 * x.rows:
         raise ValueError("distill_topk_bwd: bad stats")
     stats = stats.contiguous()
     d, ds = x.grad()

@@ -427,7 +427,7 @@ int bdh_token_logprobs_bwd(const void* logits, int dtype, const int64_t l_stride
  * When the list holds every token there is no other class (r = 0). A row with no logit above -inf
  * has loss +inf and gradient 0.
  * bdh_distill_topk writes the loss per row and, with dlogits, the gradient of the sum of the losses
- * in the same call (the logits are read from memory once); stats (4 floats per row, may be null) is
+ * in the same call (the logits are read from memory once); stats (8 floats per row, 16-byte aligned, may be null) is
  * what bdh_distill_topk_bwd reads, which multiplies the gradient of each row by g_loss. A row is
  * held in the shared memory of up to 8 CTAs, so V is at most BDH_DISTILL_VOCAB_MAX.
  */
