@@ -210,17 +210,6 @@ __device__ __forceinline__ SoftState soft_merge(const SoftState& x, const SoftSt
   const float fx = ex2(dx), fy = ex2(dy);
   return {m, fmaf(x.s, fx, y.s * fy), fmaf(fx, fmaf(dx, x.s, x.a), fy * fmaf(dy, y.s, y.a))};
 }
-__device__ __forceinline__ SoftState soft_warp(SoftState st, float c) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const SoftState other = {__shfl_xor_sync(0xffffffffu, st.m, o),
-                             __shfl_xor_sync(0xffffffffu, st.s, o),
-                             __shfl_xor_sync(0xffffffffu, st.a, o)};
-    st = soft_merge(st, other, c);
-  }
-  return st;
-}
-
 // Raise the state's maximum to m (not below it; NaN stays).
 __device__ __forceinline__ void soft_raise(SoftState& st, float m, float c) {
   const float d = max_nan((st.m - m) * c, kExpFloor);
@@ -264,6 +253,15 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
+}
+// The lanes' states as one.
+__device__ __forceinline__ SoftState soft_join(SoftState st, float c) {
+  const float m = warp_max(st.m);
+  if (m == neg_inf()) return soft_empty();
+  soft_raise(st, m, c);
+  st.s = warp_sum(st.s);
+  st.a = warp_sum(st.a);
+  return st;
 }
 // Softmax state of a row that a warp holds N elements a lane of: the maximum first, then the sums.
 template <bool ENTROPY, int N>

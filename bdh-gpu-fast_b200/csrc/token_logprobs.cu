@@ -26,6 +26,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kWarpTop = 16;     // longest list of the warp form: half of its threads' maxima
+constexpr int kWarpRow = 8192;   // longest row that a warp reads
+constexpr int kWarpRows = 16;    // rows for every SM from which a warp takes a row
 constexpr int kMaxCells = 48;    // cells per thread; longer rows put more batches into a cell
 constexpr int kMaxCluster = 8;
 
@@ -127,6 +129,162 @@ __host__ __device__ constexpr size_t group_smem(int K, int cells, int cluster) {
   return (n + 15) & ~size_t(15);
 }
 
+// A given token's logit, asked for before the row is read so that the two loads' latencies pass
+// under it.
+struct Token {
+  bool given, left_out;  // a token inside the vocabulary; the index that counts as none
+  float z;
+};
+template <typename T>
+__device__ __forceinline__ Token load_token(const TokenLogprobsArgs& a, const T* x, int64_t o, int64_t i) {
+  Token t = {false, false, 0.0f};
+  const int64_t at = a.tokens[o * a.t_strides[0] + i * a.t_strides[1]];
+  t.left_out = at == a.ignore_index;
+  t.given = !t.left_out && at >= 0 && at < a.V;
+  if (t.given) t.z = logit_at<T>(x, at);
+  return t;
+}
+
+// The row's figures from its softmax state (one thread); returns ln of the sum.
+__device__ __forceinline__ float ln_sum(const SoftState& st) {
+  return st.m == neg_inf() ? neg_inf() : logf(st.s);  // -inf: nothing above -inf in the row
+}
+__device__ __forceinline__ float logprob_of(float z, const SoftState& st, float ln_s, float inv_t) {
+  return st.m == neg_inf() ? neg_inf() : (z - st.m) * inv_t - ln_s;
+}
+__device__ __forceinline__ void write_figures(const TokenLogprobsArgs& a, int64_t row, const SoftState& st,
+                                              float ln_s, float inv_t, const Token& t) {
+  const bool none = st.m == neg_inf();
+  if (a.lse != nullptr) a.lse[row] = none ? neg_inf() : fmaf(st.m, inv_t, ln_s);
+  if (a.entropy != nullptr) a.entropy[row] = none ? 0.0f : ln_s - kLn2 * st.a / st.s;
+  if (a.stats != nullptr) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(st.m, ln_s);
+  if (a.tokens != nullptr)
+    a.logprob[row] = t.left_out ? 0.0f : t.given ? logprob_of(t.z, st, ln_s, inv_t) : quiet_nan();
+}
+
+// ------------------------------------------------------------------ a warp for a short row
+// Rows of at most kShort elements stay in registers (E elements a lane and one of the row's
+// unaligned ends): the maximum first, then the sums; for the list, the elements' keys. Lists up to
+// kWarpTop are bounded by the lanes' largest keys, where that leaves no more candidates than there is
+// room for; longer ones by the elements' own.
+constexpr int kShort = 1024;
+constexpr int kShortRoom = kTopMax + top_slack(kTopMax) + 1;
+
+template <typename T, int E, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_logprobs_short_kernel(TokenLogprobsArgs a) {
+  constexpr int kV = kVec<T>, kVecs = E / kV;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  if (row >= a.outer * a.inner) return;
+  const int64_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
+  const int V = static_cast<int>(a.V);
+  const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
+  const RowSpan span = row_span(x, V);
+  const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
+  uint4 w[kVecs];
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const int v = u * 32 + lane;
+    w[u] = v < span.vecs ? __ldg(vec + v) : void_vec<T>();
+  }
+  int edge = -1;  // this lane's element of the row's ends
+  if (lane < span.head) edge = lane;
+  if (lane >= 8 && lane - 8 < span.tail) edge = V - span.tail + lane - 8;
+  const float edge_x = edge >= 0 ? logit_at<T>(x, edge) : neg_inf();
+  Token tok = {false, true, 0.0f};
+  if (lane == 0 && a.tokens != nullptr) tok = load_token(a, x, o, i);
+  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
+  float xs[E];
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    float part[kV];
+    unpack(w[u], part);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) xs[u * kV + e] = part[e];
+  }
+  const SoftState st = soft_of_warp<true>(xs, edge_x, c);
+  const float ln_s = ln_sum(st);
+  if (lane == 0) write_figures(a, row, st, ln_s, inv_t, tok);
+  if (!TOP) return;
+
+  __shared__ uint64_t room[kWarps][kShortRoom];
+  __shared__ int found[kWarps];
+  uint64_t* cand = room[warp];
+  const int K = static_cast<int>(a.K);
+  auto index_of = [&](int u, int e) { return span.head + (u * 32 + lane) * kV + e; };
+  uint32_t keys[E], own = 0, own_at = 0xffffffffu;
+  const uint32_t edge_key = edge >= 0 ? value_key(edge_x) : 0u;
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      const uint32_t k = u * 32 + lane < span.vecs ? value_key(xs[u * kV + e]) : 0u;
+      keys[u * kV + e] = k;
+      if (k > own) {
+        own = k;
+        own_at = index_of(u, e);
+      }
+    }
+  if (edge_key > own) {
+    own = edge_key;
+    own_at = edge;
+  }
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, own);
+  uint64_t bound = 0;
+  bool by_element = true;
+  if (K <= kWarpTop && __popc(__ballot_sync(0xffffffffu, own != 0)) >= K) {
+    const uint32_t lo = __reduce_min_sync(0xffffffffu, own != 0 ? own : 0xffffffffu);
+    bound = list_bound(
+        K, lo, hi, V, [&](uint32_t v) { return __popc(__ballot_sync(0xffffffffu, own >= v)); },
+        [&](uint32_t v, uint32_t at) { return __popc(__ballot_sync(0xffffffffu, own == v && own_at <= at)); });
+    by_element = false;
+  }
+  auto above = [&](uint32_t k, int at) {
+    return k != 0 && ((static_cast<uint64_t>(k) << 32) | (0xffffffffu - static_cast<uint32_t>(at))) >= bound;
+  };
+  auto count = [&](auto in) {
+    int n = in(edge_key, edge) ? 1 : 0;
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+      for (int e = 0; e < kV; ++e) n += in(keys[u * kV + e], index_of(u, e)) ? 1 : 0;
+    return static_cast<int>(__reduce_add_sync(0xffffffffu, n));
+  };
+  if (!by_element) by_element = count(above) > kShortRoom;
+  if (by_element) {
+    bound = list_bound(
+        K, 1u, hi, V, [&](uint32_t v) { return count([&](uint32_t k, int) { return k >= v; }); },
+        [&](uint32_t v, uint32_t at) {
+          return count([&](uint32_t k, int j) { return k == v && static_cast<uint32_t>(j) <= at; });
+        });
+  }
+  if (lane == 0) found[warp] = 0;
+  __syncwarp();
+  auto offer = [&](uint32_t k, int at) {
+    if (!above(k, at)) return;
+    const int n = atomicAdd(&found[warp], 1);
+    if (n < kShortRoom) cand[n] = (static_cast<uint64_t>(k) << 32) | (0xffffffffu - static_cast<uint32_t>(at));
+  };
+  offer(edge_key, edge);
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+    for (int e = 0; e < kV; ++e) offer(keys[u * kV + e], index_of(u, e));
+  __syncwarp();
+  const int n = found[warp];
+  for (int j = lane; j < n; j += 32) {
+    const uint64_t mine = cand[j];
+    int place = 0;
+    for (int q = 0; q < n; ++q) place += cand[q] > mine ? 1 : 0;
+    if (place < K) {
+      a.top_index[row * K + place] = key_index(mine);
+      a.top_logprob[row * K + place] =
+          logprob_of(key_value(static_cast<uint32_t>(mine >> 32)), st, ln_s, inv_t);
+    }
+  }
+}
+
+// ------------------------------------------- a warp, a CTA or a cluster for longer rows
 template <typename T, int G, int U, bool TOP>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsArgs a,
                                                                   ForwardPlan plan) {
@@ -152,6 +310,8 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
   const int64_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
   const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
   const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
+  Token tok = {false, true, 0.0f};
+  if (tid == 0 && rank == 0 && a.tokens != nullptr) tok = load_token(a, x, o, i);
 
   // This CTA's slice of the vectors; the row's head goes with the first slice, its tail with the last.
   const RowSpan span = row_span(x, V);
@@ -220,13 +380,11 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
   if (TOP && in_cell > 0) cells[cell++ * G + tid] = cell_max;
   const float own_max = st.m;
 
-  st = soft_warp(st, c);
+  st = soft_join(st, c);
   if (G > 32) {
     if ((threadIdx.x & 31) == 0) sh.warp_part[threadIdx.x >> 5] = st;
     __syncthreads();
-    st = sh.warp_part[0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) st = soft_merge(st, sh.warp_part[w], c);
+    st = soft_join((threadIdx.x & 31) < kWarps ? sh.warp_part[threadIdx.x & 31] : soft_empty(), c);
   }
 
   if (TOP) {
@@ -350,23 +508,8 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
     for (int r = 1; r < C; ++r) st = soft_merge(st, sh.part[r], c);
   }
 
-  const bool none = st.m == neg_inf();  // nothing above -inf in the row
-  const float ln_s = none ? neg_inf() : logf(st.s);
-  if (tid == 0) {
-    if (a.lse != nullptr) a.lse[row] = none ? neg_inf() : fmaf(st.m, inv_t, ln_s);
-    if (a.entropy != nullptr) a.entropy[row] = none ? 0.0f : ln_s - kLn2 * st.a / st.s;
-    if (a.stats != nullptr) {
-      a.stats[2 * row] = st.m;
-      a.stats[2 * row + 1] = ln_s;
-    }
-    if (a.tokens != nullptr) {
-      const int64_t tok = a.tokens[o * a.t_strides[0] + i * a.t_strides[1]];
-      float lp = quiet_nan();
-      if (tok == a.ignore_index) lp = 0.0f;
-      else if (tok >= 0 && tok < V) lp = none ? neg_inf() : (logit_at<T>(x, tok) - st.m) * inv_t - ln_s;
-      a.logprob[row] = lp;
-    }
-  }
+  const float ln_s = ln_sum(st);
+  if (tid == 0) write_figures(a, row, st, ln_s, inv_t, tok);
   if (TOP) {
     for (int n = tid; n < C * K; n += G) {
       const uint64_t mine = lists[n];
@@ -385,7 +528,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
       if (place < K) {
         a.top_index[row * K + place] = key_index(mine);
         a.top_logprob[row * K + place] =
-            none ? neg_inf() : (key_value(static_cast<uint32_t>(mine >> 32)) - st.m) * inv_t - ln_s;
+            logprob_of(key_value(static_cast<uint32_t>(mine >> 32)), st, ln_s, inv_t);
       }
     }
   }
@@ -534,14 +677,23 @@ int launch_forward(const TokenLogprobsArgs& a, int cluster, cudaStream_t stream)
   return launch_check("token_logprobs launch");
 }
 
+template <typename T, int E>
+int launch_short(const TokenLogprobsArgs& a, cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>((a.outer * a.inner + kWarps - 1) / kWarps);
+  if (a.K > 0) token_logprobs_short_kernel<T, E, true><<<grid, kThreads, 0, stream>>>(a);
+  else token_logprobs_short_kernel<T, E, false><<<grid, kThreads, 0, stream>>>(a);
+  return launch_check("token_logprobs launch");
+}
+
 template <typename T>
 int forward_by_size(const TokenLogprobsArgs& a, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner, vecs = a.V / kVec<T>;
-  if (a.V <= 1024 && a.K <= kWarpTop) {
-    if (vecs <= 32) return launch_forward<T, 32, 1>(a, 1, stream);
-    if (vecs <= 64) return launch_forward<T, 32, 2>(a, 1, stream);
+  if (a.V <= 256) return launch_short<T, 8>(a, stream);
+  if (a.V <= 512) return launch_short<T, 16>(a, stream);
+  if (a.V <= kShort) return launch_short<T, 32>(a, stream);
+  // Many rows of a middling length: a warp each.
+  if (a.V <= kWarpRow && a.K <= kWarpTop && rows >= kWarpRows * sm_count_here())
     return launch_forward<T, 32, kUnroll>(a, 1, stream);
-  }
   // Few rows: split each until there are some CTAs for every SM or a slice is one batch.
   int cluster = 1;
   while (cluster < kMaxCluster && rows * cluster < 4 * sm_count_here() &&
