@@ -18,6 +18,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/stl.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <cstdint>
@@ -750,6 +752,99 @@ at::Tensor distill_topk_bwd(const at::Tensor& logits, const at::Tensor& index,
   return d;
 }
 
+// The operators as autograd nodes (kernels/logits.py has the same in Python for the ctypes
+// binding). Each is differentiable once: a second derivative raises, as once_differentiable's does.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+MaybeTensor maybe(const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : std::nullopt; }
+at::Tensor defined_or_not(const MaybeTensor& t) { return t.value_or(at::Tensor()); }
+
+variable_list once(variable_list grads, const at::Tensor& logits) {
+  if (!at::GradMode::is_enabled()) return grads;
+  // beside the logits, so that a second derivative by anything they come from finds the error
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice an operator on logits, which is differentiable once", 2);
+  grads[0] = (*error)({grads[0], logits})[0];
+  return grads;
+}
+
+struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits,
+                               const MaybeTensor& tokens, int64_t top_k, double temperature,
+                               int64_t ignore_index) {
+    auto [logprob, entropy, lse, top_logprob, top_index, stats] =
+        token_logprobs(logits, tokens, top_k, temperature, ignore_index, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, defined_or_not(tokens), *stats, entropy, defined_or_not(top_index)});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    variable_list out = {entropy, lse};  // the figures asked for: a node has no undefined outputs
+    if (logprob.has_value()) out.push_back(*logprob);
+    if (top_index.has_value()) {
+      ctx->mark_non_differentiable({*top_index});
+      out.push_back(*top_logprob);
+      out.push_back(*top_index);
+    }
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list out(5);
+    const variable_list saved = ctx->get_saved_variables();
+    const size_t top = saved[1].defined() ? 3 : 2;
+    const at::Tensor g_logprob = saved[1].defined() ? g[2] : at::Tensor(),
+                     g_top = saved[4].defined() ? g[top] : at::Tensor();
+    if (!g[0].defined() && !g[1].defined() && !g_logprob.defined() && !g_top.defined()) return out;
+    out[0] = token_logprobs_bwd(saved[0], maybe(saved[1]), saved[2], saved[3], maybe(saved[4]),
+                                maybe(g_logprob), maybe(g[0]), maybe(g[1]), maybe(g_top),
+                                ctx->saved_data["temperature"].toDouble(),
+                                ctx->saved_data["ignore_index"].toInt());
+    return once(out, saved[0]);
+  }
+};
+
+std::tuple<MaybeTensor, at::Tensor, at::Tensor, MaybeTensor, MaybeTensor> token_logprobs_autograd(
+    const at::Tensor& logits, const MaybeTensor& tokens, int64_t top_k, double temperature,
+    int64_t ignore_index) {
+  if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
+    auto r = token_logprobs(logits, tokens, top_k, temperature, ignore_index, false);
+    return {std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r), std::get<4>(r)};
+  }
+  const variable_list r = TokenLogprobsFn::apply(logits, tokens, top_k, temperature, ignore_index);
+  const size_t top = tokens.has_value() ? 3 : 2;
+  return {tokens.has_value() ? MaybeTensor(r[2]) : std::nullopt, r[0], r[1],
+          top_k > 0 ? MaybeTensor(r[top]) : std::nullopt,
+          top_k > 0 ? MaybeTensor(r[top + 1]) : std::nullopt};
+}
+
+struct DistillTopkFn : torch::autograd::Function<DistillTopkFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& index,
+                            const at::Tensor& teacher, const MaybeTensor& weight,
+                            double temperature, bool tail) {
+    auto [loss, d, stats] = distill_topk(logits, index, teacher, weight, temperature, tail, false, true);
+    ctx->save_for_backward({logits, index, teacher, defined_or_not(weight), *stats});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["tail"] = tail;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list out(6);
+    out[0] = distill_topk_bwd(saved[0], saved[1], saved[2], maybe(saved[3]), saved[4], g[0],
+                              ctx->saved_data["temperature"].toDouble(),
+                              ctx->saved_data["tail"].toBool());
+    return once(out, saved[0]);
+  }
+};
+
+at::Tensor distill_topk_autograd(const at::Tensor& logits, const at::Tensor& index,
+                                 const at::Tensor& teacher, const MaybeTensor& weight,
+                                 double temperature, bool tail) {
+  if (!at::GradMode::is_enabled() || !logits.requires_grad())
+    return std::get<0>(distill_topk(logits, index, teacher, weight, temperature, tail, false, false));
+  return DistillTopkFn::apply(logits, index, teacher, weight, temperature, tail);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -806,6 +901,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("distill_topk_bwd", &distill_topk_bwd, "gradient of distill_topk's loss by the logits",
         py::arg("logits"), py::arg("teacher_index"), py::arg("teacher_logprob"), py::arg("weight"),
         py::arg("stats"), py::arg("g_loss"), py::arg("temperature") = 1.0, py::arg("tail") = false);
+  m.def("token_logprobs_autograd", &token_logprobs_autograd,
+        "(logprob, entropy, lse, top_logprob, top_index), differentiable by the logits",
+        py::arg("logits"), py::arg("tokens"), py::arg("top_k"), py::arg("temperature"),
+        py::arg("ignore_index"));
+  m.def("distill_topk_autograd", &distill_topk_autograd,
+        "loss against a teacher's list of top tokens, differentiable by the logits",
+        py::arg("logits"), py::arg("teacher_index"), py::arg("teacher_logprob"), py::arg("weight"),
+        py::arg("temperature"), py::arg("tail"));
   m.def("abi_version", &bdh_abi_version, "ABI version of the loaded libbdh_sm100.so");
   m.attr("has_cuda") = true;
 }

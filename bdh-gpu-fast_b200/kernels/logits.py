@@ -18,7 +18,6 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import sm100_attn, sm100_ext, sm100_logits
 
@@ -39,6 +38,17 @@ def _ops():
     return sm100_logits if ops is sm100_attn else ops
 
 
+def _once(d: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
+    """A gradient that raises where it is itself differentiated. (torch's once_differentiable lets
+    it pass as a constant when the upstream gradient needs none; this one depends on the logits.)"""
+    if not torch.is_grad_enabled():
+        return d
+    error = torch._C._functions.DelayedError(
+        "trying to differentiate twice an operator on logits, which is differentiable once", 2)
+    return error(d, logits)[0]
+
+
+# The autograd nodes of the ctypes binding; the extension has its own (a tenth of the host time).
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top_k, temperature, ignore_index):
@@ -52,14 +62,13 @@ class _TokenLogprobsFn(torch.autograd.Function):
         return logprob, entropy, lse, top, index
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_logprob, g_entropy, g_lse, g_top, _):
         if g_logprob is None and g_entropy is None and g_lse is None and g_top is None:
             return (None,) * 5
         logits, tokens, stats, entropy, index = ctx.saved_tensors
-        return (_ops().token_logprobs_bwd(logits, tokens, stats, entropy, index, g_logprob,
-                                          g_entropy, g_lse, g_top, *ctx.opts),
-                None, None, None, None)
+        d = _ops().token_logprobs_bwd(logits, tokens, stats, entropy, index, g_logprob, g_entropy,
+                                      g_lse, g_top, *ctx.opts)
+        return _once(d, logits), None, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top_k: int = 0,
@@ -75,11 +84,15 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     logit makes its position's figures NaN. ``logprob``, ``entropy``, ``lse`` and ``top_logprob``
     carry gradients to the logits.
     """
+    ops = _ops()
+    if ops is not sm100_logits:
+        return TokenLogprobs._make(ops.token_logprobs_autograd(logits, tokens, top_k, temperature,
+                                                               ignore_index))
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobsFn.apply(logits, tokens, top_k, temperature,
                                                      ignore_index))
-    return TokenLogprobs(*_ops().token_logprobs(logits, tokens, top_k, temperature,
-                                                ignore_index)[:5])
+    return TokenLogprobs(*ops.token_logprobs(logits, tokens, top_k, temperature,
+                                             ignore_index)[:5])
 
 
 class _DistillTopkFn(torch.autograd.Function):
@@ -92,11 +105,10 @@ class _DistillTopkFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_loss):
         logits, index, teacher, weight, stats = ctx.saved_tensors
-        return (_ops().distill_topk_bwd(logits, index, teacher, weight, stats, g_loss, *ctx.opts),
-                None, None, None, None, None)
+        d = _ops().distill_topk_bwd(logits, index, teacher, weight, stats, g_loss, *ctx.opts)
+        return _once(d, logits), None, None, None, None, None
 
 
 def _constant_teacher(teacher_logprob, weight) -> None:
@@ -123,10 +135,14 @@ def distill_topk_loss(logits: torch.Tensor, teacher_index: torch.Tensor,
     convention is wanted. Differentiable with respect to the logits.
     """
     _constant_teacher(teacher_logprob, weight)
+    ops = _ops()
+    if ops is not sm100_logits:
+        return ops.distill_topk_autograd(logits, teacher_index, teacher_logprob, weight,
+                                         temperature, tail)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillTopkFn.apply(logits, teacher_index, teacher_logprob, weight, temperature,
                                     tail)
-    return _ops().distill_topk(logits, teacher_index, teacher_logprob, weight, temperature, tail)[0]
+    return ops.distill_topk(logits, teacher_index, teacher_logprob, weight, temperature, tail)[0]
 
 
 def distill_topk_loss_grad(logits: torch.Tensor, teacher_index: torch.Tensor,

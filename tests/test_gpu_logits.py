@@ -553,9 +553,43 @@ def test_refusals():
     torch.cuda.synchronize()
 
 
-def test_double_backward_is_refused():
+@pytest.mark.parametrize("binding", ["ext", "ctypes"])
+def test_double_backward_is_refused(binding, monkeypatch):
+    monkeypatch.setenv("BDH_SM100_EXT", "1" if binding == "ext" else "0")
     x = torch.randn(2, 16, device="cuda", requires_grad=True)
     r = kernels.token_logprobs(x, torch.zeros(2, dtype=torch.long, device="cuda"))
     (d,) = torch.autograd.grad(r.logprob.sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError):
-        torch.autograd.grad(d.sum(), x)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad((d * d).sum() + x.sum(), x)
+    idx = torch.zeros(2, 3, dtype=torch.long, device="cuda")
+    loss = kernels.distill_topk_loss(x, idx, torch.zeros(2, 3, device="cuda"))
+    (d,) = torch.autograd.grad(loss.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad((d * d).sum() + x.sum(), x)
+
+
+def test_both_bindings_autograd_gives_the_same_bits(monkeypatch):
+    V, shape = 700, (2, 5)
+    x = make(shape, V, torch.bfloat16)
+    tok = tokens(shape, V).cuda()
+    index, lp = (t.cuda() for t in lists(shape, V, 9))
+    got = {}
+    for binding in ("1", "0"):
+        monkeypatch.setenv("BDH_SM100_EXT", binding)
+        z = x.clone().requires_grad_(True)
+        r = kernels.token_logprobs(z, tok, top_k=4, temperature=0.9)
+        loss = kernels.distill_topk_loss(z, index, lp, temperature=1.2, tail=True)
+        (r.logprob.sum() + (r.entropy * 0.3).sum() + r.top_logprob.sum() + loss.sum()).backward()
+        assert not r.top_index.requires_grad and r.lse.requires_grad
+        got[binding] = [r.logprob, r.entropy, r.lse, r.top_logprob, r.top_index, loss, z.grad]
+    for p, q in zip(got["1"], got["0"]):
+        assert torch.equal(p, q)
+
+
+def test_logits_changed_after_the_forward_are_noticed():
+    x = torch.randn(3, 50, device="cuda", requires_grad=True)
+    y = x * 1.0
+    r = kernels.token_logprobs(y, torch.zeros(3, dtype=torch.long, device="cuda"))
+    y.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        r.logprob.sum().backward()
