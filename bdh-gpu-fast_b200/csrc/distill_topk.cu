@@ -34,8 +34,8 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kPiece = 16384;             // elements of a row per CTA of the streaming backward
-constexpr int kSliceBytes = 48 * 1024;    // of a row per CTA, while the cluster may grow
-static_assert(kThreads - 32 >= kTopMax, "one thread per slot, and a warp beside them");
+constexpr int kSliceBytes = 68 * 1024;    // of a row per CTA, while the cluster may grow
+static_assert(kThreads >= kTopMax, "one thread per slot");
 
 constexpr int kStats = 8;  // floats per row: see RowStats
 
@@ -327,12 +327,11 @@ __global__ void __launch_bounds__(kThreads, E <= 16 && S == 1 ? 4 : 3) distill_s
 
 // ------------------------------------------------------------ a CTA or a cluster for a row
 struct CtaShared {
-  SoftState part[kMaxCluster];
-  int part_repeated[kMaxCluster];
-  SoftState warp_part[kWarps];
-  SoftState top;  // softmax state of the listed tokens
+  float2 part[kMaxCluster * kWarps];  // maximum and sum of every warp of the cluster
+  int repeated[kMaxCluster];          // a token is twice in the list, and in that CTA's slice
+  SoftState top;                      // softmax state of the listed tokens
   float total, r, shift;
-  int index[kTopMax];  // -1: empty slot (or one past the vocabulary)
+  int index[kTopMax];  // -1: empty slot; V: a token past the vocabulary
   float lnq[kTopMax], q[kTopMax], z[kTopMax];
   float mass[kTopMax];  // q summed over the slots of the same token; below 0: not its first slot
 };
@@ -341,7 +340,7 @@ constexpr size_t kCtaShared = (sizeof(CtaShared) + 15) & ~size_t(15);
 
 // Masses of repeated tokens to the first slot of each, and the listed tokens' softmax state
 // (one warp).
-__device__ __forceinline__ void list_state(CtaShared& sh, int K, int lane, float c, bool repeated) {
+__device__ __forceinline__ void list_state(CtaShared& sh, int K, int V, int lane, float c, bool repeated) {
   float zs[kTopMax / 32];
 #pragma unroll
   for (int s = 0; s < kTopMax / 32; ++s) {
@@ -349,8 +348,9 @@ __device__ __forceinline__ void list_state(CtaShared& sh, int K, int lane, float
     zs[s] = neg_inf();
     if (j >= K) continue;
     const int at = sh.index[j];
-    float mass = at >= 0 ? sh.q[j] : -1.0f;
-    if (repeated && at >= 0) {
+    const bool token = at >= 0 && at < V;
+    float mass = token ? sh.q[j] : -1.0f;
+    if (repeated && token) {
       mass = 0.0f;
       bool first = true;
       for (int k = 0; k < K; ++k)
@@ -406,23 +406,29 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillTopkArgs 
                  : "memory");
   const int edge = tid < head ? tid : tid - head < tail ? n - tail + tid - head : -1;
   if (edge >= 0) held[edge] = x[from + edge];
-  int at = -1;  // this thread's slot: its token, where it lies in the slice
-  bool bad = false;
   if (tid < K) {
-    at = slot_token(a.index[o * a.i_strides[0] + i * a.i_strides[1] + tid * a.i_strides[2]], V);
+    const int at = slot_token(a.index[o * a.i_strides[0] + i * a.i_strides[1] + tid * a.i_strides[2]], V);
     const float t = a.teacher[o * a.t_strides[0] + i * a.t_strides[1] + tid * a.t_strides[2]];
-    sh.lnq[tid] = at >= 0 ? t : neg_inf();
-    bad = at == V;
-    if (bad) at = -1;
-    sh.z[tid] = at >= 0 ? logit_at<T>(x, at) : neg_inf();
     sh.index[tid] = at;
-    at = at >= from && at < from + n ? at - from : -1;
+    sh.lnq[tid] = at >= 0 ? t : neg_inf();
+    sh.z[tid] = at >= 0 && at < V ? logit_at<T>(x, at) : neg_inf();
   }
   const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
   asm volatile("cp.async.wait_all;" ::: "memory");
-  bad = __syncthreads_or(bad);
-  if (at >= 0) put_slot(held, at, tid);
-  if (warp == kWarps - 1) {  // (the slots are the first warps')
+  __syncthreads();  // the slice and the list are in shared memory
+  auto in_slice = [&](int at) { return at >= from && at < from + n; };
+  if (warp == 0) {  // strike the listed tokens out
+    for (int j = lane; j < K; j += 32)
+      if (in_slice(sh.index[j])) put_slot(held, sh.index[j] - from, j);
+    __syncwarp();
+    bool other = false;
+    for (int j = lane; j < K; j += 32)
+      if (in_slice(sh.index[j])) other |= get_slot(held, sh.index[j] - from) != j;
+    other = __any_sync(0xffffffffu, other);  // and all have read
+    for (int j = lane; j < K; j += 32)
+      if (in_slice(sh.index[j])) logit_put(held, sh.index[j] - from, neg_inf());
+    if (lane == 0) sh.repeated[rank] = other ? 1 : 0;
+  } else if (warp == 1) {  // the list's masses
     float m = neg_inf(), shift = 0.0f, total = 0.0f;
     if (!a.tail) {
       for (int j = lane; j < K; j += 32) m = max_nan(m, sh.lnq[j]);
@@ -433,82 +439,69 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillTopkArgs 
         shift = m + logf(warp_sum(s));
       }
     }
+    bool bad = false;
     for (int j = lane; j < K; j += 32) {
       const float l = sh.lnq[j] - shift, q = expf(l);
       sh.lnq[j] = l;
       sh.q[j] = q;
       total += q;
+      bad |= sh.index[j] == V;
     }
     total = warp_sum(total);
+    bad = __any_sync(0xffffffffu, bad);
     if (lane == 0) {
       sh.total = bad ? quiet_nan() : total;  // a token past the vocabulary: NaN throughout
       sh.r = a.tail ? max_nan(0.0f, 1.0f - total) : 0.0f;
       sh.shift = shift;
     }
     __syncwarp();
-    list_state(sh, K, lane, c, false);
+    list_state(sh, K, V, lane, c, false);
   }
-  __syncthreads();
-  bool repeated = __syncthreads_or(at >= 0 && get_slot(held, at) != tid);
-  if (at >= 0) logit_put(held, at, neg_inf());
   __syncthreads();
 
   SoftState rest = soft_empty();
   if (edge >= 0) soft_add(rest, logit_at<T>(held, edge), c);
   for (int b = 0; b < vecs; b += kThreads * kUnroll) {
-    float xs[kUnroll * kV];
+    uint4 wv[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int v = b + u * kThreads + tid;
-      float part[kV];
-      unpack(v < vecs ? hvec[v] : void_vec<T>(), part);
-#pragma unroll
-      for (int e = 0; e < kV; ++e) xs[u * kV + e] = part[e];
+      wv[u] = v < vecs ? hvec[v] : void_vec<T>();
     }
-    float m = xs[0];
-#pragma unroll
-    for (int e = 1; e < kUnroll * kV; ++e) m = max_nan(m, xs[e]);
+    const float m = max_of(wv, T());
     if (!(m <= rest.m)) soft_raise(rest, max_nan(m, rest.m), c);
-    if (rest.m != neg_inf()) soft_sum<false>(rest, xs, c);
-  }
-  {
-    const float m = warp_max(rest.m);
-    if (m != neg_inf()) soft_raise(rest, m, c);
-    rest.s = warp_sum(rest.s);
-  }
-  if (lane == 0) sh.warp_part[warp] = rest;
-  __syncthreads();
-  if (C > 1) cluster_wait();
-  if (warp == 0) {  // the CTA's state, to every CTA of the cluster
-    SoftState mine = lane < kWarps ? sh.warp_part[lane] : soft_empty();
-    const float m = warp_max(mine.m);
-    if (m != neg_inf()) soft_raise(mine, m, c);
-    mine.s = warp_sum(mine.s);
-    if (C == 1 && lane == 0) {
-      sh.part[0] = mine;
-      sh.part_repeated[0] = repeated ? 1 : 0;
-    } else if (C > 1 && lane < C) {
-      const uint32_t to = peer_smem(&sh.part[rank], lane);
-      peer_store(to, m);
-      peer_store(to + 4, mine.s);
-      peer_store(peer_smem(&sh.part_repeated[rank], lane), __int_as_float(repeated ? 1 : 0));
+    if (rest.m != neg_inf()) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        float xs[kV];
+        unpack(wv[u], xs);
+        soft_sum<false>(rest, xs, c);
+      }
     }
   }
-  if (C > 1) {
+  rest = soft_join(rest, c);
+  if (C > 1) {  // every warp's state to every CTA of the cluster
+    cluster_wait();
+    if (lane < C) {
+      const uint32_t to = peer_smem(&sh.part[rank * kWarps + warp], lane);
+      peer_store(to, rest.m);
+      peer_store(to + 4, rest.s);
+      if (warp == 0) peer_store(peer_smem(&sh.repeated[rank], lane), __int_as_float(sh.repeated[rank]));
+    }
     cluster_arrive();
     cluster_wait();
   } else {
+    if (lane == 0) sh.part[warp] = make_float2(rest.m, rest.s);
     __syncthreads();
   }
-  rest = {sh.part[0].m, sh.part[0].s, 0.0f};
-  repeated = sh.part_repeated[0] != 0;
-  for (int k = 1; k < C; ++k) {
-    rest = soft_merge(rest, {sh.part[k].m, sh.part[k].s, 0.0f}, c);
-    repeated |= sh.part_repeated[k] != 0;
-  }
-  if (repeated) {
+  rest = soft_empty();
+  for (int k = lane; k < C * kWarps; k += 32)
+    rest = soft_merge(rest, {sh.part[k].x, sh.part[k].y, 0.0f}, c);
+  rest = soft_join(rest, c);
+  const bool repeated = __any_sync(0xffffffffu, lane < C && sh.repeated[lane] != 0);
+  if (repeated) {  // in every CTA of the cluster
     __syncthreads();
-    if (warp == 0) list_state(sh, K, lane, c, true);
+    if (warp == 1) list_state(sh, K, V, lane, c, true);
     __syncthreads();
   }
   const SoftState all = soft_merge(rest, {sh.top.m, sh.top.s, 0.0f}, c);
@@ -553,8 +546,8 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillTopkArgs 
   }
   if (g.none) return;
   __syncthreads();
-  if (at >= 0 && !(sh.mass[tid] < 0.0f))
-    logit_put(d, from + at, listed_gradient(g, sh.z[tid], sh.mass[tid], c));
+  if (tid < K && in_slice(sh.index[tid]) && !(sh.mass[tid] < 0.0f))
+    logit_put(d, sh.index[tid], listed_gradient(g, sh.z[tid], sh.mass[tid], c));
 }
 
 // --------------------------------------------------- the gradient from the forward's statistics

@@ -125,6 +125,31 @@ __device__ __forceinline__ void store_vec(uint16_t* p, const float (&x)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(cvt_bf16x2(x[0], x[1]), cvt_bf16x2(x[2], x[3]),
                                             cvt_bf16x2(x[4], x[5]), cvt_bf16x2(x[6], x[7]));
 }
+// The largest element of N vectors (bf16 in pairs, where one instruction compares two).
+template <int N>
+__device__ __forceinline__ float max_of(const uint4 (&w)[N], float) {
+  float m = neg_inf();
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    float x[4];
+    unpack(w[u], x);
+    m = max_nan(m, max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3])));
+  }
+  return m;
+}
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <int N>
+__device__ __forceinline__ float max_of(const uint4 (&w)[N], uint16_t) {
+  uint32_t m = 0xff80ff80u;
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+    m = max_bf16x2(m, max_bf16x2(max_bf16x2(w[u].x, w[u].y), max_bf16x2(w[u].z, w[u].w)));
+  return max_nan(bf16x2_lo(m), bf16x2_hi(m));
+}
 // A vector of -inf: what a place past the end of a row counts as.
 template <typename T>
 __device__ __forceinline__ uint4 void_vec();

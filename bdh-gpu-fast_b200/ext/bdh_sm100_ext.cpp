@@ -15,6 +15,7 @@
 // tensor raises), fp32 and bf16 only, and scratch memory comes from the PyTorch caching
 // allocator (the library itself never allocates).
 #include <ATen/MemoryOverlap.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/stl.h>
@@ -609,6 +610,12 @@ std::vector<int64_t> with_entries(const LogitRows& x, int64_t k) {
 
 using MaybeTensor = std::optional<at::Tensor>;
 
+// A new tensor on the logits' device from the caching allocator (of the current stream), without
+// at::empty's dispatch: a small call spends most of its host time on its outputs.
+at::Tensor fresh(const LogitRows& x, at::IntArrayRef shape, at::ScalarType dtype) {
+  return at::detail::empty_cuda(shape, dtype, x.t.device(), std::nullopt);
+}
+
 // (logprob, entropy, lse, top_logprob, top_index, stats) per row; None where not asked for.
 std::tuple<MaybeTensor, at::Tensor, at::Tensor, MaybeTensor, MaybeTensor, MaybeTensor>
 token_logprobs(const at::Tensor& logits, const MaybeTensor& tokens, int64_t top_k,
@@ -620,15 +627,14 @@ token_logprobs(const at::Tensor& logits, const MaybeTensor& tokens, int64_t top_
   check_temperature(temperature, "token_logprobs");
   const std::optional<BesideRows> tok = token_rows(x, tokens, "token_logprobs");
   const c10::cuda::CUDAGuard guard(x.t.device());
-  const auto f32 = x.t.options().dtype(at::kFloat);
   MaybeTensor logprob, top_logprob, top_index, stats;
-  if (tok.has_value()) logprob = at::empty(x.lead, f32);
-  at::Tensor entropy = at::empty(x.lead, f32), lse = at::empty(x.lead, f32);
+  if (tok.has_value()) logprob = fresh(x, x.lead, at::kFloat);
+  at::Tensor entropy = fresh(x, x.lead, at::kFloat), lse = fresh(x, x.lead, at::kFloat);
   if (top_k > 0) {
-    top_logprob = at::empty(with_entries(x, top_k), f32);
-    top_index = at::empty(with_entries(x, top_k), f32.dtype(at::kLong));
+    top_logprob = fresh(x, with_entries(x, top_k), at::kFloat);
+    top_index = fresh(x, with_entries(x, top_k), at::kLong);
   }
-  if (want_stats) stats = at::empty({x.rows(), 2}, f32);
+  if (want_stats) stats = fresh(x, {x.rows(), 2}, at::kFloat);
   auto fp = [](const MaybeTensor& t) { return t.has_value() ? t->data_ptr<float>() : nullptr; };
   check_rc(bdh_token_logprobs(
                x.t.data_ptr(), dtype_code(x.t), x.strides,
@@ -671,7 +677,7 @@ at::Tensor token_logprobs_bwd(const at::Tensor& logits, const MaybeTensor& token
     ti = rowmajor(top_index, at::kLong, k * x.rows(), "top_index");
     gt = rowmajor(g_top, at::kFloat, k * x.rows(), "g_top");
   }
-  at::Tensor d = at::empty(logits.sizes(), x.t.options());
+  at::Tensor d = fresh(x, logits.sizes(), x.t.scalar_type());
   const int64_t ds[2] = {x.inner * x.V, x.V};
   check_rc(bdh_token_logprobs_bwd(
                x.t.data_ptr(), dtype_code(x.t), x.strides,
@@ -711,11 +717,10 @@ std::tuple<at::Tensor, MaybeTensor, MaybeTensor> distill_topk(
   const LogitRows x(logits, "distill_topk");
   const c10::cuda::CUDAGuard guard(x.t.device());
   const DistillList l = distill_list(x, index, teacher, weight, temperature);
-  const auto f32 = x.t.options().dtype(at::kFloat);
-  at::Tensor loss = at::empty(x.lead, f32);
+  at::Tensor loss = fresh(x, x.lead, at::kFloat);
   MaybeTensor d, stats;
-  if (want_grad) d = at::empty(logits.sizes(), x.t.options());
-  if (want_stats) stats = at::empty({x.rows(), 8}, f32);
+  if (want_grad) d = fresh(x, logits.sizes(), x.t.scalar_type());
+  if (want_stats) stats = fresh(x, {x.rows(), 8}, at::kFloat);
   const int64_t ds[2] = {x.inner * x.V, x.V};
   check_rc(bdh_distill_topk(x.t.data_ptr(), dtype_code(x.t), x.strides,
                             l.index.t.data_ptr<int64_t>(), l.index.strides,
@@ -740,7 +745,7 @@ at::Tensor distill_topk_bwd(const at::Tensor& logits, const at::Tensor& index,
       stats.numel() != 8 * x.rows())
     TORCH_CHECK_VALUE(false, "distill_topk_bwd: bad stats");
   const at::Tensor st = stats.contiguous();
-  at::Tensor d = at::empty(logits.sizes(), x.t.options());
+  at::Tensor d = fresh(x, logits.sizes(), x.t.scalar_type());
   const int64_t ds[2] = {x.inner * x.V, x.V};
   check_rc(bdh_distill_topk_bwd(x.t.data_ptr(), dtype_code(x.t), x.strides,
                                 l.index.t.data_ptr<int64_t>(), l.index.strides,
