@@ -41,7 +41,7 @@ constexpr int kStats = 8;  // floats per row: see RowStats
 
 // What the forward leaves for the gradient.
 struct RowStats {
-  float m, ln_s;            // largest logit, ln of the sum of exp((x - m) / temperature)
+  float m, ln_s;            // a base near the largest logit, ln of the sum of exp((x - m) / temperature)
   float rest_m, ln_rest;    // the same of the unlisted tokens
   float total, r;           // mass of the list, and of the class beside it
   float shift;              // ln q = teacher's value - shift
@@ -461,24 +461,23 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillTopkArgs 
 
   SoftState rest = soft_empty();
   if (edge >= 0) soft_add(rest, logit_at<T>(held, edge), c);
+  SoftSums sums(rest);
+  const float slack = kBaseSlack / c;
   for (int b = 0; b < vecs; b += kThreads * kUnroll) {
     uint4 wv[kUnroll];
+    if (b + kThreads * kUnroll <= vecs) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int v = b + u * kThreads + tid;
-      wv[u] = v < vecs ? hvec[v] : void_vec<T>();
-    }
-    const float m = max_of(wv, T());
-    if (!(m <= rest.m)) soft_raise(rest, max_nan(m, rest.m), c);
-    if (rest.m != neg_inf()) {
+      for (int u = 0; u < kUnroll; ++u) wv[u] = hvec[b + u * kThreads + tid];
+    } else {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        float xs[kV];
-        unpack(wv[u], xs);
-        soft_sum<false>(rest, xs, c);
+        const int v = b + u * kThreads + tid;
+        wv[u] = v < vecs ? hvec[v] : void_vec<T>();
       }
     }
+    sums.add<false, T>(wv, max_of(wv, T()), c, slack);
   }
+  rest = sums.state();
   rest = soft_join(rest, c);
   if (C > 1) {  // every warp's state to every CTA of the cluster
     cluster_wait();

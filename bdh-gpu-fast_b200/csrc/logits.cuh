@@ -38,6 +38,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return y;
 }
 
+// One instruction on sm_100.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
 template <typename T>
 __device__ __forceinline__ float logit_at(const T* p, int64_t i);
 template <>
@@ -133,7 +140,7 @@ __device__ __forceinline__ float max_of(const uint4 (&w)[N], float) {
   for (int u = 0; u < N; ++u) {
     float x[4];
     unpack(w[u], x);
-    m = max_nan(m, max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3])));
+    m = max_nan(max_nan(m, x[0], x[1]), x[2], x[3]);
   }
   return m;
 }
@@ -268,6 +275,57 @@ __device__ __forceinline__ void soft_sum(SoftState& st, const float (&x)[N], flo
     st.a += a0 + a1;
   }
 }
+
+// A thread's running softmax state over vectors: the two sums in pairs, and a base m that is a value
+// of the row but may be below its largest by up to kBaseSlack in the exponent, so that the sums are
+// rescaled a few times a row and not whenever a new maximum comes (terms stay below 2^kBaseSlack).
+constexpr float kBaseSlack = 8.0f;
+struct SoftSums {
+  float m;
+  F2 s, a;
+  __device__ __forceinline__ explicit SoftSums(const SoftState& st)
+      : m(st.m), s(f2(st.s, 0.0f)), a(f2(st.a, 0.0f)) {}
+  // N vectors whose largest element is `largest`.
+  template <bool ENTROPY, typename T, int N>
+  __device__ __forceinline__ void add(const uint4 (&w)[N], float largest, float c, float slack) {
+    if (!(largest <= m + slack)) {  // a NaN too
+      const float to = max_nan(largest, m);
+      const float d = max_nan((m - to) * c, kExpFloor), f = ex2(d);
+      const F2 ff = f2(f, f);
+      if (ENTROPY) a = f2_mul(ff, f2_fma(f2(d, d), s, a));
+      s = f2_mul(ff, s);
+      m = to;
+    }
+    if (m == neg_inf()) return;
+    const F2 nm = f2(-m, -m), cc = f2(c, c);
+    F2 ps = f2(0.0f, 0.0f), pa = f2(0.0f, 0.0f);
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      float x[kVec<T>];
+      unpack(w[u], x);
+#pragma unroll
+      for (int i = 0; i < kVec<T>; i += 2) {
+        float t0, t1;
+        f2_split(f2_mul(f2_add(f2(x[i], x[i + 1]), nm), cc), t0, t1);
+        if (ENTROPY) {
+          t0 = max_nan(t0, kExpFloor);
+          t1 = max_nan(t1, kExpFloor);
+        }
+        const F2 e = f2(ex2(t0), ex2(t1));
+        ps = f2_add(ps, e);
+        if (ENTROPY) pa = f2_fma(e, f2(t0, t1), pa);
+      }
+    }
+    s = f2_add(s, ps);
+    if (ENTROPY) a = f2_add(a, pa);
+  }
+  __device__ __forceinline__ SoftState state() const {
+    float s0, s1, a0, a1;
+    f2_split(s, s0, s1);
+    f2_split(a, a0, a1);
+    return {m, s0 + s1, a0 + a1};
+  }
+};
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll

@@ -1,7 +1,6 @@
 // extern "C" entries of the operators on logits: argument checks and the launches of
 // token_logprobs.cu and distill_topk.cu. Nothing here allocates; every call is stream-ordered
 // and graph-capturable.
-#include <cmath>
 #include <cstring>
 #include <string>
 
@@ -29,7 +28,7 @@ int check_rows(const char* what, int dtype, int64_t outer, int64_t inner, int64_
   if (outer > most || inner > most || (inner > 0 && outer > most / inner))
     return refuse(what, "at most 2^31 - 1 rows");
   if (K > BDH_TOP_MAX) return refuse(what, "at most BDH_TOP_MAX entries in a row's list");
-  if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(1.0f / temperature))
+  if (!(temperature > 1e-30f && temperature < 1e30f))  // so that 1 / temperature has room as well
     return refuse(what, "temperature must be positive and finite");
   return BDH_OK;
 }

@@ -25,9 +25,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kWarpTop = 16;     // longest list of the warp form: half of its threads' maxima
+constexpr int kWarpTop = 16;     // longest list that a short row bounds by its lanes' maxima
 constexpr int kWarpRow = 8192;   // longest row that a warp reads
 constexpr int kWarpRows = 16;    // rows for every SM from which a warp takes a row
+constexpr int kWarpList = 32;    // longest list of a warp's row (its candidates' room)
+constexpr int kWarpCells = 16;   // vectors per lane up to which each is a cell in a warp's row
 constexpr int kMaxCells = 48;    // cells per thread; longer rows put more batches into a cell
 constexpr int kMaxCluster = 8;
 
@@ -81,23 +83,8 @@ __device__ __forceinline__ uint64_t list_bound(int K, uint32_t lo, uint32_t hi, 
 }
 
 struct ForwardPlan {
-  int cells, cell_batches;  // per thread; batches in a cell
+  int cells, cell_vecs;  // per thread, and vectors in a cell: one, or a number of batches
   int cluster;
-};
-
-template <int G>
-struct Group;
-template <>
-struct Group<32> {
-  static __device__ __forceinline__ void sync() { __syncwarp(); }
-  static __device__ __forceinline__ int count(bool p) {
-    return __popc(__ballot_sync(0xffffffffu, p));
-  }
-};
-template <>
-struct Group<kThreads> {
-  static __device__ __forceinline__ void sync() { __syncthreads(); }
-  static __device__ __forceinline__ int count(bool p) { return __syncthreads_count(p); }
 };
 
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
@@ -107,26 +94,6 @@ __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
     k = other > k ? other : k;
   }
   return k;
-}
-
-// Shared memory of one group; cells and candidates follow it (forward_smem).
-struct GroupShared {
-  SoftState part[kMaxCluster];
-  uint64_t best[kWarps];
-  SoftState warp_part[kWarps];
-  uint32_t lo[kWarps], hi[kWarps];
-  int found, queued;
-};
-
-template <typename T, int G>
-__host__ __device__ constexpr size_t group_smem(int K, int cells, int cluster) {
-  size_t n = sizeof(GroupShared);
-  if (K > 0) {
-    n += (static_cast<size_t>(cells) * G * sizeof(float) + 7) & ~size_t(7);
-    n += static_cast<size_t>(candidate_room<T>(K)) * (sizeof(uint64_t) + sizeof(int));
-    n += static_cast<size_t>(cluster) * K * sizeof(uint64_t);
-  }
-  return (n + 15) & ~size_t(15);
 }
 
 // A given token's logit, asked for before the row is read so that the two loads' latencies pass
@@ -285,102 +252,135 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_short_kernel(TokenLog
 }
 
 // ------------------------------------------- a warp, a CTA or a cluster for longer rows
-template <typename T, int G, int U, bool TOP>
+// Shared memory of one group of G threads; with a list its cells, candidates, lists and queue follow.
+struct GroupShared {
+  SoftState part[kMaxCluster];
+  SoftState warp_part[kWarps];
+  uint64_t best[kWarps];
+  uint64_t bound;
+  int found, queued;
+};
+// The list's bound is searched among the cells themselves in a warp's row, and among the threads'
+// largest cells in a CTA's.
+template <int G>
+__host__ __device__ constexpr int bound_items(int cells) {
+  return G == 32 ? (cells + 1) * 32 : G;
+}
+// Candidates and queue; the items' indices, which are needed before them, take their place.
+template <typename T, int G>
+__host__ __device__ constexpr size_t candidate_smem(int K, int cells) {
+  const size_t cand = static_cast<size_t>(candidate_room<T>(K)) * (sizeof(uint64_t) + sizeof(int));
+  const size_t at = static_cast<size_t>(bound_items<G>(cells)) * sizeof(int);
+  return ((cand > at ? cand : at) + 7) & ~size_t(7);
+}
+constexpr size_t kGroupShared = (sizeof(GroupShared) + 7) & ~size_t(7);
+template <typename T, int G>
+__host__ __device__ constexpr size_t group_smem(int K, int cells, int cluster) {
+  size_t n = kGroupShared;
+  if (K > 0)
+    n += candidate_smem<T, G>(K, cells) + static_cast<size_t>(cluster) * K * sizeof(uint64_t) +
+         sizeof(int) * (static_cast<size_t>(cells + 1) * G + (G == 32 ? 0 : G));
+  return (n + 15) & ~size_t(15);
+}
+template <int G>
+__device__ __forceinline__ void group_sync() {
+  if (G == 32) __syncwarp();
+  else __syncthreads();
+}
+
+template <typename T, int G, bool TOP>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsArgs a,
                                                                   ForwardPlan plan) {
   extern __shared__ __align__(16) uint8_t smem[];
-  using Gr = Group<G>;
-  constexpr int kV = kVec<T>;
+  constexpr int kV = kVec<T>, U = kUnroll;
   const int K = static_cast<int>(a.K), V = static_cast<int>(a.V);
   const int C = G == 32 ? 1 : plan.cluster;
   const uint32_t rank = C > 1 ? cta_rank() : 0;
   const int tid = threadIdx.x % G, group = threadIdx.x / G;
+  const uint32_t row32 = G == 32 ? blockIdx.x * (kThreads / G) + group : blockIdx.x / static_cast<uint32_t>(C);
+  const int64_t row = row32;
+  if (row >= a.outer * a.inner) return;  // whole warps of the warp form
+  if (C > 1) cluster_arrive();  // every CTA's shared memory may be written once all have started
+  const int64_t o = row32 / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
+  const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
+  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t, slack = kBaseSlack / c;
+
   uint8_t* base = smem + group * group_smem<T, G>(K, plan.cells, C);
   GroupShared& sh = *reinterpret_cast<GroupShared*>(base);
-  float* cells = reinterpret_cast<float*>(base + sizeof(GroupShared));
-  uint64_t* cand = reinterpret_cast<uint64_t*>(
-      base + sizeof(GroupShared) + ((static_cast<size_t>(plan.cells) * G * 4 + 7) & ~size_t(7)));
-  uint64_t* lists = cand + candidate_room<T>(K);
-  int* queue = reinterpret_cast<int*>(lists + C * K);  // cells to look at again
-  const int64_t rows = a.outer * a.inner;
-  const int64_t row = G == 32 ? static_cast<int64_t>(blockIdx.x) * (kThreads / G) + group
-                              : static_cast<int64_t>(blockIdx.x) / C;
-  if (row >= rows) return;  // whole warps of the warp form
-  if (C > 1) cluster_arrive();  // every CTA's shared memory may be written once all have started
-  const int64_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
-  const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
-  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
-  Token tok = {false, true, 0.0f};
-  if (tid == 0 && rank == 0 && a.tokens != nullptr) tok = load_token(a, x, o, i);
+  uint64_t* cand = reinterpret_cast<uint64_t*>(base + kGroupShared);
+  int* queue = reinterpret_cast<int*>(cand + candidate_room<T>(K));  // cells to look at again
+  uint32_t* item_at = reinterpret_cast<uint32_t*>(cand);  // where a value's first element is
+  uint64_t* lists = reinterpret_cast<uint64_t*>(base + kGroupShared + candidate_smem<T, G>(K, plan.cells));
+  uint32_t* cells = reinterpret_cast<uint32_t*>(lists + C * K);  // [cell][thread]: largest value key
+  uint32_t* items = cells + (plan.cells + 1) * G;                // threads' largest (not for a warp)
 
   // This CTA's slice of the vectors; the row's head goes with the first slice, its tail with the last.
   const RowSpan span = row_span(x, V);
   const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
   const int per = (span.vecs + C - 1) / C;
   const int v0 = min(static_cast<int>(rank) * per, span.vecs), v1 = min(v0 + per, span.vecs);
-  SoftState st = soft_empty();
+  uint4 next[U];
+  auto load = [&](int b) {
+    if (b + G * U <= v1) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) next[u] = __ldg(vec + b + u * G + tid);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int v = b + u * G + tid;
+        next[u] = v < v1 ? __ldg(vec + v) : void_vec<T>();
+      }
+    }
+  };
+  load(v0);
+  Token tok = {false, true, 0.0f};
+  if (tid == 0 && rank == 0 && a.tokens != nullptr) tok = load_token(a, x, o, i);
   int edge = -1;  // this thread's element of the row's ends
   if (rank == 0 && tid < span.head) edge = tid;
   if (rank == C - 1 && tid >= 8 && tid - 8 < span.tail) edge = V - span.tail + tid - 8;
-  float edge_x = neg_inf();
-  if (edge >= 0) {
-    edge_x = logit_at<T>(x, edge);
-    soft_add(st, edge_x, c);
-  }
-  // For the list: an index that the first occurrence of the thread's maximum is not above.
-  int at_most = edge >= 0 ? edge : span.head + (v0 + tid) * kV + kV - 1;
-  const bool any = edge >= 0 || v0 + tid < v1;
+  const float edge_x = edge >= 0 ? logit_at<T>(x, edge) : neg_inf();
+  SoftState st = soft_empty();
+  if (edge >= 0) soft_add(st, edge_x, c);
+  SoftSums sums(st);
 
-  int cell = 0, in_cell = 0;
+  int cell = 0, in_cell = 0;          // TOP: cells written, vectors in the open one
+  uint32_t own = 0;                   // largest key of the thread
   float cell_max = neg_inf();
+  auto put_cell = [&](float largest, bool any) {
+    const uint32_t k = any ? value_key(largest) : 0u;
+    cells[cell++ * G + tid] = k;
+    own = max(own, k);
+  };
   for (int b = v0; b < v1; b += G * U) {
     uint4 w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int v = b + u * G + tid;
-      w[u] = v < v1 ? __ldg(vec + v) : void_vec<T>();
-    }
-    float xs[U * kV], vmax[U];
+    for (int u = 0; u < U; ++u) w[u] = next[u];
+    if (b + G * U < v1) load(b + G * U);
+    float largest;
+    if (TOP && plan.cell_vecs == 1) {
+      largest = neg_inf();
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float part[kV];
-      unpack(w[u], part);
-      vmax[u] = part[0];
-#pragma unroll
-      for (int e = 0; e < kV; ++e) {
-        xs[u * kV + e] = part[e];
-        if (e > 0) vmax[u] = max_nan(vmax[u], part[e]);
+      for (int u = 0; u < U; ++u) {
+        const uint4 one[1] = {w[u]};
+        const float m = max_of(one, T());
+        if (b + u * G < v1) put_cell(m, b + u * G + tid < v1);
+        largest = max_nan(largest, m);
       }
-    }
-    float m = vmax[0];
-#pragma unroll
-    for (int u = 1; u < U; ++u) m = max_nan(m, vmax[u]);
-    if (!(m <= st.m)) {  // a larger one, or a NaN here or before (at_most may then rise further)
+    } else {
+      largest = max_of(w, T());
       if (TOP) {
-        int u_first = U - 1;
-        if (m == m) {
-#pragma unroll
-          for (int u = U - 2; u >= 0; --u)
-            if (vmax[u] == m) u_first = u;
+        cell_max = max_nan(cell_max, largest);
+        in_cell += U;
+        if (in_cell == plan.cell_vecs || b + G * U >= v1) {
+          put_cell(cell_max, b + (U - in_cell) * G + tid < v1);
+          in_cell = 0;
+          cell_max = neg_inf();
         }
-        at_most = span.head + (b + u_first * G + tid) * kV + kV - 1;
-      }
-      soft_raise(st, max_nan(m, st.m), c);
-    }
-    if (st.m != neg_inf()) soft_sum<true>(st, xs, c);
-    if (TOP) {
-      cell_max = max_nan(cell_max, m);
-      if (++in_cell == plan.cell_batches) {
-        cells[cell++ * G + tid] = cell_max;
-        in_cell = 0;
-        cell_max = neg_inf();
       }
     }
+    sums.add<true, T>(w, largest, c, slack);
   }
-  if (TOP && in_cell > 0) cells[cell++ * G + tid] = cell_max;
-  const float own_max = st.m;
-
-  st = soft_join(st, c);
+  st = soft_join(sums.state(), c);
   if (G > 32) {
     if ((threadIdx.x & 31) == 0) sh.warp_part[threadIdx.x >> 5] = st;
     __syncthreads();
@@ -388,33 +388,104 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
   }
 
   if (TOP) {
-    // A bound below K elements of the slice: value key lo, and an index among elements of that value.
-    const uint32_t key = any ? value_key(own_max) : 0u;
-    at_most = min(at_most, V - 1);
+    const uint32_t edge_key = edge >= 0 ? value_key(edge_x) : 0u;
+    cells[cell * G + tid] = edge_key;  // the last cell: the row's ends
+    own = max(own, edge_key);
+    const int n_items = G == 32 ? (cell + 1) * 32 : G;
+    if (G > 32) items[tid] = own;
     if (tid == 0) sh.found = sh.queued = 0;
-    uint64_t bound = 0;
-    if (Gr::count(any) >= K) {
-      uint32_t lo = __reduce_min_sync(0xffffffffu, any ? key : 0xffffffffu);
-      uint32_t hi = __reduce_max_sync(0xffffffffu, key);
-      if (G > 32) {
-        if ((threadIdx.x & 31) == 0) {
-          sh.lo[threadIdx.x >> 5] = lo;
-          sh.hi[threadIdx.x >> 5] = hi;
-        }
-        __syncthreads();
-        for (int w = 0; w < kWarps; ++w) {
-          lo = min(lo, sh.lo[w]);
-          hi = max(hi, sh.hi[w]);
-        }
+    group_sync<G>();
+    const uint32_t* keys = G == 32 ? cells : items;
+    const int most = K + top_slack(K);
+    // First by value (one warp): at least K items at or above lo, as a rule not many more.
+    if (tid < 32) {
+      uint32_t lo = 0xffffffffu, hi = 0;
+      int some = 0;
+      for (int n = tid; n < n_items; n += 32) {
+        const uint32_t k = keys[n];
+        if (k != 0) lo = min(lo, k);
+        hi = max(hi, k);
+        some += k != 0 ? 1 : 0;
       }
-      bound = list_bound(
-          K, lo, hi, V, [&](uint32_t v) { return Gr::count(key >= v); },
-          [&](uint32_t v, uint32_t at) {
-            return Gr::count(key == v && static_cast<uint32_t>(at_most) <= at);
-          });
+      lo = __reduce_min_sync(0xffffffffu, lo);
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      some = __reduce_add_sync(0xffffffffu, some);
+      auto from = [&](uint32_t v) {
+        int n = 0;
+        for (int k = tid; k < n_items; k += 32) n += keys[k] >= v ? 1 : 0;
+        return static_cast<int>(__reduce_add_sync(0xffffffffu, n));
+      };
+      uint64_t bound = 0;  // fewer than K items: every element is a candidate
+      if (some >= K) {
+        int n = some;
+        ++hi;
+        while (hi - lo > 1 && n > most) {
+          const uint32_t mid = lo + (hi - lo) / 2;
+          const int now = from(mid);
+          if (now >= K) {
+            lo = mid;
+            n = now;
+          } else {
+            hi = mid;
+          }
+        }
+        // the low word: how many items may still be dropped by index, where too many share lo
+        bound = (static_cast<uint64_t>(lo) << 32) | (n > most ? static_cast<uint32_t>(from(lo + 1)) + 1u : 0u);
+      }
+      if (tid == 0) sh.bound = bound;
     }
-    Gr::sync();  // sh.found is set
-    const uint32_t bound_value = static_cast<uint32_t>(bound >> 32);
+    group_sync<G>();
+    uint64_t bound = sh.bound;
+    const uint32_t lo = static_cast<uint32_t>(bound >> 32);
+    uint32_t last = 0xffffffffu;  // of elements with value lo, those up to this index
+    auto first_at = [&](int q) {  // the first element with value lo of this thread's cell q
+      if (q == cell) return static_cast<uint32_t>(edge);
+      for (int n = 0; n < plan.cell_vecs; ++n) {
+        const int v = v0 + (q * plan.cell_vecs + n) * G + tid;
+        if (v >= v1) break;
+        float part[kV];
+        unpack(__ldg(vec + v), part);
+#pragma unroll
+        for (int e = 0; e < kV; ++e)
+          if (value_key(part[e]) == lo) return static_cast<uint32_t>(span.head + v * kV + e);
+      }
+      return 0xffffffffu;
+    };
+    if (static_cast<uint32_t>(bound) != 0) {
+      // Then, where too many items share the value, by the index of its first element in each.
+      const int above = static_cast<int>(static_cast<uint32_t>(bound)) - 1;
+      if (G == 32) {
+        for (int q = 0; q <= cell; ++q)
+          item_at[q * 32 + tid] = cells[q * 32 + tid] == lo ? first_at(q) : 0xffffffffu;
+      } else {
+        uint32_t at = 0xffffffffu;
+        if (own == lo)
+          for (int q = 0; q <= cell; ++q)
+            if (cells[q * G + tid] == lo) at = min(at, first_at(q));
+        item_at[tid] = at;
+      }
+      group_sync<G>();
+      if (tid < 32) {
+        uint32_t left = 0, right = static_cast<uint32_t>(V);
+        int n = n_items;
+        while (left < right && n > most - above) {
+          const uint32_t mid = left + (right - left) / 2;
+          int now = 0;
+          for (int k = tid; k < n_items; k += 32) now += item_at[k] <= mid ? 1 : 0;
+          now = __reduce_add_sync(0xffffffffu, now);
+          if (now >= K - above) {
+            right = mid;
+            n = now;
+          } else {
+            left = mid + 1;
+          }
+        }
+        if (tid == 0) sh.bound = right;
+      }
+      group_sync<G>();
+      last = static_cast<uint32_t>(sh.bound);  // item_at is done with: candidates may come
+      bound = (static_cast<uint64_t>(lo) << 32) | (0xffffffffu - last);
+    }
     const int room = candidate_room<T>(K);
     auto offer = [&](float v, int at) {
       const uint64_t k = top_key(v, at);
@@ -424,35 +495,30 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
       }
     };
     if (edge >= 0) offer(edge_x, edge);
-    if (value_key(own_max) >= bound_value) {
-      const uint32_t last = 0xffffffffu - static_cast<uint32_t>(bound);
+    if (own >= lo)
       for (int q = 0; q < cell; ++q) {
-        const uint32_t k = value_key(cells[q * G + tid]);
-        const uint32_t first = span.head + (v0 + q * plan.cell_batches * G * U + tid) * kV;
-        if (k < bound_value || (k == bound_value && first > last)) continue;
+        const uint32_t k = cells[q * G + tid];
+        const int v = v0 + q * plan.cell_vecs * G + tid;
+        if (k < lo || v >= v1 || (k == lo && static_cast<uint32_t>(span.head + v * kV) > last)) continue;
         const int n = atomicAdd(&sh.queued, 1);
-        if (n < room) queue[n] = q * G + tid;
+        if (n < room) queue[n] = v;
       }
-    }
-    Gr::sync();
+    group_sync<G>();
     // All threads on the queued cells' vectors, one each, so that their loads are under way together.
-    const int in_cell_vecs = plan.cell_batches * U;
-    if (sh.queued <= room) {
-      for (int n = tid; n < sh.queued * in_cell_vecs; n += G) {
-        const int item = queue[n / in_cell_vecs], q = item / G;
-        const int v = v0 + (q * in_cell_vecs + n % in_cell_vecs) * G + item % G;
+    const int queued = sh.queued;
+    if (queued <= room)
+      for (int n = tid; n < queued * plan.cell_vecs; n += G) {
+        const int v = queue[n / plan.cell_vecs] + n % plan.cell_vecs * G;
         if (v >= v1) continue;
         float part[kV];
         unpack(__ldg(vec + v), part);
 #pragma unroll
         for (int e = 0; e < kV; ++e) offer(part[e], span.head + v * kV + e);
       }
-    }
-    Gr::sync();
-    const int found = sh.queued <= room ? sh.found : room + 1;
-    uint64_t* list = C > 1 ? lists + rank * K : lists;  // this slice's K largest in order
+    uint64_t* list = lists + rank * K;  // this slice's K largest in order
     for (int k = tid; k < K; k += G) list[k] = 0;
-    Gr::sync();
+    group_sync<G>();
+    const int found = queued <= room ? sh.found : room + 1;
     if (found <= room) {
       for (int n = tid; n < found; n += G) {
         const uint64_t mine = cand[n];
@@ -462,13 +528,13 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
       }
     } else {
       // More elements above the bound than there is room for: large values that keep to few
-      // threads' cells. K rounds of "the largest below the last one" over the slice.
-      uint64_t last = ~0ull;
+      // cells. K rounds of "the largest below the last one" over the slice.
+      uint64_t before = ~0ull;
       for (int k = 0; k < K; ++k) {
         uint64_t best = 0;
         auto look = [&](float v, int at) {
           const uint64_t q = top_key(v, at);
-          if (q < last && q > best) best = q;
+          if (q < before && q > best) best = q;
         };
         if (edge >= 0) look(edge_x, edge);
         for (int v = v0 + tid; v < v1; v += G) {
@@ -485,10 +551,10 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
           for (int w = 0; w < kWarps; ++w) best = sh.best[w] > best ? sh.best[w] : best;
         }
         if (tid == 0) list[k] = best;
-        last = best;
+        before = best;
       }
     }
-    Gr::sync();
+    group_sync<G>();
   }
 
   if (C > 1) {
@@ -504,8 +570,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
-    st = sh.part[0];
-    for (int r = 1; r < C; ++r) st = soft_merge(st, sh.part[r], c);
+    st = soft_join((threadIdx.x & 31) < C ? sh.part[threadIdx.x & 31] : soft_empty(), c);
   }
 
   const float ln_s = ln_sum(st);
@@ -517,13 +582,13 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
       int place = n % K;
       for (int r = 0; r < C; ++r) {  // and how many of the other slices' lists come before it
         if (r == n / K) continue;
-        int lo = 0, hi = K;
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if (lists[r * K + mid] > mine) lo = mid + 1;
-          else hi = mid;
+        int left = 0, right = K;
+        while (left < right) {
+          const int mid = (left + right) / 2;
+          if (lists[r * K + mid] > mine) left = mid + 1;
+          else right = mid;
         }
-        place += lo;
+        place += left;
       }
       if (place < K) {
         a.top_index[row * K + place] = key_index(mine);
@@ -642,18 +707,21 @@ int sm_count_here() {
   return sm_count(dev);
 }
 
-template <typename T, int G, int U>
+template <typename T, int G>
 int launch_forward(const TokenLogprobsArgs& a, int cluster, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
   ForwardPlan plan;
   plan.cluster = cluster;
-  const int64_t vecs = (a.V / kVec<T> + cluster - 1) / cluster;
-  const int64_t batches = std::max<int64_t>(1, (vecs + G * U - 1) / (G * U));
-  plan.cell_batches = static_cast<int>((batches + kMaxCells - 1) / kMaxCells);
-  plan.cells = static_cast<int>((batches + plan.cell_batches - 1) / plan.cell_batches);
+  // vectors that a thread reads of its slice; a cell for each in a warp's row while they are few
+  const int64_t mine = std::max<int64_t>(1, ((a.V / kVec<T> + cluster - 1) / cluster + G - 1) / G);
+  const int64_t batches = (mine + kUnroll - 1) / kUnroll;
+  plan.cell_vecs = G == 32 && mine <= kWarpCells
+                       ? 1
+                       : static_cast<int>((batches + kMaxCells - 1) / kMaxCells) * kUnroll;
+  plan.cells = static_cast<int>((mine + plan.cell_vecs - 1) / plan.cell_vecs);
   constexpr int kGroups = kThreads / G;
   const size_t smem = kGroups * group_smem<T, G>(static_cast<int>(a.K), plan.cells, cluster);
-  auto* kern = a.K > 0 ? token_logprobs_kernel<T, G, U, true> : token_logprobs_kernel<T, G, U, false>;
+  auto* kern = a.K > 0 ? token_logprobs_kernel<T, G, true> : token_logprobs_kernel<T, G, false>;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                static_cast<int>(smem));
@@ -692,14 +760,14 @@ int forward_by_size(const TokenLogprobsArgs& a, cudaStream_t stream) {
   if (a.V <= 512) return launch_short<T, 16>(a, stream);
   if (a.V <= kShort) return launch_short<T, 32>(a, stream);
   // Many rows of a middling length: a warp each.
-  if (a.V <= kWarpRow && a.K <= kWarpTop && rows >= kWarpRows * sm_count_here())
-    return launch_forward<T, 32, kUnroll>(a, 1, stream);
+  if (a.V <= kWarpRow && a.K <= kWarpList && rows >= kWarpRows * sm_count_here())
+    return launch_forward<T, 32>(a, 1, stream);
   // Few rows: split each until there are some CTAs for every SM or a slice is one batch.
   int cluster = 1;
   while (cluster < kMaxCluster && rows * cluster < 4 * sm_count_here() &&
          vecs / (2 * cluster) >= kThreads * kUnroll)
     cluster *= 2;
-  return launch_forward<T, kThreads, kUnroll>(a, cluster, stream);
+  return launch_forward<T, kThreads>(a, cluster, stream);
 }
 
 template <typename T>
