@@ -9,16 +9,19 @@
 //
 // A slot with token < 0 is empty; a repeated token's masses add; a row of weight 0 is not read.
 // The unlisted tokens are summed by themselves, so that s keeps its digits when the list holds
-// nearly everything. A row's slice is copied to shared memory (cp.async), the listed tokens are
-// struck out there (-inf), the rest is summed from it and, in the same call, turned into the
-// gradient from it, so that the logits cross HBM once. A warp takes a short row; else a CTA, or a
-// cluster whose CTAs hold a slice each and exchange their sums through distributed shared memory.
-// The backward from stored statistics has nothing to sum and streams.
+// nearly everything.
 //
-// Repeated tokens are found while striking out: every slot writes its number in place of its token's
-// logit and reads it back, and where one finds another's number the masses are added up by a search
-// (K^2 comparisons, which as a rule cost more than the row itself and are seldom needed).
+// A row that a warp takes passes through shared memory: the listed tokens are struck out there (-inf),
+// the rest is summed from it and turned into the gradient from it. Repeated tokens are found on the
+// way: every slot writes its number in place of its token's logit and reads it back.
+// A longer row is streamed by a CTA, or by a cluster whose CTAs take a slice each and exchange their
+// sums through distributed shared memory; a bit per element in shared memory says what is listed (and
+// was set twice for a repeated token). For the gradient the slice is streamed again: the slices in
+// flight are 64 KB for each of some 600 CTAs, so that the second read finds them in L2.
+// Where a token is repeated its masses are added up by a search (K^2 comparisons, seldom needed).
+// The backward from stored statistics has nothing to sum.
 #include <algorithm>
+#include <cstdlib>
 #include <string>
 
 #include "bdh_sm100.h"
@@ -34,8 +37,10 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kPiece = 16384;             // elements of a row per CTA of the streaming backward
+constexpr int kWarpRowBytes = 8 * 1024;  // longest row that a warp takes
+constexpr int kWarpRows = 16;             // rows for every SM from which it does
 constexpr int kSliceBytes = 68 * 1024;    // of a row per CTA, while the cluster may grow
-static_assert(kThreads >= kTopMax, "one thread per slot");
+
 
 constexpr int kStats = 8;  // floats per row: see RowStats
 
@@ -49,12 +54,17 @@ struct RowStats {
 };
 static_assert(sizeof(RowStats) == kStats * sizeof(float), "stored as it is");
 
-// What the gradient needs of a row: dx_i = 2^(c (x_i - m) + shift) coef for unlisted tokens.
+// What the gradient needs of a row. Unlisted tokens: the map below, with a tail relative to their own
+// sum s, however small it is: p_i (total - r / s) = (p_i / s) (total s - r).
 struct RowGradient {
-  float m, shift, coef;        // unlisted: with a tail relative to their own sum s, however small
-  float top_m, top_shift;      // listed: p = 2^(c (z - top_m) + top_shift)
-  float scale, total;          // listed: scale (p total - mass)
-  bool none;                   // no logit above -inf in the row
+  float top_m, top_l2;   // listed: p = 2^(c (z - top_m) - top_l2), scale (p total - mass)
+  float scale, total;
+  float m, l2, coef;     // unlisted
+  bool none;             // no logit above -inf in the row
+  __device__ __forceinline__ RowMap unlisted(float c) const { return RowMap(c, m, l2, coef, 0.0f); }
+  __device__ __forceinline__ float listed(float z, float mass, float c) const {
+    return scale * (ex2(fmaf(z - top_m, c, -top_l2)) * total - mass);
+  }
 };
 __device__ __forceinline__ RowGradient row_gradient(const RowStats& st, int tail, float inv_t,
                                                     float scale) {
@@ -62,47 +72,20 @@ __device__ __forceinline__ RowGradient row_gradient(const RowStats& st, int tail
   g.none = st.m == neg_inf();
   g.scale = scale * inv_t;
   g.total = st.total + st.r;
-  g.top_m = st.m;
-  g.top_shift = -st.ln_s * kLog2e;
-  g.m = st.m;
-  g.shift = g.top_shift;
+  g.top_m = g.m = st.m;
+  g.top_l2 = g.l2 = st.ln_s * kLog2e;
   g.coef = g.scale * g.total;
   if (tail) {
-    // p_i (total - r / s) = (p_i / s) (total s - r); nothing is unlisted and above -inf: all zeros
     const float s = expf((st.rest_m - st.m) * inv_t + st.ln_rest - st.ln_s);
-    const bool empty = st.rest_m == neg_inf();
+    const bool empty = st.rest_m == neg_inf();  // nothing unlisted above -inf: zeros
     g.m = empty ? 0.0f : st.rest_m;
-    g.shift = empty ? neg_inf() : -st.ln_rest * kLog2e;
+    g.l2 = empty ? 0.0f : st.ln_rest * kLog2e;
     g.coef = empty ? 0.0f : g.scale * (g.total * s - st.r);
     if (g.total != g.total) g.coef = g.total;
   }
+  if (g.none) g.m = g.l2 = 0.0f;
   return g;
 }
-__device__ __forceinline__ float listed_gradient(const RowGradient& g, float z, float mass, float c) {
-  return g.scale * (ex2(fmaf(z - g.top_m, c, g.top_shift)) * g.total - mass);
-}
-// The formula for unlisted tokens, on one element and on two.
-struct Unlisted {
-  RowGradient g;
-  float c;
-  F2 nm2, c2, shift2, coef2;
-  __device__ __forceinline__ Unlisted(const RowGradient& g_, float c_)
-      : g(g_), c(c_), nm2(f2(-g_.m, -g_.m)), c2(f2(c_, c_)), shift2(f2(g_.shift, g_.shift)),
-        coef2(f2(g_.coef, g_.coef)) {}
-  __device__ __forceinline__ float operator()(float x) const {
-    return ex2(fmaf(x - g.m, c, g.shift)) * g.coef;
-  }
-  __device__ __forceinline__ void operator()(float x0, float x1, float& d0, float& d1) const {
-    float y0, y1;
-    f2_split(f2_fma(f2_add(f2(x0, x1), nm2), c2, shift2), y0, y1);
-    f2_split(f2_mul(f2(ex2(y0), ex2(y1)), coef2), d0, d1);
-  }
-};
-struct Nothing {
-  __device__ __forceinline__ float operator()(float) const { return 0.0f; }
-  __device__ __forceinline__ void operator()(float, float, float& a, float& b) const { a = b = 0.0f; }
-};
-
 // Loss of a row from its list (one warp; `slot(f)` calls f(ln q, q, z) for the lane's slots).
 template <typename Slots>
 __device__ __forceinline__ float warp_loss(const RowStats& st, float inv_t, Slots slots) {
@@ -137,6 +120,10 @@ __device__ __forceinline__ int get_slot(const float* p, int64_t at) {
 }
 __device__ __forceinline__ int get_slot(const uint16_t* p, int64_t at) { return p[at]; }
 
+struct Nothing {
+  __device__ __forceinline__ float operator()(float) const { return 0.0f; }
+};
+
 template <typename T>
 __device__ __forceinline__ float row_weight(const DistillTopkArgs& a, int64_t o, int64_t i) {
   return a.weight.p != nullptr ? a.weight.p[o * a.weight.strides[0] + i * a.weight.strides[1]] : 1.0f;
@@ -162,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, E <= 16 && S == 1 ? 4 : 3) distill_s
              : nullptr;
   const float w = row_weight<T>(a, o, i);
   if (w == 0.0f) {
-    if (d != nullptr) map_row<T, 32>(x, d, V, lane, true, Nothing(), Nothing());
+    if (d != nullptr) map_row<T, 32>(x, d, V, lane, true, Nothing());
     if (lane == 0) a.loss[row] = 0.0f;
     return;
   }
@@ -297,8 +284,8 @@ __global__ void __launch_bounds__(kThreads, E <= 16 && S == 1 ? 4 : 3) distill_s
   if (d == nullptr) return;
 
   const RowGradient g = row_gradient(st, a.tail, inv_t, w);
-  const Unlisted f(g, c);
-  if (edge >= 0) logit_put(d, edge, g.none ? 0.0f : f(edge_x));
+  const RowMap f = g.unlisted(c);
+  if (edge >= 0) logit_put(d, edge, g.none ? 0.0f : f.plain(edge_x));
   T* out = d + span.head;
   const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
 #pragma unroll
@@ -307,10 +294,7 @@ __global__ void __launch_bounds__(kThreads, E <= 16 && S == 1 ? 4 : 3) distill_s
     if (v >= span.vecs) continue;
     float ds[kV];
 #pragma unroll
-    for (int e = 0; e < kV; e += 2) {
-      f(xs[u * kV + e], xs[u * kV + e + 1], ds[e], ds[e + 1]);
-      if (g.none) ds[e] = ds[e + 1] = 0.0f;
-    }
+    for (int e = 0; e < kV; ++e) ds[e] = g.none ? 0.0f : f.plain(xs[u * kV + e]);
     if (aligned) {
       store_vec(out + v * kV, ds);
     } else {
@@ -322,187 +306,91 @@ __global__ void __launch_bounds__(kThreads, E <= 16 && S == 1 ? 4 : 3) distill_s
   __syncwarp();
 #pragma unroll
   for (int s = 0; s < S; ++s)
-    if (!(mass[s] < 0.0f)) logit_put(d, at[s], listed_gradient(g, z[s], mass[s], c));
+    if (!(mass[s] < 0.0f)) logit_put(d, at[s], g.listed(z[s], mass[s], c));
 }
 
-// ------------------------------------------------------------ a CTA or a cluster for a row
-struct CtaShared {
-  float2 part[kMaxCluster * kWarps];  // maximum and sum of every warp of the cluster
-  int repeated[kMaxCluster];          // a token is twice in the list, and in that CTA's slice
-  SoftState top;                      // softmax state of the listed tokens
+// ------------------------------------------------------------------ the list of a longer row
+struct RowShared {
+  SoftState top;  // softmax state of the listed tokens
   float total, r, shift;
-  int index[kTopMax];  // -1: empty slot; V: a token past the vocabulary
-  float lnq[kTopMax], q[kTopMax], z[kTopMax];
-  float mass[kTopMax];  // q summed over the slots of the same token; below 0: not its first slot
+  int pad[2];
 };
-static_assert(sizeof(CtaShared) % 4 == 0, "the slice follows, aligned");
-constexpr size_t kCtaShared = (sizeof(CtaShared) + 15) & ~size_t(15);
+struct List {   // arrays of list_room(K)
+  int* index;   // -1: empty slot; V: a token past the vocabulary
+  float* lnq;
+  float* q;
+  float* z;     // the student's logit
+  float* mass;  // q summed over the slots of the same token; below 0: not its first slot
+};
+__host__ __device__ constexpr int list_room(int K) { return (K + 31) / 32 * 32; }
+__host__ __device__ constexpr size_t list_bytes(int K) {
+  return 5 * sizeof(float) * static_cast<size_t>(list_room(K));
+}
+__device__ __forceinline__ List list_at(uint8_t* p, int K) {
+  float* f = reinterpret_cast<float*>(p);
+  const int room = list_room(K);
+  return {reinterpret_cast<int*>(f), f + room, f + 2 * room, f + 3 * room, f + 4 * room};
+}
 
-// Masses of repeated tokens to the first slot of each, and the listed tokens' softmax state
-// (one warp).
-__device__ __forceinline__ void list_state(CtaShared& sh, int K, int V, int lane, float c, bool repeated) {
+// q, the masses and the totals of the list in shared memory (one warp).
+__device__ __forceinline__ void list_masses(RowShared& sh, const List& l, int K, int V, int tail, int lane) {
+  float m = neg_inf(), shift = 0.0f, total = 0.0f;
+  if (!tail) {
+    for (int j = lane; j < K; j += 32) m = max_nan(m, l.lnq[j]);
+    m = warp_max(m);
+    if (m != neg_inf()) {
+      float s = 0.0f;
+      for (int j = lane; j < K; j += 32) s += expf(l.lnq[j] - m);
+      shift = m + logf(warp_sum(s));
+    }
+  }
+  bool bad = false;
+  for (int j = lane; j < K; j += 32) {
+    const int at = l.index[j];
+    const float lq = l.lnq[j] - shift, q = expf(lq);
+    l.lnq[j] = lq;
+    l.q[j] = q;
+    l.mass[j] = at >= 0 && at < V ? q : -1.0f;
+    total += q;
+    bad |= at == V;
+  }
+  total = warp_sum(total);
+  bad = __any_sync(0xffffffffu, bad);
+  if (lane == 0) {
+    sh.total = bad ? quiet_nan() : total;  // a token past the vocabulary: NaN throughout
+    sh.r = tail ? max_nan(0.0f, 1.0f - total) : 0.0f;
+    sh.shift = shift;
+  }
+}
+// The listed tokens' softmax state (one warp); with `repeated`, of each token's first slot, to which
+// the masses of the others go.
+__device__ __forceinline__ void list_state(RowShared& sh, const List& l, int K, int V, int lane, float c,
+                                           bool repeated) {
   float zs[kTopMax / 32];
 #pragma unroll
   for (int s = 0; s < kTopMax / 32; ++s) {
     const int j = s * 32 + lane;
     zs[s] = neg_inf();
     if (j >= K) continue;
-    const int at = sh.index[j];
-    const bool token = at >= 0 && at < V;
-    float mass = token ? sh.q[j] : -1.0f;
-    if (repeated && token) {
-      mass = 0.0f;
-      bool first = true;
+    const int at = l.index[j];
+    bool first = at >= 0 && at < V;
+    if (repeated && first) {
+      float mass = 0.0f;
       for (int k = 0; k < K; ++k)
-        if (sh.index[k] == at) {
-          mass += sh.q[k];
+        if (l.index[k] == at) {
+          mass += l.q[k];
           if (k < j) first = false;
         }
-      if (!first) mass = -1.0f;
+      l.mass[j] = first ? mass : -1.0f;
     }
-    sh.mass[j] = mass;
-    if (!(mass < 0.0f)) zs[s] = sh.z[j];
+    if (first) zs[s] = l.z[j];
   }
   const SoftState top = soft_of_warp<false>(zs, neg_inf(), c);
   if (lane == 0) sh.top = top;
 }
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillTopkArgs a, int C) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  constexpr int kV = kVec<T>;
-  CtaShared& sh = *reinterpret_cast<CtaShared*>(smem);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int V = static_cast<int>(a.V), K = static_cast<int>(a.K);
-  const uint32_t rank = C > 1 ? cta_rank() : 0;
-  const int64_t row = blockIdx.x / static_cast<uint32_t>(C);
-  const int64_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
-  const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
-  T* d = a.dlogits != nullptr
-             ? static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1]
-             : nullptr;
-
-  // This CTA's slice: vectors [v0, v1) between the row's 16-byte boundaries, the row's head with
-  // the first slice and its tail with the last; n elements from `from`.
-  const RowSpan span = row_span(x, V);
-  const int per = (span.vecs + C - 1) / C;
-  const int v0 = min(static_cast<int>(rank) * per, span.vecs), v1 = min(v0 + per, span.vecs);
-  const int head = rank == 0 ? span.head : 0, tail = rank == C - 1 ? span.tail : 0;
-  const int from = span.head + v0 * kV - head, vecs = v1 - v0, n = head + vecs * kV + tail;
-
-  const float w = row_weight<T>(a, o, i);
-  if (w == 0.0f) {  // the whole cluster
-    if (d != nullptr) map_row<T, kThreads>(x + from, d + from, n, tid, true, Nothing(), Nothing());
-    if (tid == 0 && rank == 0) a.loss[row] = 0.0f;
-    return;
-  }
-  if (C > 1) cluster_arrive();  // shared memory may be written once all CTAs have started
-
-  T* held = reinterpret_cast<T*>(smem + kCtaShared) + (kV - head) % kV;  // element from + e: held[e]
-  const uint4* vec = reinterpret_cast<const uint4*>(x + span.head) + v0;
-  uint4* hvec = reinterpret_cast<uint4*>(held + head);
-  for (int v = tid; v < vecs; v += kThreads)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hvec + v)), "l"(vec + v)
-                 : "memory");
-  const int edge = tid < head ? tid : tid - head < tail ? n - tail + tid - head : -1;
-  if (edge >= 0) held[edge] = x[from + edge];
-  if (tid < K) {
-    const int at = slot_token(a.index[o * a.i_strides[0] + i * a.i_strides[1] + tid * a.i_strides[2]], V);
-    const float t = a.teacher[o * a.t_strides[0] + i * a.t_strides[1] + tid * a.t_strides[2]];
-    sh.index[tid] = at;
-    sh.lnq[tid] = at >= 0 ? t : neg_inf();
-    sh.z[tid] = at >= 0 && at < V ? logit_at<T>(x, at) : neg_inf();
-  }
-  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
-  asm volatile("cp.async.wait_all;" ::: "memory");
-  __syncthreads();  // the slice and the list are in shared memory
-  auto in_slice = [&](int at) { return at >= from && at < from + n; };
-  if (warp == 0) {  // strike the listed tokens out
-    for (int j = lane; j < K; j += 32)
-      if (in_slice(sh.index[j])) put_slot(held, sh.index[j] - from, j);
-    __syncwarp();
-    bool other = false;
-    for (int j = lane; j < K; j += 32)
-      if (in_slice(sh.index[j])) other |= get_slot(held, sh.index[j] - from) != j;
-    other = __any_sync(0xffffffffu, other);  // and all have read
-    for (int j = lane; j < K; j += 32)
-      if (in_slice(sh.index[j])) logit_put(held, sh.index[j] - from, neg_inf());
-    if (lane == 0) sh.repeated[rank] = other ? 1 : 0;
-  } else if (warp == 1) {  // the list's masses
-    float m = neg_inf(), shift = 0.0f, total = 0.0f;
-    if (!a.tail) {
-      for (int j = lane; j < K; j += 32) m = max_nan(m, sh.lnq[j]);
-      m = warp_max(m);
-      if (m != neg_inf()) {
-        float s = 0.0f;
-        for (int j = lane; j < K; j += 32) s += expf(sh.lnq[j] - m);
-        shift = m + logf(warp_sum(s));
-      }
-    }
-    bool bad = false;
-    for (int j = lane; j < K; j += 32) {
-      const float l = sh.lnq[j] - shift, q = expf(l);
-      sh.lnq[j] = l;
-      sh.q[j] = q;
-      total += q;
-      bad |= sh.index[j] == V;
-    }
-    total = warp_sum(total);
-    bad = __any_sync(0xffffffffu, bad);
-    if (lane == 0) {
-      sh.total = bad ? quiet_nan() : total;  // a token past the vocabulary: NaN throughout
-      sh.r = a.tail ? max_nan(0.0f, 1.0f - total) : 0.0f;
-      sh.shift = shift;
-    }
-    __syncwarp();
-    list_state(sh, K, V, lane, c, false);
-  }
-  __syncthreads();
-
-  SoftState rest = soft_empty();
-  if (edge >= 0) soft_add(rest, logit_at<T>(held, edge), c);
-  SoftSums sums(rest);
-  const float slack = kBaseSlack / c;
-  for (int b = 0; b < vecs; b += kThreads * kUnroll) {
-    uint4 wv[kUnroll];
-    if (b + kThreads * kUnroll <= vecs) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) wv[u] = hvec[b + u * kThreads + tid];
-    } else {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int v = b + u * kThreads + tid;
-        wv[u] = v < vecs ? hvec[v] : void_vec<T>();
-      }
-    }
-    sums.add<false, T>(wv, max_of(wv, T()), c, slack);
-  }
-  rest = sums.state();
-  rest = soft_join(rest, c);
-  if (C > 1) {  // every warp's state to every CTA of the cluster
-    cluster_wait();
-    if (lane < C) {
-      const uint32_t to = peer_smem(&sh.part[rank * kWarps + warp], lane);
-      peer_store(to, rest.m);
-      peer_store(to + 4, rest.s);
-      if (warp == 0) peer_store(peer_smem(&sh.repeated[rank], lane), __int_as_float(sh.repeated[rank]));
-    }
-    cluster_arrive();
-    cluster_wait();
-  } else {
-    if (lane == 0) sh.part[warp] = make_float2(rest.m, rest.s);
-    __syncthreads();
-  }
-  rest = soft_empty();
-  for (int k = lane; k < C * kWarps; k += 32)
-    rest = soft_merge(rest, {sh.part[k].x, sh.part[k].y, 0.0f}, c);
-  rest = soft_join(rest, c);
-  const bool repeated = __any_sync(0xffffffffu, lane < C && sh.repeated[lane] != 0);
-  if (repeated) {  // in every CTA of the cluster
-    __syncthreads();
-    if (warp == 1) list_state(sh, K, V, lane, c, true);
-    __syncthreads();
-  }
+// The row's statistics from the unlisted tokens' state.
+__device__ __forceinline__ RowStats row_stats(const RowShared& sh, const SoftState& rest, bool repeated,
+                                              float c) {
   const SoftState all = soft_merge(rest, {sh.top.m, sh.top.s, 0.0f}, c);
   RowStats st;
   st.m = all.m;
@@ -513,40 +401,364 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillTopkArgs 
   st.r = sh.r;
   st.shift = sh.shift;
   st.repeated = repeated ? 1.0f : 0.0f;
-  if (rank == 0 && warp == 0) {
-    const float loss = warp_loss(st, inv_t, [&](auto f) {
-      for (int j = lane; j < K; j += 32) f(sh.lnq[j], sh.q[j], sh.z[j]);
-    });
-    if (lane == 0) {
-      a.loss[row] = w * loss;
-      if (a.stats != nullptr) *reinterpret_cast<RowStats*>(a.stats + kStats * row) = st;
-    }
+  return st;
+}
+__device__ __forceinline__ void write_loss(const DistillTopkArgs& a, const RowStats& st, const List& l,
+                                           int64_t row, float w, float inv_t, int lane) {
+  const int K = static_cast<int>(a.K);
+  const float loss = warp_loss(st, inv_t, [&](auto f) {
+    for (int j = lane; j < K; j += 32) f(l.lnq[j], l.q[j], l.z[j]);
+  });
+  if (lane == 0) {
+    a.loss[row] = w * loss;
+    if (a.stats != nullptr) *reinterpret_cast<RowStats*>(a.stats + kStats * row) = st;
   }
+}
+
+// ------------------------------------------------------------------ a warp for a middling row
+// Bytes of the row: its vectors, and one more each for the row's head and tail.
+template <typename T>
+__host__ __device__ constexpr size_t held_bytes(int64_t V) {
+  return (static_cast<size_t>(V / kVec<T>) + 2) * 16;
+}
+__host__ __device__ constexpr size_t held_at(int K) {
+  return (sizeof(RowShared) + list_bytes(K) + 15) & ~size_t(15);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 5) distill_warp_kernel(DistillTopkArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int kV = kVec<T>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int V = static_cast<int>(a.V), K = static_cast<int>(a.K);
+  const uint32_t row32 = blockIdx.x * kWarps + warp;
+  const int64_t row = row32;
+  if (row >= a.outer * a.inner) return;
+  const int64_t o = row32 / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
+  const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
+  T* d = a.dlogits != nullptr
+             ? static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1]
+             : nullptr;
+  uint8_t* base = smem + warp * (held_at(K) + held_bytes<T>(V));
+  RowShared& sh = *reinterpret_cast<RowShared*>(base);
+  const List l = list_at(base + sizeof(RowShared), K);
+  const RowSpan span = row_span(x, V);
+  const float w = row_weight<T>(a, o, i);
+  T* held = reinterpret_cast<T*>(base + held_at(K)) + (kV - span.head) % kV;
+  const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
+  uint4* hvec = reinterpret_cast<uint4*>(held + span.head);
+  for (int v = lane; v < span.vecs; v += 32)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hvec + v)), "l"(vec + v)
+                 : "memory");
+  const int edge = lane < span.head               ? lane
+                   : lane - span.head < span.tail ? V - span.tail + lane - span.head
+                                                  : -1;
+  if (edge >= 0) held[edge] = x[edge];
+  for (int j = lane; j < K; j += 32) {
+    const int at = slot_token(a.index[o * a.i_strides[0] + i * a.i_strides[1] + j * a.i_strides[2]], V);
+    const float t = a.teacher[o * a.t_strides[0] + i * a.t_strides[1] + j * a.t_strides[2]];
+    l.index[j] = at;
+    l.lnq[j] = at >= 0 ? t : neg_inf();
+  }
+  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (w == 0.0f) {  // (the row was on its way before its weight was there)
+    if (d != nullptr) map_row<T, 32>(x, d, V, lane, true, Nothing());
+    if (lane == 0) a.loss[row] = 0.0f;
+    return;
+  }
+  __syncwarp();
+  auto is_token = [&](int at) { return at >= 0 && at < V; };
+  for (int j = lane; j < K; j += 32) l.z[j] = is_token(l.index[j]) ? logit_at<T>(held, l.index[j]) : neg_inf();
+  __syncwarp();
+  for (int j = lane; j < K; j += 32)
+    if (is_token(l.index[j])) put_slot(held, l.index[j], j);
+  __syncwarp();
+  bool repeated = false;
+  for (int j = lane; j < K; j += 32)
+    if (is_token(l.index[j])) repeated |= get_slot(held, l.index[j]) != j;
+  repeated = __any_sync(0xffffffffu, repeated);  // and all have read
+  for (int j = lane; j < K; j += 32)
+    if (is_token(l.index[j])) logit_put(held, l.index[j], neg_inf());
+  list_masses(sh, l, K, V, a.tail, lane);
+  __syncwarp();
+  list_state(sh, l, K, V, lane, c, repeated);
+  __syncwarp();
+
+  SoftSums<false> sums;
+  const float slack = kBaseSlack / c;
+  for (int b = 0; b < span.vecs; b += 32 * kUnroll) {
+    uint4 wv[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int v = b + u * 32 + lane;
+      wv[u] = v < span.vecs ? hvec[v] : void_vec<T>();
+    }
+    sums.add<T>(wv, max_of(wv, T()), c, slack);
+  }
+  SoftState rest = sums.wide ? soft_slowly<T, 32>(hvec, 0, span.vecs, lane, c) : sums.state(c);
+  if (edge >= 0) soft_add(rest, logit_at<T>(held, edge), c);
+  rest = soft_join(rest, c);
+  const RowStats st = row_stats(sh, rest, repeated, c);
+  write_loss(a, st, l, row, w, inv_t, lane);
   if (d == nullptr) return;
 
   const RowGradient g = row_gradient(st, a.tail, inv_t, w);
-  const Unlisted f(g, c);
-  T* out = d + from + head;
-  if ((reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
-    if (edge >= 0) logit_put(d, from + edge, g.none ? 0.0f : f(logit_at<T>(held, edge)));
-    for (int v = tid; v < vecs; v += kThreads) {
+  const RowMap f = g.unlisted(c);
+  T* out = d + span.head;
+  if ((reinterpret_cast<uintptr_t>(out) & 15u) == 0 && !f.wide) {
+    if (edge >= 0) logit_put(d, edge, g.none ? 0.0f : f(logit_at<T>(held, edge)));
+    for (int v = lane; v < span.vecs; v += 32) {
       float xs[kV], ds[kV];
       unpack(hvec[v], xs);
 #pragma unroll
-      for (int e = 0; e < kV; e += 2) {
-        f(xs[e], xs[e + 1], ds[e], ds[e + 1]);
-        if (g.none) ds[e] = ds[e + 1] = 0.0f;
-      }
+      for (int e = 0; e < kV; ++e) ds[e] = g.none ? 0.0f : f(xs[e]);
       store_vec(out + static_cast<int64_t>(v) * kV, ds);
     }
   } else {  // x and d lie differently in their vectors
-    for (int e = tid; e < n; e += kThreads)
-      logit_put(d, from + e, g.none ? 0.0f : f(logit_at<T>(held, e)));
+    for (int e = lane; e < V; e += 32) logit_put(d, e, g.none ? 0.0f : f.of(logit_at<T>(held, e)));
   }
   if (g.none) return;
+  __syncwarp();
+  for (int j = lane; j < K; j += 32)
+    if (is_token(l.index[j]) && !(l.mass[j] < 0.0f))
+      logit_put(d, l.index[j], g.listed(l.z[j], l.mass[j], c));
+}
+
+// ------------------------------------------------------------------ a CTA or a cluster for a long row
+struct CtaShared {
+  float2 part[kMaxCluster * kWarps];  // base and sum of every warp of the cluster
+  int repeated[kMaxCluster];          // a token is twice in the list, and in that CTA's slice
+  uint32_t edge_bits;                 // which of the row's ends are listed, a bit per element
+  RowShared row;
+  RowGradient gradient;
+};
+// The slice's bits: a byte per vector, the vectors of a thread's batch in one word.
+__host__ __device__ constexpr size_t bits_at(int K) {
+  return (sizeof(CtaShared) + list_bytes(K) + 15) & ~size_t(15);
+}
+template <typename T>
+__host__ __device__ constexpr int slice_batches(int64_t V, int cluster) {
+  return static_cast<int>(((V / kVec<T> + cluster - 1) / cluster + kThreads * kUnroll - 1) /
+                          (kThreads * kUnroll));
+}
+static_assert(kUnroll == 4, "a batch's bytes make a word");
+
+// -inf in the places of a vector that the bits name.
+__device__ __forceinline__ void strike(uint4& w, uint32_t bits, float) {
+  if (bits & 1) w.x = 0xff800000u;
+  if (bits & 2) w.y = 0xff800000u;
+  if (bits & 4) w.z = 0xff800000u;
+  if (bits & 8) w.w = 0xff800000u;
+}
+__device__ __forceinline__ uint32_t strike_pair(uint32_t w, uint32_t bits) {
+  if (bits & 1) w = (w & 0xffff0000u) | 0xff80u;
+  if (bits & 2) w = (w & 0xffffu) | 0xff800000u;
+  return w;
+}
+__device__ __forceinline__ void strike(uint4& w, uint32_t bits, uint16_t) {
+  w.x = strike_pair(w.x, bits);
+  w.y = strike_pair(w.y, bits >> 2);
+  w.z = strike_pair(w.z, bits >> 4);
+  w.w = strike_pair(w.w, bits >> 6);
+}
+
+// kThreads threads stream; one warp more has the list.
+template <typename T>
+__global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTopkArgs a, int C) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int kV = kVec<T>, kStep = kThreads * kUnroll;
+  CtaShared& sh = *reinterpret_cast<CtaShared*>(smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool lister = warp == kWarps;
+  const int V = static_cast<int>(a.V), K = static_cast<int>(a.K);
+  const List l = list_at(smem + sizeof(CtaShared), K);
+  uint32_t* bits = reinterpret_cast<uint32_t*>(smem + bits_at(K));
+  const uint32_t rank = C > 1 ? cta_rank() : 0;
+  const uint32_t row32 = blockIdx.x / static_cast<uint32_t>(C);
+  const int64_t row = row32;
+  const int64_t o = row32 / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
+  const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
+  T* d = a.dlogits != nullptr
+             ? static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1]
+             : nullptr;
+  if (C > 1) cluster_arrive();  // shared memory may be written once all CTAs have started
+  // This CTA's slice: vectors [v0, v1) between the row's 16-byte boundaries, the row's head with
+  // the first slice and its tail with the last; n elements from `from`.
+  const float w = row_weight<T>(a, o, i);
+  const RowSpan span = row_span(x, V);
+  const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
+  const int per = (span.vecs + C - 1) / C;
+  const int v0 = min(static_cast<int>(rank) * per, span.vecs), v1 = min(v0 + per, span.vecs);
+  const int head = rank == 0 ? span.head : 0, tail = rank == C - 1 ? span.tail : 0;
+  const int from = span.head + v0 * kV - head, n = head + (v1 - v0) * kV + tail;
+  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
+
+  uint4 next[kUnroll];
+  int edge = -1;
+  float edge_x = neg_inf();
+  int slot_at[kTopMax / 32];  // the lister's slots
+  if (!lister) {
+    load_batch<T, kThreads>(next, vec, v0, v1, tid);
+    edge = tid < head ? from + tid : tid - head < tail ? V - tail + tid - head : -1;
+    if (edge >= 0) edge_x = logit_at<T>(x, edge);
+    for (int k = tid; k < slice_batches<T>(V, C) * kThreads; k += kThreads) bits[k] = 0;
+    if (tid == 0) sh.edge_bits = 0;
+  } else {
+#pragma unroll
+    for (int s = 0; s < kTopMax / 32; ++s) {
+      const int j = s * 32 + lane;
+      slot_at[s] = -1;
+      if (j >= K) continue;
+      slot_at[s] = slot_token(a.index[o * a.i_strides[0] + i * a.i_strides[1] + j * a.i_strides[2]], V);
+      const float t = a.teacher[o * a.t_strides[0] + i * a.t_strides[1] + j * a.t_strides[2]];
+      l.index[j] = slot_at[s];
+      l.lnq[j] = slot_at[s] >= 0 ? t : neg_inf();
+    }
+  }
+  if (w == 0.0f) {  // the whole cluster; a batch of the row was on its way
+    if (!lister && d != nullptr)
+      map_row<T, kThreads>(x + from, d + from, n, tid, true, Nothing());
+    if (tid == 0 && rank == 0) a.loss[row] = 0.0f;
+    if (C > 1) cluster_wait();
+    return;
+  }
   __syncthreads();
-  if (tid < K && in_slice(sh.index[tid]) && !(sh.mass[tid] < 0.0f))
-    logit_put(d, sh.index[tid], listed_gradient(g, sh.z[tid], sh.mass[tid], c));
+  auto in_slice = [&](int at) { return at >= from && at < from + n; };  // (and below V)
+  if (lister) {
+    bool repeated = false;
+#pragma unroll
+    for (int s = 0; s < kTopMax / 32; ++s) {
+      const int at = slot_at[s];
+      if (!in_slice(at)) continue;
+      const int e = at - from - head, v = e >= 0 ? e / kV : -1;
+      uint32_t bit, before;
+      if (e < 0 || v >= v1 - v0) {  // an end: bits as the threads that hold them
+        bit = 1u << (e < 0 ? at - from : head + at - (V - tail));
+        before = atomicOr(&sh.edge_bits, bit);
+      } else {
+        const int in_batch = v % kStep;
+        bit = 1u << (in_batch / kThreads * 8 + e % kV);
+        before = atomicOr(&bits[v / kStep * kThreads + in_batch % kThreads], bit);
+      }
+      repeated |= (before & bit) != 0;
+    }
+    __syncthreads();  // the bits are set
+    // While the others stream: the list; then, of all, the row's statistics and what the gradient needs.
+#pragma unroll
+    for (int s = 0; s < kTopMax / 32; ++s) {
+      const int at = slot_at[s];
+      if (s * 32 + lane < K) l.z[s * 32 + lane] = at >= 0 && at < V ? logit_at<T>(x, at) : neg_inf();
+    }
+    repeated = __any_sync(0xffffffffu, repeated);
+    list_masses(sh.row, l, K, V, a.tail, lane);
+    __syncwarp();
+    list_state(sh.row, l, K, V, lane, c, false);
+    if (C > 1) {
+      cluster_wait();
+      if (lane < C) peer_store(peer_smem(&sh.repeated[rank], lane), __int_as_float(repeated ? 1 : 0));
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      if (lane == 0) sh.repeated[0] = repeated ? 1 : 0;
+      __syncthreads();
+    }
+    repeated = __any_sync(0xffffffffu, lane < C && sh.repeated[lane] != 0);
+    if (repeated) list_state(sh.row, l, K, V, lane, c, true);  // in every CTA of the cluster
+    SoftState rest = soft_empty();
+    for (int k = lane; k < C * kWarps; k += 32)
+      rest = soft_merge(rest, {sh.part[k].x, sh.part[k].y, 0.0f}, c);
+    rest = soft_join(rest, c);
+    __syncwarp();
+    const RowStats st = row_stats(sh.row, rest, repeated, c);
+    const RowGradient g = row_gradient(st, a.tail, inv_t, w);
+    if (d != nullptr) {
+      if (lane == 0) sh.gradient = g;
+      __syncthreads();
+    }
+    if (rank == 0) write_loss(a, st, l, row, w, inv_t, lane);
+    if (d == nullptr || g.none) return;
+    __syncthreads();  // the unlisted tokens' gradients are written
+    for (int j = lane; j < K; j += 32)
+      if (in_slice(l.index[j]) && !(l.mass[j] < 0.0f))
+        logit_put(d, l.index[j], g.listed(l.z[j], l.mass[j], c));
+    return;
+  }
+
+  __syncthreads();  // the bits are set
+  SoftSums<false> sums;
+  const float slack = kBaseSlack / c;
+  const uint32_t* my_bits = bits + tid;
+  stream<T, kThreads>(next, vec, v0, v1, tid, [&](uint4 (&wv)[kUnroll], int) {
+    const uint32_t struck = *my_bits;
+    my_bits += kThreads;
+    if (struck != 0) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) strike(wv[u], struck >> 8 * u, T());
+    }
+    sums.add<T>(wv, max_of(wv, T()), c, slack);
+  });
+  if (d != nullptr) load_batch<T, kThreads>(next, vec, v0, v1, tid);  // again, for the gradient
+  SoftState rest = soft_empty();
+  if (!sums.wide) {
+    rest = sums.state(c);
+  } else {
+#pragma unroll 1
+    for (int v = v0 + tid, at = 0; v < v1; v += kThreads, ++at)
+#pragma unroll 1
+      for (int e = 0; e < kV; ++e)
+        if ((bits[at / kUnroll * kThreads + tid] >> (at % kUnroll * 8 + e) & 1) == 0)
+          soft_add(rest, logit_at<T>(reinterpret_cast<const T*>(vec), static_cast<int64_t>(v) * kV + e), c);
+  }
+  if (edge >= 0 && (sh.edge_bits >> tid & 1) == 0) soft_add(rest, edge_x, c);
+  {
+    const float m = warp_max(rest.m);
+    if (m != neg_inf()) soft_raise(rest, m, c);
+    rest.s = warp_sum(rest.s);
+  }
+  if (C > 1) {  // every warp's state to every CTA of the cluster
+    cluster_wait();
+    if (lane < C) {
+      const uint32_t to = peer_smem(&sh.part[rank * kWarps + warp], lane);
+      peer_store(to, rest.m);
+      peer_store(to + 4, rest.s);
+    }
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    if (lane == 0) sh.part[warp] = make_float2(rest.m, rest.s);
+    __syncthreads();
+  }
+  if (d == nullptr) return;
+  __syncthreads();
+  const RowGradient& g = sh.gradient;
+  const bool none = g.none;
+  const RowMap f = g.unlisted(c);
+  if (edge >= 0) logit_put(d, edge, none ? 0.0f : f.of(edge_x));
+  if (f.wide || none) {
+    map_row<T, kThreads>(x + from + head, d + from + head, n - head - tail, tid, none, f);
+  } else {
+    T* out = d + span.head;
+    const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+    stream<T, kThreads>(next, vec, v0, v1, tid, [&](const uint4 (&wv)[kUnroll], int b) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int v = b + u * kThreads + tid;
+        if (v >= v1) break;
+        float xs[kV], ds[kV];
+        unpack(wv[u], xs);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) ds[e] = ex2(fmaf(xs[e], f.c, -f.b)) * f.k0;
+        if (aligned) {
+          store_vec(out + static_cast<int64_t>(v) * kV, ds);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kV; ++e) logit_put(out, static_cast<int64_t>(v) * kV + e, ds[e]);
+        }
+      }
+    });
+  }
+  if (!none) __syncthreads();
 }
 
 // --------------------------------------------------- the gradient from the forward's statistics
@@ -565,15 +777,14 @@ __global__ void __launch_bounds__(kThreads) distill_topk_bwd_kernel(DistillTopkA
   T* d = static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1];
   const float w = row_weight<T>(a, o, i);
   if (w == 0.0f) {
-    map_row<T, G>(x + from, d + from, n, tid, true, Nothing(), Nothing());
+    map_row<T, G>(x + from, d + from, n, tid, true, Nothing());
     return;
   }
   const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
   const RowStats st = *reinterpret_cast<const RowStats*>(a.stats + kStats * row);
   const float up = a.g_loss.p[o * a.g_loss.strides[0] + i * a.g_loss.strides[1]];
   const RowGradient g = row_gradient(st, a.tail, inv_t, w * up);
-  const Unlisted f(g, c);
-  map_row<T, G>(x + from, d + from, n, tid, g.none, f, f);
+  map_row<T, G>(x + from, d + from, n, tid, g.none, g.unlisted(c));
   if (g.none) return;
   if (G == 32) __syncwarp();
   else __syncthreads();
@@ -594,7 +805,7 @@ __global__ void __launch_bounds__(kThreads) distill_topk_bwd_kernel(DistillTopkA
         }
       if (!first) continue;
     }
-    logit_put(d, at, listed_gradient(g, logit_at<T>(x, at), mass, c));
+    logit_put(d, at, g.listed(logit_at<T>(x, at), mass, c));
   }
 }
 
@@ -615,6 +826,13 @@ int launch_short(const DistillTopkArgs& a, cudaStream_t stream) {
   return launch_check("distill_topk launch", cudaSuccess);
 }
 
+int allow_smem(const void* kern, size_t smem) {
+  if (smem <= 48 * 1024) return BDH_OK;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  return e == cudaSuccess ? BDH_OK : launch_check("distill_topk shared memory", e);
+}
+
 template <typename T>
 int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
   if (a.V <= 256) return launch_short<T, 8>(a, stream);
@@ -622,27 +840,29 @@ int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
   if (a.V <= kShort) return launch_short<T, 32>(a, stream);
   int dev = 0;
   cudaGetDevice(&dev);
+  const int K = static_cast<int>(a.K);
   const int64_t rows = a.outer * a.inner, bytes = a.V * static_cast<int64_t>(sizeof(T));
+  if (bytes <= kWarpRowBytes && rows >= kWarpRows * sm_count(dev)) {
+    const size_t smem = kWarps * (held_at(K) + held_bytes<T>(a.V));
+    if (int rc = allow_smem(reinterpret_cast<const void*>(distill_warp_kernel<T>), smem)) return rc;
+    distill_warp_kernel<T><<<static_cast<unsigned>((rows + kWarps - 1) / kWarps), kThreads, smem, stream>>>(a);
+    return launch_check("distill_topk launch", cudaSuccess);
+  }
   int cluster = 1;
   while (cluster < kMaxCluster &&
-         (bytes > static_cast<int64_t>(cluster) * kSliceBytes ||
+         (bytes > static_cast<int64_t>(cluster) * (getenv("SLICE") ? atoi(getenv("SLICE")) : kSliceBytes) ||
           (rows * cluster < 4 * sm_count(dev) && bytes >= cluster * int64_t(32768))))
     cluster *= 2;
   if (rows * cluster >= int64_t(1) << 31) {
     set_error("distill_topk: too many rows for this vocabulary");
     return BDH_ERR_INVALID;
   }
-  // a slice's vectors, and one more for the row's head and one for its tail
-  const size_t smem = kCtaShared + (static_cast<size_t>((a.V / kVec<T> + cluster - 1) / cluster) + 2) * 16;
-  auto* kern = distill_topk_kernel<T>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem));
-    if (e != cudaSuccess) return launch_check("distill_topk shared memory", e);
-  }
+  const size_t smem = bits_at(K) + static_cast<size_t>(slice_batches<T>(a.V, cluster)) * kThreads * kUnroll;
+  auto* kern = distill_cta_kernel<T>;
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * cluster));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kThreads + 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

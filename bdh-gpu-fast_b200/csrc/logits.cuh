@@ -2,14 +2,18 @@
 // distill_topk.cu): element access, the running softmax state of a row and the order of a row's
 // top list.
 //
-// With c = log2(e) / temperature and the row's running maximum m (of the raw logits), a part of
-// a row is summed as
+// With c = log2(e) / temperature and a base m near the row's largest logit, a part of a row is
+// summed as
 //   s = sum 2^(c (x - m)),   a = sum 2^(c (x - m)) c (x - m)
 // so that the row's log normaliser is  m / temperature + ln s  and its entropy  ln s - ln2 a / s.
-// Differences x - m are formed before the scaling: a row filled with the type's lowest value (a
-// mask) then gives zeros, where c x - c m would overflow. Exponents are clamped at -200, where
-// 2^t is already 0 in fp32, so that a masked (-inf) element adds 0 to both sums, not -inf * 0.
-// Maxima are the NaN-propagating ones: a NaN logit ends up in every result of its row.
+// Exponents are clamped at -200, where 2^t is already 0 in fp32, so that a masked (-inf) element adds
+// 0 to both sums, not -inf * 0. Maxima are the NaN-propagating ones: a NaN logit ends up in every
+// result of its row.
+//
+// The inner loops take c x - b with a whole number b near c m: one fused multiply-add, exact but for
+// its last rounding (c m itself would be rounded, by 2^-24 |c m| for the whole sum), and rescaling by
+// powers of two. Where |c m| is past kWide that has no digits left, or overflows (a row filled with
+// the type's lowest value as a mask): such rows take the differences x - m before the scaling.
 #pragma once
 
 #include <cstdint>
@@ -80,35 +84,6 @@ __device__ __forceinline__ RowSpan row_span(const T* p, int n) {
   return r;
 }
 
-// Two fp32 in a register pair: sm_100's packed arithmetic does both with one instruction, each
-// rounded as its scalar form.
-struct F2 {
-  uint64_t v;
-};
-__device__ __forceinline__ F2 f2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void f2_split(const F2& x, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
-}
-__device__ __forceinline__ F2 f2_add(const F2& a, const F2& b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 f2_mul(const F2& a, const F2& b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 f2_fma(const F2& a, const F2& b, const F2& c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-
 // The elements of a 16-byte vector as fp32.
 __device__ __forceinline__ void unpack(const uint4& u, float (&x)[4]) {
   x[0] = __uint_as_float(u.x);
@@ -171,11 +146,38 @@ __device__ __forceinline__ uint4 void_vec<uint16_t>() {
 
 constexpr int kUnroll = 4;  // vectors that a thread has in flight (a batch)
 
-// d[i] = f(x[i]) for n elements by a group of G threads: `pair` on two elements, `single` on one,
-// or zeros. Vectors where x and d lie alike; else vectors are read and elements written.
-template <typename T, int G, typename Single, typename Pair>
-__device__ __forceinline__ void map_row(const T* x, T* d, int n, int tid, bool zero, Single single,
-                                        Pair pair) {
+// A group of G threads over the vectors [v0, v1): f(w, b) for every batch w of its kUnroll vectors
+// b + u G + tid (-inf past the end), with the next batch's loads under way meanwhile. `next` is the
+// batch at v0, asked for by the caller (load_batch) as early as it can.
+template <typename T, int G>
+__device__ __forceinline__ void load_batch(uint4 (&w)[kUnroll], const uint4* vec, int b, int v1, int tid) {
+  if (b + G * kUnroll <= v1) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) w[u] = __ldg(vec + b + u * G + tid);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int v = b + u * G + tid;
+      w[u] = v < v1 ? __ldg(vec + v) : void_vec<T>();
+    }
+  }
+}
+template <typename T, int G, typename F>
+__device__ __forceinline__ void stream(uint4 (&next)[kUnroll], const uint4* vec, int v0, int v1, int tid, F f) {
+  constexpr int kStep = G * kUnroll;
+  for (int b = v0; b < v1; b += kStep) {
+    uint4 w[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) w[u] = next[u];
+    if (b + kStep < v1) load_batch<T, G>(next, vec, b + kStep, v1, tid);
+    f(w, b);
+  }
+}
+
+// d[i] = f(x[i]) for n elements by a group of G threads, or zeros without reading. Vectors where x and
+// d lie alike; else vectors are read and elements written.
+template <typename T, int G, typename F>
+__device__ __forceinline__ void map_row(const T* x, T* d, int n, int tid, bool zero, F f) {
   constexpr int kV = kVec<T>;
   const RowSpan span = row_span(x, n);
   const bool aligned = (reinterpret_cast<uintptr_t>(d + span.head) & 15u) == 0;
@@ -183,7 +185,7 @@ __device__ __forceinline__ void map_row(const T* x, T* d, int n, int tid, bool z
   T* out = d + span.head;
   for (int e = tid; e < span.head + span.tail; e += G) {
     const int at = e < span.head ? e : n - span.tail + (e - span.head);
-    logit_put(d, at, zero ? 0.0f : single(logit_at<T>(x, at)));
+    logit_put(d, at, zero ? 0.0f : f(logit_at<T>(x, at)));
   }
   for (int b = 0; b < span.vecs; b += G * kUnroll) {
     uint4 w[kUnroll];
@@ -203,7 +205,7 @@ __device__ __forceinline__ void map_row(const T* x, T* d, int n, int tid, bool z
       } else {
         unpack(w[u], xs);
 #pragma unroll
-        for (int e = 0; e < kV; e += 2) pair(xs[e], xs[e + 1], ds[e], ds[e + 1]);
+        for (int e = 0; e < kV; ++e) ds[e] = f(xs[e]);
       }
       if (aligned) {
         store_vec(out + static_cast<int64_t>(v) * kV, ds);
@@ -218,7 +220,7 @@ __device__ __forceinline__ void map_row(const T* x, T* d, int n, int tid, bool z
 // Softmax state of a part of a row: maximum, sum, and exponent-weighted sum (see above).
 struct SoftState {
   float m, s, a;
-};
+};  // m: a value of the row, -inf for none above it
 __device__ __forceinline__ SoftState soft_empty() { return {neg_inf(), 0.0f, 0.0f}; }
 __device__ __forceinline__ void soft_add(SoftState& st, float x, float c) {
   const float m = max_nan(st.m, x);
@@ -242,7 +244,7 @@ __device__ __forceinline__ SoftState soft_merge(const SoftState& x, const SoftSt
   const float fx = ex2(dx), fy = ex2(dy);
   return {m, fmaf(x.s, fx, y.s * fy), fmaf(fx, fmaf(dx, x.s, x.a), fy * fmaf(dy, y.s, y.a))};
 }
-// Raise the state's maximum to m (not below it; NaN stays).
+// Raise the state's base to m (not below it; NaN stays).
 __device__ __forceinline__ void soft_raise(SoftState& st, float m, float c) {
   const float d = max_nan((st.m - m) * c, kExpFloor);
   const float f = ex2(d);
@@ -250,82 +252,125 @@ __device__ __forceinline__ void soft_raise(SoftState& st, float m, float c) {
   st.s *= f;
   st.m = m;
 }
-// Add N elements none of which is above the state's maximum, which is not -inf.
-template <bool ENTROPY, int N>
-__device__ __forceinline__ void soft_sum(SoftState& st, const float (&x)[N], float c) {
-  const F2 nm = f2(-st.m, -st.m), cc = f2(c, c);
-  F2 s = f2(0.0f, 0.0f), a = f2(0.0f, 0.0f);
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    float t0, t1;
-    f2_split(f2_mul(f2_add(f2(x[i], x[i + 1]), nm), cc), t0, t1);
-    if (ENTROPY) {
-      t0 = max_nan(t0, kExpFloor);
-      t1 = max_nan(t1, kExpFloor);
-    }
-    const F2 e = f2(ex2(t0), ex2(t1));
-    s = f2_add(s, e);
-    if (ENTROPY) a = f2_fma(e, f2(t0, t1), a);
-  }
-  float s0, s1, a0, a1;
-  f2_split(s, s0, s1);
-  st.s += s0 + s1;
-  if (ENTROPY) {
-    f2_split(a, a0, a1);
-    st.a += a0 + a1;
-  }
-}
 
-// A thread's running softmax state over vectors: the two sums in pairs, and a base m that is a value
-// of the row but may be below its largest by up to kBaseSlack in the exponent, so that the sums are
-// rescaled a few times a row and not whenever a new maximum comes (terms stay below 2^kBaseSlack).
+constexpr float kWide = 4194304.0f;  // 2^22
+// 2^n for a whole n <= 0.
+__device__ __forceinline__ float pow2(float n) {
+  return n < -126.0f ? 0.0f : __int_as_float((static_cast<int>(n) + 127) << 23);
+}
+// A thread's running sums over vectors. The base may be below the largest element so far by up to
+// kBaseSlack in the exponent (terms stay below 2^kBaseSlack), so that the sums are rescaled a few
+// times a row and not whenever a new maximum comes. A thread that meets a base it cannot use stops
+// and says so (`wide`); its part is then summed with soft_add.
 constexpr float kBaseSlack = 8.0f;
+template <bool ENTROPY>
 struct SoftSums {
-  float m;
-  F2 s, a;
-  __device__ __forceinline__ explicit SoftSums(const SoftState& st)
-      : m(st.m), s(f2(st.s, 0.0f)), a(f2(st.a, 0.0f)) {}
-  // N vectors whose largest element is `largest`.
-  template <bool ENTROPY, typename T, int N>
-  __device__ __forceinline__ void add(const uint4 (&w)[N], float largest, float c, float slack) {
-    if (!(largest <= m + slack)) {  // a NaN too
-      const float to = max_nan(largest, m);
-      const float d = max_nan((m - to) * c, kExpFloor), f = ex2(d);
-      const F2 ff = f2(f, f);
-      if (ENTROPY) a = f2_mul(ff, f2_fma(f2(d, d), s, a));
-      s = f2_mul(ff, s);
-      m = to;
+  float m = neg_inf(), limit = neg_inf(), base = 0.0f;  // the base's element, the largest it serves
+  float s[2] = {0.0f, 0.0f}, a[2] = {0.0f, 0.0f};
+  bool wide = false;
+  __device__ __forceinline__ void raise(float largest, float c, float slack) {
+    const float b = largest * c;
+    if (!(fabsf(b) < kWide)) {  // NaN too
+      wide = true;
+      return;
     }
-    if (m == neg_inf()) return;
-    const F2 nm = f2(-m, -m), cc = f2(c, c);
-    F2 ps = f2(0.0f, 0.0f), pa = f2(0.0f, 0.0f);
+    const float to = rintf(b);
+    if (m != neg_inf()) {
+      const float d = base - to, f = pow2(d);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (ENTROPY) a[i] = f * fmaf(max_nan(d, kExpFloor), s[i], a[i]);
+        s[i] *= f;
+      }
+    }
+    base = to;
+    m = largest;
+    limit = largest + slack;
+  }
+  // N vectors whose largest element is `largest`.
+  template <typename T, int N>
+  __device__ __forceinline__ void add(const uint4 (&w)[N], float largest, float c, float slack) {
+    if (!(largest <= limit)) raise(largest, c, slack);  // a NaN too
+    if (wide || m == neg_inf()) return;
+    float ps[2] = {0.0f, 0.0f}, pa[2] = {0.0f, 0.0f};  // (a batch's own sums: fewer terms in a row)
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       float x[kVec<T>];
       unpack(w[u], x);
 #pragma unroll
-      for (int i = 0; i < kVec<T>; i += 2) {
-        float t0, t1;
-        f2_split(f2_mul(f2_add(f2(x[i], x[i + 1]), nm), cc), t0, t1);
-        if (ENTROPY) {
-          t0 = max_nan(t0, kExpFloor);
-          t1 = max_nan(t1, kExpFloor);
-        }
-        const F2 e = f2(ex2(t0), ex2(t1));
-        ps = f2_add(ps, e);
-        if (ENTROPY) pa = f2_fma(e, f2(t0, t1), pa);
+      for (int i = 0; i < kVec<T>; ++i) {
+        const float t = fmaf(x[i], c, -base), e = ex2(t);
+        ps[i % 2] += e;
+        if (ENTROPY) pa[i % 2] = fmaf(e, max_nan(t, kExpFloor), pa[i % 2]);
       }
     }
-    s = f2_add(s, ps);
-    if (ENTROPY) a = f2_add(a, pa);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s[i] += ps[i];
+      if (ENTROPY) a[i] += pa[i];
+    }
   }
-  __device__ __forceinline__ SoftState state() const {
-    float s0, s1, a0, a1;
-    f2_split(s, s0, s1);
-    f2_split(a, a0, a1);
-    return {m, s0 + s1, a0 + a1};
+  __device__ __forceinline__ SoftState state(float c) const {
+    if (m == neg_inf()) return soft_empty();
+    const float t = fmaf(m, c, -base), f = ex2(-t), sum = s[0] + s[1];
+    return {m, sum * f, ENTROPY ? f * fmaf(-t, sum, a[0] + a[1]) : 0.0f};
   }
 };
+// The same for a thread's part of the vectors [v0, v1) where it was too wide.
+template <typename T, int G>
+__device__ __forceinline__ SoftState soft_slowly(const uint4* vec, int v0, int v1, int tid, float c) {
+  SoftState st = soft_empty();
+  const T* x = reinterpret_cast<const T*>(vec);
+#pragma unroll 1
+  for (int v = v0 + tid; v < v1; v += G)
+#pragma unroll 1
+    for (int e = 0; e < kVec<T>; ++e) soft_add(st, logit_at<T>(x, static_cast<int64_t>(v) * kVec<T> + e), c);
+  return st;
+}
+
+// An element's exponential times what the row has for all: p (k0 + k1 log2 p) with
+// log2 p = c (x - m) - l2, for a row's base m and log2 sum l2. As 2^t (K0 + K1 t) with t = c x - b.
+struct RowMap {
+  float c, b, k0, k1;
+  float m, l2, w0, w1;  // the plain form, for a wide row
+  bool wide, with_log;
+  __device__ __forceinline__ RowMap(float c_, float m_, float l2_, float w0_, float w1_)
+      : c(c_), m(m_), l2(l2_), w0(w0_), w1(w1_) {
+    wide = !(fabsf(m * c) < kWide);
+    with_log = w1 != 0.0f;  // NaN counts
+    b = rintf(m * c);
+    const float shift = -fmaf(m, c, -b) - l2, f = exp2f(shift);
+    k0 = fmaf(w1, shift, w0) * f;
+    k1 = w1 * f;
+  }
+  __device__ __forceinline__ float plain(float x) const {
+    const float y = fmaf(x - m, c, -l2);
+    return ex2(y) * (with_log ? fmaf(w1, max_nan(y, kExpFloor), w0) : w0);
+  }
+  __device__ __forceinline__ float of(float x) const { return wide ? plain(x) : (*this)(x); }
+  __device__ __forceinline__ float operator()(float x) const {
+    const float t = fmaf(x, c, -b);
+    return ex2(t) * (with_log ? fmaf(k1, max_nan(t, kExpFloor), k0) : k0);
+  }
+};
+// d = map(x) for n elements of a row by a group of G threads. A warp's rows are short and do not wait
+// for arithmetic: the plain form, in which a single token's probability is exactly 1.
+template <typename T, int G>
+__device__ __forceinline__ void map_row(const T* x, T* d, int n, int tid, bool zero, const RowMap& map) {
+  if (G == 32) {
+    map_row<T, G>(x, d, n, tid, zero, [&](float v) { return map.plain(v); });
+  } else if (map.wide && !zero) {
+#pragma unroll 1
+    for (int e = tid; e < n; e += G) logit_put(d, e, map.of(logit_at<T>(x, e)));
+  } else if (map.with_log) {
+    map_row<T, G>(x, d, n, tid, zero, [&](float v) {
+      const float t = fmaf(v, map.c, -map.b);
+      return ex2(t) * fmaf(map.k1, max_nan(t, kExpFloor), map.k0);
+    });
+  } else {
+    map_row<T, G>(x, d, n, tid, zero, [&](float v) { return ex2(fmaf(v, map.c, -map.b)) * map.k0; });
+  }
+}
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -352,13 +397,18 @@ __device__ __forceinline__ SoftState soft_of_warp(const float (&x)[N], float edg
   float m = edge;
 #pragma unroll
   for (int i = 0; i < N; ++i) m = max_nan(m, x[i]);
-  SoftState st = {warp_max(m), 0.0f, 0.0f};
-  if (st.m == neg_inf()) return st;
-  soft_sum<ENTROPY>(st, x, c);
-  const float t = max_nan((edge - st.m) * c, kExpFloor), e = ex2(t);
-  st.s = warp_sum(st.s + e);
-  if (ENTROPY) st.a = warp_sum(fmaf(e, t, st.a));
-  return st;
+  m = warp_max(m);
+  if (m == neg_inf()) return soft_empty();
+  float t = max_nan((edge - m) * c, kExpFloor), e = ex2(t);
+  float s = e, a = e * t;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    t = max_nan((x[i] - m) * c, kExpFloor);
+    e = ex2(t);
+    s += e;
+    if (ENTROPY) a = fmaf(e, t, a);
+  }
+  return {m, warp_sum(s), ENTROPY ? warp_sum(a) : 0.0f};
 }
 
 // Order of a row's top list: larger values first, an equal value's lower index first; -0 equals

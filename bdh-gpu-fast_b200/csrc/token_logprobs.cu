@@ -319,29 +319,15 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
   const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
   const int per = (span.vecs + C - 1) / C;
   const int v0 = min(static_cast<int>(rank) * per, span.vecs), v1 = min(v0 + per, span.vecs);
-  uint4 next[U];
-  auto load = [&](int b) {
-    if (b + G * U <= v1) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) next[u] = __ldg(vec + b + u * G + tid);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int v = b + u * G + tid;
-        next[u] = v < v1 ? __ldg(vec + v) : void_vec<T>();
-      }
-    }
-  };
-  load(v0);
+  uint4 first[U];
+  load_batch<T, G>(first, vec, v0, v1, tid);
   Token tok = {false, true, 0.0f};
   if (tid == 0 && rank == 0 && a.tokens != nullptr) tok = load_token(a, x, o, i);
   int edge = -1;  // this thread's element of the row's ends
   if (rank == 0 && tid < span.head) edge = tid;
   if (rank == C - 1 && tid >= 8 && tid - 8 < span.tail) edge = V - span.tail + tid - 8;
   const float edge_x = edge >= 0 ? logit_at<T>(x, edge) : neg_inf();
-  SoftState st = soft_empty();
-  if (edge >= 0) soft_add(st, edge_x, c);
-  SoftSums sums(st);
+  SoftSums<true> sums;
 
   int cell = 0, in_cell = 0;          // TOP: cells written, vectors in the open one
   uint32_t own = 0;                   // largest key of the thread
@@ -351,11 +337,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
     cells[cell++ * G + tid] = k;
     own = max(own, k);
   };
-  for (int b = v0; b < v1; b += G * U) {
-    uint4 w[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = next[u];
-    if (b + G * U < v1) load(b + G * U);
+  stream<T, G>(first, vec, v0, v1, tid, [&](const uint4 (&w)[U], int b) {
     float largest;
     if (TOP && plan.cell_vecs == 1) {
       largest = neg_inf();
@@ -378,9 +360,11 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
         }
       }
     }
-    sums.add<true, T>(w, largest, c, slack);
-  }
-  st = soft_join(sums.state(), c);
+    sums.add<T>(w, largest, c, slack);
+  });
+  SoftState st = sums.wide ? soft_slowly<T, G>(vec, v0, v1, tid, c) : sums.state(c);
+  if (edge >= 0) soft_add(st, edge_x, c);
+  st = soft_join(st, c);
   if (G > 32) {
     if ((threadIdx.x & 31) == 0) sh.warp_part[threadIdx.x >> 5] = st;
     __syncthreads();
@@ -651,30 +635,16 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(TokenLogpr
     else __syncthreads();
     for (int k = 1; k <= K; ++k) sum -= sh.add[k];
   }
-  // With y = log2 p: p (sum - g_entropy (ln p + entropy)) / temperature = 2^y (k0 + k1 y)
-  const float shift = none ? 0.0f : -ln_s * kLog2e, m0 = none ? 0.0f : m;
-  const float k0 = (sum - g_ent * ent) * inv_t, k1 = -g_ent * kLn2 * inv_t;
-  const bool with_y = g_ent != 0.0f;  // NaN counts
-  const F2 nm2 = f2(-m0, -m0), c2 = f2(c, c), shift2 = f2(shift, shift);
-  auto dense = [&](float v) {
-    const float y = fmaf(v - m0, c, shift);
-    return with_y ? ex2(y) * fmaf(k1, max_nan(y, kExpFloor), k0) : ex2(y) * k0;
-  };
-  auto pair = [&](float x0, float x1, float& d0, float& d1) {
-    float y0, y1;
-    f2_split(f2_fma(f2_add(f2(x0, x1), nm2), c2, shift2), y0, y1);
-    const F2 p = f2(ex2(y0), ex2(y1));
-    F2 w = f2(k0, k0);
-    if (with_y) w = f2_fma(f2(k1, k1), f2(max_nan(y0, kExpFloor), max_nan(y1, kExpFloor)), w);
-    f2_split(f2_mul(p, w), d0, d1);
-  };
-  map_row<T, G>(x + from, d + from, n, tid, none, dense, pair);
+  // p (sum - g_entropy (ln p + entropy)) / temperature
+  const RowMap dense(c, none ? 0.0f : m, none ? 0.0f : ln_s * kLog2e, (sum - g_ent * ent) * inv_t,
+                     -g_ent * kLn2 * inv_t);
+  map_row<T, G>(x + from, d + from, n, tid, none, dense);
   if (none) return;
   if (K == 0) {
     if (tok < from || tok >= from + n) return;
     if (G == 32) __syncwarp();
     else __syncthreads();
-    if (tid == 0) logit_put(d, tok, fmaf(g_tok, inv_t, dense(logit_at<T>(x, tok))));
+    if (tid == 0) logit_put(d, tok, fmaf(g_tok, inv_t, (G == 32 ? dense.plain(logit_at<T>(x, tok)) : dense.of(logit_at<T>(x, tok)))));
     return;
   }
   if (G == 32) __syncwarp();
@@ -688,7 +658,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(TokenLogpr
         mine = j > k;
         add += sh.add[j];
       }
-    if (mine) logit_put(d, at, fmaf(add, inv_t, dense(logit_at<T>(x, at))));
+    if (mine) logit_put(d, at, fmaf(add, inv_t, (G == 32 ? dense.plain(logit_at<T>(x, at)) : dense.of(logit_at<T>(x, at)))));
   }
 }
 

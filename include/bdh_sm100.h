@@ -428,10 +428,10 @@ int bdh_token_logprobs_bwd(const void* logits, int dtype, const int64_t l_stride
  * has loss +inf and gradient 0.
  * bdh_distill_topk writes the loss per row and, with dlogits, the gradient of the sum of the losses
  * in the same call (the logits are read from memory once); stats (8 floats per row, 16-byte aligned, may be null) is
- * what bdh_distill_topk_bwd reads, which multiplies the gradient of each row by g_loss. A row is
- * held in the shared memory of up to 8 CTAs, so V is at most BDH_DISTILL_VOCAB_MAX.
+ * what bdh_distill_topk_bwd reads, which multiplies the gradient of each row by g_loss. A bit per
+ * token is held in the shared memory of up to 8 CTAs, so V is at most BDH_DISTILL_VOCAB_MAX.
  */
-#define BDH_DISTILL_VOCAB_MAX 393216
+#define BDH_DISTILL_VOCAB_MAX 2097152
 int bdh_distill_topk(const void* logits, int dtype, const int64_t l_strides[2],
                      const int64_t* index, const int64_t i_strides[3], const float* teacher,
                      const int64_t t_strides[3], const float* weight, const int64_t w_strides[2],

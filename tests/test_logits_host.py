@@ -111,7 +111,7 @@ def test_distill_entries_refuse_on_the_host():
                                     None, s, 1, inner, V, K, T, 0, None)
 
     for kw, word in (({"dtype": 2}, b"dtype"), ({"K": 0}, b"at least one"), ({"K": 200}, b"BDH_TOP_MAX"),
-                     ({"V": 393217}, b"BDH_DISTILL_VOCAB_MAX"),
+                     ({"V": 2097153}, b"BDH_DISTILL_VOCAB_MAX"),
                      ({"V": -3}, b"negative"), ({"T": 0.0}, b"temperature"), ({"index": None}, b"null")):
         assert fwd(**kw) == 1, kw
         assert word in lib.bdh_last_error()
