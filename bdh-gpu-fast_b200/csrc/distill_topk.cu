@@ -21,7 +21,6 @@
 // Where a token is repeated its masses are added up by a search (K^2 comparisons, seldom needed).
 // The backward from stored statistics has nothing to sum.
 #include <algorithm>
-#include <cstdlib>
 #include <string>
 
 #include "bdh_sm100.h"
@@ -37,8 +36,9 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kPiece = 16384;             // elements of a row per CTA of the streaming backward
-constexpr int kWarpRowBytes = 8 * 1024;  // longest row that a warp takes
-constexpr int kWarpRows = 16;             // rows for every SM from which it does
+constexpr int kWarpRowBytes = 24 * 1024;  // longest row that a warp takes
+constexpr int kWarpRows = 8;               // rows for every SM from which it does
+constexpr int kWarpsHeld = 4;              // rows of a CTA then
 constexpr int kSliceBytes = 68 * 1024;    // of a row per CTA, while the cluster may grow
 
 
@@ -86,16 +86,16 @@ __device__ __forceinline__ RowGradient row_gradient(const RowStats& st, int tail
   if (g.none) g.m = g.l2 = 0.0f;
   return g;
 }
-// Loss of a row from its list (one warp; `slot(f)` calls f(ln q, q, z) for the lane's slots).
-template <typename Slots>
-__device__ __forceinline__ float warp_loss(const RowStats& st, float inv_t, Slots slots) {
+// Loss of a row from its list (L lanes; `slots(f)` calls f(ln q, q, z) for the lane's slots).
+template <int L, typename Slots>
+__device__ __forceinline__ float row_loss(const RowStats& st, float inv_t, Slots slots) {
   const bool none = st.m == neg_inf();
   float loss = 0.0f;
   slots([&](float lnq, float q, float z) {
     const float lp = none || z == neg_inf() ? neg_inf() : (z - st.m) * inv_t - st.ln_s;
     if (!(q <= 0.0f)) loss = fmaf(q, lnq - lp, loss);
   });
-  loss = warp_sum(loss);
+  loss = warp_sum<L>(loss);
   if (st.r > 0.0f) {
     const float ls = st.rest_m == neg_inf() ? neg_inf()
                                             : (st.rest_m - st.m) * inv_t + st.ln_rest - st.ln_s;
@@ -128,52 +128,54 @@ template <typename T>
 __device__ __forceinline__ float row_weight(const DistillTopkArgs& a, int64_t o, int64_t i) {
   return a.weight.p != nullptr ? a.weight.p[o * a.weight.strides[0] + i * a.weight.strides[1]] : 1.0f;
 }
-// ------------------------------------------------------------------ a warp for a short row
-// Rows of at most kShort elements: the slots and the row's elements stay in the lanes' registers
-// (S slots, E elements and one of the row's unaligned ends); the row passes through shared memory
-// for the slots to find their logits.
+// ------------------------------------------------------------------ lanes for a short row
+// Rows of at most kShort elements: the slots and the row's elements stay in registers, S slots and E
+// elements (and up to two of its unaligned ends) in each of the L lanes that have a row; the row passes
+// through shared memory for the slots to find their logits. With few lanes a row the shuffles and the
+// row's own figures serve several rows at once (a byte model's 256: 4 rows a warp).
 constexpr int kShort = 1024;
 
-template <typename T, int E, int S>
-__global__ void __launch_bounds__(kThreads, E <= 16 && S == 1 ? 4 : 3) distill_short_kernel(DistillTopkArgs a) {
-  constexpr int kV = kVec<T>, kVecs = E / kV;
-  __shared__ __align__(16) T rows_held[kWarps][(kVecs * 32 + 2) * kV];
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (row >= a.outer * a.inner) return;
-  const int64_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
+template <typename T, int L, int E, int S>
+__global__ void __launch_bounds__(kThreads) distill_short_kernel(DistillTopkArgs a, FastDiv inner) {
+  constexpr int kV = kVec<T>, kVecs = E / kV, kEnds = L < 16 ? 2 : 1, kN = E + kEnds;
+  __shared__ __align__(16) T rows_held[kThreads / L][(kVecs * L + 2) * kV];
+  const int lane = threadIdx.x % L, rows = static_cast<int>(a.outer * a.inner);
+  int row = static_cast<int>(blockIdx.x * (kThreads / L) + threadIdx.x / L);
+  const bool live = row < rows;
+  if (!__any_sync(0xffffffffu, live)) return;
+  if (!live) row = rows - 1;  // (the warp's other rows need these lanes)
+  int o, i;
+  inner.divmod(row, o, i);
   const int V = static_cast<int>(a.V), K = static_cast<int>(a.K);
   const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
-  T* d = a.dlogits != nullptr
-             ? static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1]
-             : nullptr;
   const float w = row_weight<T>(a, o, i);
-  if (w == 0.0f) {
-    if (d != nullptr) map_row<T, 32>(x, d, V, lane, true, Nothing());
-    if (lane == 0) a.loss[row] = 0.0f;
-    return;
-  }
   // the row on its way to shared memory, the list to registers
   const RowSpan span = row_span(x, V);
-  T* held = rows_held[threadIdx.x >> 5] + (kV - span.head) % kV;
+  T* held = rows_held[threadIdx.x / L] + (kV - span.head) % kV;
   const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
   uint4* hvec = reinterpret_cast<uint4*>(held + span.head);
 #pragma unroll
   for (int u = 0; u < kVecs; ++u) {
-    const int v = u * 32 + lane;
+    const int v = u * L + lane;
     if (v < span.vecs)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hvec + v)), "l"(vec + v)
                    : "memory");
   }
-  int edge = -1;  // this lane's element of the row's ends
-  if (lane < span.head) edge = lane;
-  if (lane >= 8 && lane - 8 < span.tail) edge = V - span.tail + lane - 8;
-  if (edge >= 0) held[edge] = x[edge];
+  int end[kEnds];  // elements of the row's ends, or -1
+  if (kEnds == 2) {
+    end[0] = lane < span.head ? lane : -1;
+    end[kEnds - 1] = lane < span.tail ? V - span.tail + lane : -1;
+  } else {
+    end[0] = lane < span.head ? lane : lane - span.head < span.tail ? V - span.tail + lane - span.head : -1;
+  }
+#pragma unroll
+  for (int e = 0; e < kEnds; ++e)
+    if (end[e] >= 0) held[end[e]] = x[end[e]];
   int at[S];
   float lnq[S], q[S], z[S], mass[S];
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    const int j = s * 32 + lane;
+    const int j = s * L + lane;
     at[s] = -1;
     lnq[s] = neg_inf();
     if (j < K) {
@@ -182,34 +184,36 @@ __global__ void __launch_bounds__(kThreads, E <= 16 && S == 1 ? 4 : 3) distill_s
       if (at[s] >= 0) lnq[s] = t;
     }
   }
-  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
+  const float inv_t = a.inv_t, c = a.c;
   RowStats st;
   st.shift = 0.0f;
   if (!a.tail) {
     float m = lnq[0], sum = 0.0f;
 #pragma unroll
     for (int s = 1; s < S; ++s) m = max_nan(m, lnq[s]);
-    m = warp_max(m);
-    if (m != neg_inf()) {
+    m = warp_max<L>(m);
+    const float from = m == neg_inf() ? 0.0f : m;
 #pragma unroll
-      for (int s = 0; s < S; ++s) sum += expf(lnq[s] - m);
-      st.shift = m + logf(warp_sum(sum));
-    }
+    for (int s = 0; s < S; ++s) sum += expf(lnq[s] - from);
+    sum = warp_sum<L>(sum);
+    if (m != neg_inf()) st.shift = m + logf(sum);
   }
   st.total = 0.0f;
-  bool bad = false;
+  float bad = 0.0f;
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     lnq[s] -= st.shift;
     q[s] = expf(lnq[s]);
     st.total += q[s];
-    bad |= at[s] == V;
-    if (at[s] == V) at[s] = -1;  // no token to find
+    if (at[s] == V) {  // no token to find
+      bad = quiet_nan();
+      at[s] = -1;
+    }
     mass[s] = at[s] >= 0 ? q[s] : -1.0f;
   }
-  st.total = warp_sum(st.total);
+  st.total = warp_sum<L>(st.total);
   st.r = a.tail ? max_nan(0.0f, 1.0f - st.total) : 0.0f;
-  if (__any_sync(0xffffffffu, bad)) st.total = quiet_nan();
+  st.total += warp_sum<L>(bad);
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncwarp();
 #pragma unroll
@@ -217,36 +221,41 @@ __global__ void __launch_bounds__(kThreads, E <= 16 && S == 1 ? 4 : 3) distill_s
   __syncwarp();
 #pragma unroll
   for (int s = 0; s < S; ++s)
-    if (at[s] >= 0) put_slot(held, at[s], s * 32 + lane);
+    if (at[s] >= 0) put_slot(held, at[s], s * L + lane);
   __syncwarp();
   bool other = false;
 #pragma unroll
-  for (int s = 0; s < S; ++s) other |= at[s] >= 0 && get_slot(held, at[s]) != s * 32 + lane;
-  st.repeated = __any_sync(0xffffffffu, other) ? 1.0f : 0.0f;  // and all have read
+  for (int s = 0; s < S; ++s) other |= at[s] >= 0 && get_slot(held, at[s]) != s * L + lane;
+  const unsigned others = __ballot_sync(0xffffffffu, other);  // and all have read
+  const unsigned mine = (L == 32 ? 0xffffffffu : (1u << L) - 1) << (threadIdx.x & 31) / L * L;
+  st.repeated = others & mine ? 1.0f : 0.0f;
 #pragma unroll
   for (int s = 0; s < S; ++s)
     if (at[s] >= 0) logit_put(held, at[s], neg_inf());
   __syncwarp();
-  if (st.repeated != 0.0f) {  // masses to the first slot of each token
+  if (others != 0) {  // in a row of the warp: masses to the first slot of each token
+    float sums[S];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      float sum = 0.0f;
+      sums[s] = 0.0f;
       bool first = at[s] >= 0;
 #pragma unroll
       for (int t = 0; t < S; ++t)
-        for (int k = 0; k < 32; ++k) {
-          const int other_at = __shfl_sync(0xffffffffu, at[t], k);
-          const float other_q = __shfl_sync(0xffffffffu, q[t], k);
+#pragma unroll 1
+        for (int k = 0; k < L; ++k) {
+          const int other_at = __shfl_sync(0xffffffffu, at[t], k, L);
+          const float other_q = __shfl_sync(0xffffffffu, q[t], k, L);
           if (other_at != at[s]) continue;
-          sum += other_q;
-          if (t * 32 + k < s * 32 + lane) first = false;
+          sums[s] += other_q;
+          if (t * L + k < s * L + lane) first = false;
         }
-      mass[s] = first ? sum : -1.0f;
+      if (!first) sums[s] = -1.0f;
     }
+#pragma unroll
+    for (int s = 0; s < S; ++s) mass[s] = sums[s];
   }
+  float zs[S];
   int distinct = 0;
-  float zs[S < 2 ? 2 : S];
-  if (S < 2) zs[1] = neg_inf();
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     const bool own = !(mass[s] < 0.0f);
@@ -254,56 +263,65 @@ __global__ void __launch_bounds__(kThreads, E <= 16 && S == 1 ? 4 : 3) distill_s
     distinct += own ? 1 : 0;
   }
   if (K >= V && a.tail) {  // where every token is listed there is no other class
-    if (__reduce_add_sync(0xffffffffu, distinct) >= V) st.r = 0.0f;
+    if (warp_sum<L>(static_cast<float>(distinct)) >= static_cast<float>(V)) st.r = 0.0f;
   }
 
-  float xs[E];
+  float xs[kN];
 #pragma unroll
   for (int u = 0; u < kVecs; ++u) {
-    const int v = u * 32 + lane;
+    const int v = u * L + lane;
     float part[kV];
     unpack(v < span.vecs ? hvec[v] : void_vec<T>(), part);
 #pragma unroll
     for (int e = 0; e < kV; ++e) xs[u * kV + e] = part[e];
   }
-  const float edge_x = edge >= 0 ? logit_at<T>(held, edge) : neg_inf();
-  const SoftState rest = soft_of_warp<false>(xs, edge_x, c);
-  const SoftState all = soft_merge(rest, soft_of_warp<false>(zs, neg_inf(), c), c);
+#pragma unroll
+  for (int e = 0; e < kEnds; ++e) xs[E + e] = end[e] >= 0 ? logit_at<T>(held, end[e]) : neg_inf();
+  SoftState rest = soft_of_lanes<false, L>(xs, c), top = soft_of_lanes<false, L>(zs, c);
+  const SoftState all = soft_merge(rest, top, c);
   st.m = all.m;
   st.ln_s = all.m == neg_inf() ? neg_inf() : logf(all.s);
   st.rest_m = rest.m;
   st.ln_rest = rest.m == neg_inf() ? neg_inf() : logf(rest.s);
-  const float loss = warp_loss(st, inv_t, [&](auto f) {
+  const float loss = row_loss<L>(st, inv_t, [&](auto f) {
 #pragma unroll
     for (int s = 0; s < S; ++s) f(lnq[s], q[s], z[s]);
   });
-  if (lane == 0) {
-    a.loss[row] = w * loss;
-    if (a.stats != nullptr) *reinterpret_cast<RowStats*>(a.stats + kStats * row) = st;
+  const bool counts = w != 0.0f;  // a row of weight 0: zeros, whatever it holds
+  if (lane == 0 && live) {
+    a.loss[row] = counts ? w * loss : 0.0f;
+    if (a.stats != nullptr)
+      *reinterpret_cast<RowStats*>(a.stats + kStats * static_cast<int64_t>(row)) = st;
   }
-  if (d == nullptr) return;
+  if (a.dlogits == nullptr) return;
 
+  T* d = static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1];
   const RowGradient g = row_gradient(st, a.tail, inv_t, w);
+  const bool zero = g.none || !counts;
   const RowMap f = g.unlisted(c);
-  if (edge >= 0) logit_put(d, edge, g.none ? 0.0f : f.plain(edge_x));
   T* out = d + span.head;
   const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+  if (live) {
 #pragma unroll
-  for (int u = 0; u < kVecs; ++u) {
-    const int v = u * 32 + lane;
-    if (v >= span.vecs) continue;
-    float ds[kV];
+    for (int e = 0; e < kEnds; ++e)
+      if (end[e] >= 0) logit_put(d, end[e], zero ? 0.0f : f.plain(xs[E + e]));
 #pragma unroll
-    for (int e = 0; e < kV; ++e) ds[e] = g.none ? 0.0f : f.plain(xs[u * kV + e]);
-    if (aligned) {
-      store_vec(out + v * kV, ds);
-    } else {
+    for (int u = 0; u < kVecs; ++u) {
+      const int v = u * L + lane;
+      if (v >= span.vecs) continue;
+      float ds[kV];
 #pragma unroll
-      for (int e = 0; e < kV; ++e) logit_put(out, v * kV + e, ds[e]);
+      for (int e = 0; e < kV; ++e) ds[e] = zero ? 0.0f : f.plain(xs[u * kV + e]);
+      if (aligned) {
+        store_vec(out + v * kV, ds);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) logit_put(out, v * kV + e, ds[e]);
+      }
     }
   }
-  if (g.none) return;
   __syncwarp();
+  if (!live || zero) return;
 #pragma unroll
   for (int s = 0; s < S; ++s)
     if (!(mass[s] < 0.0f)) logit_put(d, at[s], g.listed(z[s], mass[s], c));
@@ -385,7 +403,7 @@ __device__ __forceinline__ void list_state(RowShared& sh, const List& l, int K, 
     }
     if (first) zs[s] = l.z[j];
   }
-  const SoftState top = soft_of_warp<false>(zs, neg_inf(), c);
+  const SoftState top = soft_of_lanes<false, 32>(zs, c);
   if (lane == 0) sh.top = top;
 }
 // The row's statistics from the unlisted tokens' state.
@@ -406,7 +424,7 @@ __device__ __forceinline__ RowStats row_stats(const RowShared& sh, const SoftSta
 __device__ __forceinline__ void write_loss(const DistillTopkArgs& a, const RowStats& st, const List& l,
                                            int64_t row, float w, float inv_t, int lane) {
   const int K = static_cast<int>(a.K);
-  const float loss = warp_loss(st, inv_t, [&](auto f) {
+  const float loss = row_loss<32>(st, inv_t, [&](auto f) {
     for (int j = lane; j < K; j += 32) f(l.lnq[j], l.q[j], l.z[j]);
   });
   if (lane == 0) {
@@ -426,15 +444,16 @@ __host__ __device__ constexpr size_t held_at(int K) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 5) distill_warp_kernel(DistillTopkArgs a) {
+__global__ void __launch_bounds__(32 * kWarpsHeld, 10) distill_warp_kernel(DistillTopkArgs a, FastDiv inner) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int kV = kVec<T>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int V = static_cast<int>(a.V), K = static_cast<int>(a.K);
-  const uint32_t row32 = blockIdx.x * kWarps + warp;
+  const uint32_t row32 = blockIdx.x * kWarpsHeld + warp;
   const int64_t row = row32;
   if (row >= a.outer * a.inner) return;
-  const int64_t o = row32 / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
+  int o, i;
+  inner.divmod(static_cast<int>(row32), o, i);
   const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
   T* d = a.dlogits != nullptr
              ? static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1]
@@ -460,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 5) distill_warp_kernel(DistillTopkAr
     l.index[j] = at;
     l.lnq[j] = at >= 0 ? t : neg_inf();
   }
-  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
+  const float inv_t = a.inv_t, c = a.c;
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (w == 0.0f) {  // (the row was on its way before its weight was there)
     if (d != nullptr) map_row<T, 32>(x, d, V, lane, true, Nothing());
@@ -484,6 +503,12 @@ __global__ void __launch_bounds__(kThreads, 5) distill_warp_kernel(DistillTopkAr
   __syncwarp();
   list_state(sh, l, K, V, lane, c, repeated);
   __syncwarp();
+  if (a.tail && K >= V) {  // where every token is listed there is no other class
+    int distinct = 0;
+    for (int j = lane; j < K; j += 32) distinct += l.mass[j] < 0.0f ? 0 : 1;
+    if (__reduce_add_sync(0xffffffffu, distinct) >= V) sh.r = 0.0f;
+    __syncwarp();
+  }
 
   SoftSums<false> sums;
   const float slack = kBaseSlack / c;
@@ -494,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 5) distill_warp_kernel(DistillTopkAr
       const int v = b + u * 32 + lane;
       wv[u] = v < span.vecs ? hvec[v] : void_vec<T>();
     }
-    sums.add<T>(wv, max_of(wv, T()), c, slack);
+    sums.add<T>(wv, max_of(wv, T()), c, slack, batch_fill<32>(b, span.vecs, lane));
   }
   SoftState rest = sums.wide ? soft_slowly<T, 32>(hvec, 0, span.vecs, lane, c) : sums.state(c);
   if (edge >= 0) soft_add(rest, logit_at<T>(held, edge), c);
@@ -563,9 +588,49 @@ __device__ __forceinline__ void strike(uint4& w, uint32_t bits, uint16_t) {
   w.w = strike_pair(w.w, bits >> 6);
 }
 
+// soft_slowly with the bits' elements left out.
+template <typename T, int G>
+__device__ __forceinline__ SoftState soft_slowly_struck(const uint4* vec, int v0, int v1, int tid, float c,
+                                                        const uint32_t* bits) {
+  SoftState st = soft_empty();
+  const T* x = reinterpret_cast<const T*>(vec);
+#pragma unroll 1
+  for (int v = v0 + tid, at = 0; v < v1; v += G, ++at)
+#pragma unroll 1
+    for (int e = 0; e < kVec<T>; ++e)
+      if ((bits[at / kUnroll * G + tid] >> (at % kUnroll * 8 + e) & 1) == 0)
+        soft_add(st, logit_at<T>(x, static_cast<int64_t>(v) * kVec<T> + e), c);
+  return st;
+}
+// The unlisted tokens' gradients for the vectors [v0, v1), whose first batch is in `next` (not for a
+// wide row).
+template <typename T, int G>
+__device__ __forceinline__ void write_slice(uint4 (&next)[kUnroll], const uint4* vec, T* out, int v0, int v1,
+                                            int tid, const RowMap& f) {
+  constexpr int kV = kVec<T>;
+  const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+  stream<T, G>(next, vec, v0, v1, tid, [&](const uint4 (&wv)[kUnroll], int b) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int v = b + u * G + tid;
+      if (v >= v1) break;
+      float xs[kV], ds[kV];
+      unpack(wv[u], xs);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) ds[e] = ex2(fmaf(xs[e], f.c, -f.b)) * f.k0;
+      if (aligned) {
+        store_vec(out + static_cast<int64_t>(v) * kV, ds);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) logit_put(out, static_cast<int64_t>(v) * kV + e, ds[e]);
+      }
+    }
+  });
+}
+
 // kThreads threads stream; one warp more has the list.
 template <typename T>
-__global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTopkArgs a, int C) {
+__global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTopkArgs a, int C, FastDiv inner) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int kV = kVec<T>, kStep = kThreads * kUnroll;
   CtaShared& sh = *reinterpret_cast<CtaShared*>(smem);
@@ -577,7 +642,8 @@ __global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTo
   const uint32_t rank = C > 1 ? cta_rank() : 0;
   const uint32_t row32 = blockIdx.x / static_cast<uint32_t>(C);
   const int64_t row = row32;
-  const int64_t o = row32 / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
+  int o, i;
+  inner.divmod(static_cast<int>(row32), o, i);
   const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
   T* d = a.dlogits != nullptr
              ? static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1]
@@ -592,7 +658,7 @@ __global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTo
   const int v0 = min(static_cast<int>(rank) * per, span.vecs), v1 = min(v0 + per, span.vecs);
   const int head = rank == 0 ? span.head : 0, tail = rank == C - 1 ? span.tail : 0;
   const int from = span.head + v0 * kV - head, n = head + (v1 - v0) * kV + tail;
-  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
+  const float inv_t = a.inv_t, c = a.c;
 
   uint4 next[kUnroll];
   int edge = -1;
@@ -689,27 +755,19 @@ __global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTo
   SoftSums<false> sums;
   const float slack = kBaseSlack / c;
   const uint32_t* my_bits = bits + tid;
-  stream<T, kThreads>(next, vec, v0, v1, tid, [&](uint4 (&wv)[kUnroll], int) {
+  stream<T, kThreads>(next, vec, v0, v1, tid, [&](uint4 (&wv)[kUnroll], int b) {
     const uint32_t struck = *my_bits;
     my_bits += kThreads;
     if (struck != 0) {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) strike(wv[u], struck >> 8 * u, T());
     }
-    sums.add<T>(wv, max_of(wv, T()), c, slack);
+    sums.add<T>(wv, max_of(wv, T()), c, slack, batch_fill<kThreads>(b, v1, tid));
   });
   if (d != nullptr) load_batch<T, kThreads>(next, vec, v0, v1, tid);  // again, for the gradient
   SoftState rest = soft_empty();
-  if (!sums.wide) {
-    rest = sums.state(c);
-  } else {
-#pragma unroll 1
-    for (int v = v0 + tid, at = 0; v < v1; v += kThreads, ++at)
-#pragma unroll 1
-      for (int e = 0; e < kV; ++e)
-        if ((bits[at / kUnroll * kThreads + tid] >> (at % kUnroll * 8 + e) & 1) == 0)
-          soft_add(rest, logit_at<T>(reinterpret_cast<const T*>(vec), static_cast<int64_t>(v) * kV + e), c);
-  }
+  if (!sums.wide) rest = sums.state(c);
+  else rest = soft_slowly_struck<T, kThreads>(vec, v0, v1, tid, c, bits);
   if (edge >= 0 && (sh.edge_bits >> tid & 1) == 0) soft_add(rest, edge_x, c);
   {
     const float m = warp_max(rest.m);
@@ -738,40 +796,23 @@ __global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTo
   if (f.wide || none) {
     map_row<T, kThreads>(x + from + head, d + from + head, n - head - tail, tid, none, f);
   } else {
-    T* out = d + span.head;
-    const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
-    stream<T, kThreads>(next, vec, v0, v1, tid, [&](const uint4 (&wv)[kUnroll], int b) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int v = b + u * kThreads + tid;
-        if (v >= v1) break;
-        float xs[kV], ds[kV];
-        unpack(wv[u], xs);
-#pragma unroll
-        for (int e = 0; e < kV; ++e) ds[e] = ex2(fmaf(xs[e], f.c, -f.b)) * f.k0;
-        if (aligned) {
-          store_vec(out + static_cast<int64_t>(v) * kV, ds);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kV; ++e) logit_put(out, static_cast<int64_t>(v) * kV + e, ds[e]);
-        }
-      }
-    });
+    write_slice<T, kThreads>(next, vec, d + span.head, v0, v1, tid, f);
   }
   if (!none) __syncthreads();
 }
 
 // --------------------------------------------------- the gradient from the forward's statistics
 template <typename T, int G>
-__global__ void __launch_bounds__(kThreads) distill_topk_bwd_kernel(DistillTopkArgs a, int pieces,
-                                                                    int piece) {
+__global__ void __launch_bounds__(kThreads) distill_topk_bwd_kernel(DistillTopkArgs a, FastDiv pieces,
+                                                                    int piece, FastDiv inner) {
   const int tid = threadIdx.x % G, group = threadIdx.x / G;
   const int V = static_cast<int>(a.V), K = static_cast<int>(a.K);
-  const uint32_t unit = blockIdx.x * (kThreads / G) + group;
-  const int64_t row = unit / static_cast<uint32_t>(pieces);
+  int row32, nth, o, i;
+  pieces.divmod(static_cast<int>(blockIdx.x * (kThreads / G) + group), row32, nth);
+  const int64_t row = row32;
   if (row >= a.outer * a.inner) return;  // whole warps of the warp form
-  const int64_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
-  const int from = static_cast<int>(unit - static_cast<uint32_t>(row) * pieces) * piece;
+  inner.divmod(row32, o, i);
+  const int from = nth * piece;
   const int n = min(piece, V - from);
   const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
   T* d = static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1];
@@ -780,7 +821,7 @@ __global__ void __launch_bounds__(kThreads) distill_topk_bwd_kernel(DistillTopkA
     map_row<T, G>(x + from, d + from, n, tid, true, Nothing());
     return;
   }
-  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
+  const float inv_t = a.inv_t, c = a.c;
   const RowStats st = *reinterpret_cast<const RowStats*>(a.stats + kStats * row);
   const float up = a.g_loss.p[o * a.g_loss.strides[0] + i * a.g_loss.strides[1]];
   const RowGradient g = row_gradient(st, a.tail, inv_t, w * up);
@@ -818,11 +859,11 @@ int launch_check(const char* what, cudaError_t e) {
   return BDH_OK;
 }
 
-template <typename T, int E>
-int launch_short(const DistillTopkArgs& a, cudaStream_t stream) {
-  const unsigned grid = static_cast<unsigned>((a.outer * a.inner + kWarps - 1) / kWarps);
-  if (a.K <= 32) distill_short_kernel<T, E, 1><<<grid, kThreads, 0, stream>>>(a);
-  else distill_short_kernel<T, E, kTopMax / 32><<<grid, kThreads, 0, stream>>>(a);
+template <typename T, int L, int E, int S>
+int launch_short(const DistillTopkArgs& a, const FastDiv& inner, cudaStream_t stream) {
+  constexpr int kRows = kThreads / L;
+  const unsigned grid = static_cast<unsigned>((a.outer * a.inner + kRows - 1) / kRows);
+  distill_short_kernel<T, L, E, S><<<grid, kThreads, 0, stream>>>(a, inner);
   return launch_check("distill_topk launch", cudaSuccess);
 }
 
@@ -835,22 +876,24 @@ int allow_smem(const void* kern, size_t smem) {
 
 template <typename T>
 int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
-  if (a.V <= 256) return launch_short<T, 8>(a, stream);
-  if (a.V <= 512) return launch_short<T, 16>(a, stream);
-  if (a.V <= kShort) return launch_short<T, 32>(a, stream);
+  const FastDiv inner(static_cast<uint32_t>(a.inner));
+  if (a.V <= 256 && a.K <= 16) return launch_short<T, 8, 32, 2>(a, inner, stream);
+  if (a.V <= 512 && a.K <= 32) return launch_short<T, 16, 32, 2>(a, inner, stream);
+  if (a.V <= kShort && a.K <= 32) return launch_short<T, 32, 32, 1>(a, inner, stream);
   int dev = 0;
   cudaGetDevice(&dev);
   const int K = static_cast<int>(a.K);
   const int64_t rows = a.outer * a.inner, bytes = a.V * static_cast<int64_t>(sizeof(T));
-  if (bytes <= kWarpRowBytes && rows >= kWarpRows * sm_count(dev)) {
-    const size_t smem = kWarps * (held_at(K) + held_bytes<T>(a.V));
+  if (a.V <= kShort || (bytes <= kWarpRowBytes && rows >= kWarpRows * sm_count(dev))) {
+    const size_t smem = kWarpsHeld * (held_at(K) + held_bytes<T>(a.V));
     if (int rc = allow_smem(reinterpret_cast<const void*>(distill_warp_kernel<T>), smem)) return rc;
-    distill_warp_kernel<T><<<static_cast<unsigned>((rows + kWarps - 1) / kWarps), kThreads, smem, stream>>>(a);
+    distill_warp_kernel<T><<<static_cast<unsigned>((rows + kWarpsHeld - 1) / kWarpsHeld), 32 * kWarpsHeld, smem,
+                             stream>>>(a, inner);
     return launch_check("distill_topk launch", cudaSuccess);
   }
   int cluster = 1;
   while (cluster < kMaxCluster &&
-         (bytes > static_cast<int64_t>(cluster) * (getenv("SLICE") ? atoi(getenv("SLICE")) : kSliceBytes) ||
+         ((a.dlogits != nullptr && bytes > static_cast<int64_t>(cluster) * kSliceBytes) ||
           (rows * cluster < 4 * sm_count(dev) && bytes >= cluster * int64_t(32768))))
     cluster *= 2;
   if (rows * cluster >= int64_t(1) << 31) {
@@ -871,15 +914,16 @@ int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return launch_check("distill_topk launch", cudaLaunchKernelEx(&cfg, kern, a, cluster));
+  return launch_check("distill_topk launch", cudaLaunchKernelEx(&cfg, kern, a, cluster, inner));
 }
 
 template <typename T>
 int backward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
+  const FastDiv inner(static_cast<uint32_t>(a.inner));
   if (a.V <= kShort) {
     const unsigned grid = static_cast<unsigned>((rows + kWarps - 1) / kWarps);
-    distill_topk_bwd_kernel<T, 32><<<grid, kThreads, 0, stream>>>(a, 1, static_cast<int>(a.V));
+    distill_topk_bwd_kernel<T, 32><<<grid, kThreads, 0, stream>>>(a, FastDiv(1), static_cast<int>(a.V), inner);
   } else {
     const int64_t pieces = (a.V + kPiece - 1) / kPiece;
     if (rows * pieces >= int64_t(1) << 31) {
@@ -887,7 +931,7 @@ int backward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
       return BDH_ERR_INVALID;
     }
     distill_topk_bwd_kernel<T, kThreads><<<static_cast<unsigned>(rows * pieces), kThreads, 0, stream>>>(
-        a, static_cast<int>(pieces), kPiece);
+        a, FastDiv(static_cast<uint32_t>(pieces)), kPiece, inner);
   }
   return launch_check("distill_topk_bwd launch", cudaSuccess);
 }

@@ -317,7 +317,7 @@ struct TokenLogprobsArgs {
   int64_t t_strides[2] = {0, 0};
   int64_t ignore_index = -100;
   int64_t outer = 0, inner = 0, V = 0, K = 0;
-  float temperature = 1.0f;
+  float inv_t = 1.0f, c = 1.0f;  // 1 / temperature, and times log2(e)
   // forward outputs, one per row in row order; top_* K per row; any but stats may be null
   float* logprob = nullptr;
   float* lse = nullptr;
@@ -352,7 +352,7 @@ struct DistillTopkArgs {
   int64_t t_strides[3] = {0, 0, 0};
   RowGrad weight;  // null: 1
   int64_t outer = 0, inner = 0, V = 0, K = 0;
-  float temperature = 1.0f;
+  float inv_t = 1.0f, c = 1.0f;  // 1 / temperature, and times log2(e)
   int tail = 0;
   float* loss = nullptr;   // one per row; null in the backward form
   float* stats = nullptr;  // 8 per row (written by the forward when not null, read by the backward)

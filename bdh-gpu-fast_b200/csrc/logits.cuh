@@ -146,6 +146,11 @@ __device__ __forceinline__ uint4 void_vec<uint16_t>() {
 
 constexpr int kUnroll = 4;  // vectors that a thread has in flight (a batch)
 
+// How many of a batch's vectors b + u G + tid this warp has any of.
+template <int G>
+__device__ __forceinline__ int batch_fill(int b, int v1, int tid) {
+  return (v1 - b - (tid & ~31) + G - 1) / G;  // may be more than there are
+}
 // A group of G threads over the vectors [v0, v1): f(w, b) for every batch w of its kUnroll vectors
 // b + u G + tid (-inf past the end), with the next batch's loads under way meanwhile. `next` is the
 // batch at v0, asked for by the caller (load_batch) as early as it can.
@@ -287,14 +292,15 @@ struct SoftSums {
     m = largest;
     limit = largest + slack;
   }
-  // N vectors whose largest element is `largest`.
+  // N vectors whose largest element is `largest`; of a row's last ones, `fill` of them.
   template <typename T, int N>
-  __device__ __forceinline__ void add(const uint4 (&w)[N], float largest, float c, float slack) {
+  __device__ __forceinline__ void add(const uint4 (&w)[N], float largest, float c, float slack, int fill) {
     if (!(largest <= limit)) raise(largest, c, slack);  // a NaN too
     if (wide || m == neg_inf()) return;
     float ps[2] = {0.0f, 0.0f}, pa[2] = {0.0f, 0.0f};  // (a batch's own sums: fewer terms in a row)
 #pragma unroll
     for (int u = 0; u < N; ++u) {
+      if (u > 0 && u >= fill) break;
       float x[kVec<T>];
       unpack(w[u], x);
 #pragma unroll
@@ -372,14 +378,17 @@ __device__ __forceinline__ void map_row(const T* x, T* d, int n, int tid, bool z
   }
 }
 
+// Over the warp, or over each L neighbouring lanes of it (all lanes take part).
+template <int L = 32>
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, d));
+  for (int d = L / 2; d > 0; d >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, d));
   return v;
 }
+template <int L = 32>
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  for (int d = L / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
 }
 // The lanes' states as one.
@@ -391,24 +400,23 @@ __device__ __forceinline__ SoftState soft_join(SoftState st, float c) {
   st.a = warp_sum(st.a);
   return st;
 }
-// Softmax state of a row that a warp holds N elements a lane of: the maximum first, then the sums.
-template <bool ENTROPY, int N>
-__device__ __forceinline__ SoftState soft_of_warp(const float (&x)[N], float edge, float c) {
-  float m = edge;
+// Softmax state of a row that L lanes hold N elements each of: the maximum first, then the sums.
+template <bool ENTROPY, int L, int N>
+__device__ __forceinline__ SoftState soft_of_lanes(const float (&x)[N], float c) {
+  float m = x[0];
 #pragma unroll
-  for (int i = 0; i < N; ++i) m = max_nan(m, x[i]);
-  m = warp_max(m);
-  if (m == neg_inf()) return soft_empty();
-  float t = max_nan((edge - m) * c, kExpFloor), e = ex2(t);
-  float s = e, a = e * t;
+  for (int i = 1; i + 1 < N; i += 2) m = max_nan(m, x[i], x[i + 1]);
+  if (N % 2 == 0) m = max_nan(m, x[N - 1]);
+  m = warp_max<L>(m);
+  const float from = m == neg_inf() ? 0.0f : m;  // (all lanes go on: other lanes' rows may have more)
+  float s = 0.0f, a = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    t = max_nan((x[i] - m) * c, kExpFloor);
-    e = ex2(t);
+    const float t = max_nan((x[i] - from) * c, kExpFloor), e = ex2(t);
     s += e;
     if (ENTROPY) a = fmaf(e, t, a);
   }
-  return {m, warp_sum(s), ENTROPY ? warp_sum(a) : 0.0f};
+  return {m, warp_sum<L>(s), ENTROPY ? warp_sum<L>(a) : 0.0f};
 }
 
 // Order of a row's top list: larger values first, an equal value's lower index first; -0 equals

@@ -12,6 +12,8 @@ namespace bdh {
 
 namespace {
 
+constexpr float kLog2eHost = 1.4426950408889634f;
+
 int refuse(const char* what, const char* why) {
   set_error(std::string(what) + ": " + why);
   return BDH_ERR_INVALID;
@@ -67,7 +69,8 @@ int bdh_token_logprobs(const void* logits, int dtype, const int64_t l_strides[2]
   a.tokens = tokens;
   if (tokens != nullptr) std::memcpy(a.t_strides, t_strides, sizeof(a.t_strides));
   a.ignore_index = ignore_index;
-  a.outer = outer; a.inner = inner; a.V = V; a.K = K; a.temperature = temperature;
+  a.outer = outer; a.inner = inner; a.V = V; a.K = K;
+  a.inv_t = 1.0f / temperature; a.c = kLog2eHost * a.inv_t;
   a.logprob = logprob; a.lse = lse; a.entropy = entropy; a.stats = stats;
   a.top_logprob = top_logprob; a.top_index = top_index;
   return launch_token_logprobs(a, static_cast<cudaStream_t>(stream));
@@ -99,7 +102,8 @@ int bdh_token_logprobs_bwd(const void* logits, int dtype, const int64_t l_stride
   a.f.tokens = tokens;
   if (tokens != nullptr) std::memcpy(a.f.t_strides, t_strides, sizeof(a.f.t_strides));
   a.f.ignore_index = ignore_index;
-  a.f.outer = outer; a.f.inner = inner; a.f.V = V; a.f.K = K; a.f.temperature = temperature;
+  a.f.outer = outer; a.f.inner = inner; a.f.V = V; a.f.K = K;
+  a.f.inv_t = 1.0f / temperature; a.f.c = kLog2eHost * a.f.inv_t;
   a.f.stats = const_cast<float*>(stats);
   a.f.entropy = const_cast<float*>(entropy);
   a.f.top_index = const_cast<int64_t*>(top_index);
@@ -133,7 +137,8 @@ int bdh_distill_topk(const void* logits, int dtype, const int64_t l_strides[2],
   a.teacher = teacher;
   std::memcpy(a.t_strides, t_strides, sizeof(a.t_strides));
   a.weight = row_grad(weight, w_strides);
-  a.outer = outer; a.inner = inner; a.V = V; a.K = K; a.temperature = temperature;
+  a.outer = outer; a.inner = inner; a.V = V; a.K = K;
+  a.inv_t = 1.0f / temperature; a.c = kLog2eHost * a.inv_t;
   a.tail = tail ? 1 : 0;
   a.loss = loss; a.stats = stats;
   a.dlogits = dlogits;
@@ -164,7 +169,8 @@ int bdh_distill_topk_bwd(const void* logits, int dtype, const int64_t l_strides[
   a.teacher = teacher;
   std::memcpy(a.t_strides, t_strides, sizeof(a.t_strides));
   a.weight = row_grad(weight, w_strides);
-  a.outer = outer; a.inner = inner; a.V = V; a.K = K; a.temperature = temperature;
+  a.outer = outer; a.inner = inner; a.V = V; a.K = K;
+  a.inv_t = 1.0f / temperature; a.c = kLog2eHost * a.inv_t;
   a.tail = tail ? 1 : 0;
   a.stats = const_cast<float*>(stats);
   a.g_loss = row_grad(g_loss, g_strides);

@@ -129,63 +129,105 @@ __device__ __forceinline__ void write_figures(const TokenLogprobsArgs& a, int64_
     a.logprob[row] = t.left_out ? 0.0f : t.given ? logprob_of(t.z, st, ln_s, inv_t) : quiet_nan();
 }
 
-// ------------------------------------------------------------------ a warp for a short row
-// Rows of at most kShort elements stay in registers (E elements a lane and one of the row's
-// unaligned ends): the maximum first, then the sums; for the list, the elements' keys. Lists up to
-// kWarpTop are bounded by the lanes' largest keys, where that leaves no more candidates than there is
-// room for; longer ones by the elements' own.
+// ------------------------------------------------------------------ lanes for a short row
+// Rows of at most kShort elements stay in registers: L lanes hold E elements each of a row, and one or
+// two of its unaligned ends; the maximum first, then the sums. With few lanes a row the shuffles and
+// the row's own figures serve several rows at once (a byte model's 256: 4 rows a warp).
 constexpr int kShort = 1024;
+
+template <typename T, int L, int E>
+struct ShortRow {
+  static constexpr int kV = kVec<T>, kVecs = E / kV, kEnds = L < 16 ? 2 : 1, kN = E + kEnds;
+  RowSpan span;
+  int end[kEnds];  // elements of the row's ends, or -1
+  float x[kN];     // the vectors', then the ends'; -inf where there is none
+  __device__ __forceinline__ int index(int u, int e, int lane) const { return span.head + (u * L + lane) * kV + e; }
+  __device__ __forceinline__ bool has(int u, int lane) const { return u * L + lane < span.vecs; }
+  __device__ __forceinline__ void place(const T* p, int V, int lane) {
+    span = row_span(p, V);
+    if (kEnds == 2) {
+      end[0] = lane < span.head ? lane : -1;
+      end[kEnds - 1] = lane < span.tail ? V - span.tail + lane : -1;
+    } else {
+      end[0] = lane < span.head ? lane : lane - span.head < span.tail ? V - span.tail + lane - span.head : -1;
+    }
+  }
+  __device__ __forceinline__ void load(const T* p, int lane) {
+    const uint4* vec = reinterpret_cast<const uint4*>(p + span.head);
+    uint4 w[kVecs];
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) w[u] = has(u, lane) ? __ldg(vec + u * L + lane) : void_vec<T>();
+#pragma unroll
+    for (int i = 0; i < kEnds; ++i) x[E + i] = end[i] >= 0 ? logit_at<T>(p, end[i]) : neg_inf();
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      float part[kV];
+      unpack(w[u], part);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) x[u * kV + e] = part[e];
+    }
+  }
+};
+
+template <typename T, int L, int E>
+__global__ void __launch_bounds__(kThreads) token_logprobs_short_kernel(TokenLogprobsArgs a, FastDiv inner) {
+  const int lane = threadIdx.x % L;
+  const int rows = static_cast<int>(a.outer * a.inner);
+  int row = static_cast<int>(blockIdx.x * (kThreads / L) + threadIdx.x / L);
+  const bool live = row < rows;
+  if (!__any_sync(0xffffffffu, live)) return;
+  if (!live) row = rows - 1;  // (the warp's other rows need these lanes)
+  int o, i;
+  inner.divmod(row, o, i);
+  const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
+  ShortRow<T, L, E> r;
+  r.place(x, static_cast<int>(a.V), lane);
+  Token tok = {false, true, 0.0f};
+  if (lane == 0 && a.tokens != nullptr) tok = load_token(a, x, o, i);
+  r.load(x, lane);
+  const SoftState st = soft_of_lanes<true, L>(r.x, a.c);
+  if (lane == 0 && live) write_figures(a, row, st, ln_sum(st), a.inv_t, tok);
+}
+
+// With a list, a warp for a row: the elements' keys. Lists up to kWarpTop are bounded by the lanes'
+// largest keys, where that leaves no more candidates than there is room for; longer ones by the
+// elements' own.
 constexpr int kShortRoom = kTopMax + top_slack(kTopMax) + 1;
 
-template <typename T, int E, bool TOP>
-__global__ void __launch_bounds__(kThreads) token_logprobs_short_kernel(TokenLogprobsArgs a) {
-  constexpr int kV = kVec<T>, kVecs = E / kV;
+template <typename T, int E>
+__global__ void __launch_bounds__(kThreads) token_list_short_kernel(TokenLogprobsArgs a, FastDiv inner) {
+  using Row = ShortRow<T, 32, E>;
+  constexpr int kV = Row::kV, kVecs = Row::kVecs;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
   if (row >= a.outer * a.inner) return;
-  const int64_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
+  int o, i;
+  inner.divmod(static_cast<int>(row), o, i);
   const int V = static_cast<int>(a.V);
   const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
-  const RowSpan span = row_span(x, V);
-  const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
-  uint4 w[kVecs];
-#pragma unroll
-  for (int u = 0; u < kVecs; ++u) {
-    const int v = u * 32 + lane;
-    w[u] = v < span.vecs ? __ldg(vec + v) : void_vec<T>();
-  }
-  int edge = -1;  // this lane's element of the row's ends
-  if (lane < span.head) edge = lane;
-  if (lane >= 8 && lane - 8 < span.tail) edge = V - span.tail + lane - 8;
-  const float edge_x = edge >= 0 ? logit_at<T>(x, edge) : neg_inf();
+  Row r;
+  r.place(x, V, lane);
   Token tok = {false, true, 0.0f};
   if (lane == 0 && a.tokens != nullptr) tok = load_token(a, x, o, i);
-  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t;
-  float xs[E];
-#pragma unroll
-  for (int u = 0; u < kVecs; ++u) {
-    float part[kV];
-    unpack(w[u], part);
-#pragma unroll
-    for (int e = 0; e < kV; ++e) xs[u * kV + e] = part[e];
-  }
-  const SoftState st = soft_of_warp<true>(xs, edge_x, c);
+  r.load(x, lane);
+  const float inv_t = a.inv_t;
+  const SoftState st = soft_of_lanes<true, 32>(r.x, a.c);
   const float ln_s = ln_sum(st);
   if (lane == 0) write_figures(a, row, st, ln_s, inv_t, tok);
-  if (!TOP) return;
 
   __shared__ uint64_t room[kWarps][kShortRoom];
   __shared__ int found[kWarps];
   uint64_t* cand = room[warp];
   const int K = static_cast<int>(a.K);
-  auto index_of = [&](int u, int e) { return span.head + (u * 32 + lane) * kV + e; };
+  auto index_of = [&](int u, int e) { return r.index(u, e, lane); };
+  const int edge = r.end[0];
   uint32_t keys[E], own = 0, own_at = 0xffffffffu;
-  const uint32_t edge_key = edge >= 0 ? value_key(edge_x) : 0u;
+  const uint32_t edge_key = edge >= 0 ? value_key(r.x[E]) : 0u;
 #pragma unroll
   for (int u = 0; u < kVecs; ++u)
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
-      const uint32_t k = u * 32 + lane < span.vecs ? value_key(xs[u * kV + e]) : 0u;
+      const uint32_t k = r.has(u, lane) ? value_key(r.x[u * kV + e]) : 0u;
       keys[u * kV + e] = k;
       if (k > own) {
         own = k;
@@ -290,7 +332,7 @@ __device__ __forceinline__ void group_sync() {
 
 template <typename T, int G, bool TOP>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsArgs a,
-                                                                  ForwardPlan plan) {
+                                                                  ForwardPlan plan, FastDiv inner) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int kV = kVec<T>, U = kUnroll;
   const int K = static_cast<int>(a.K), V = static_cast<int>(a.V);
@@ -301,9 +343,10 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
   const int64_t row = row32;
   if (row >= a.outer * a.inner) return;  // whole warps of the warp form
   if (C > 1) cluster_arrive();  // every CTA's shared memory may be written once all have started
-  const int64_t o = row32 / static_cast<uint32_t>(a.inner), i = row - o * a.inner;
+  int o, i;
+  inner.divmod(static_cast<int>(row32), o, i);
   const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
-  const float inv_t = 1.0f / a.temperature, c = kLog2e * inv_t, slack = kBaseSlack / c;
+  const float inv_t = a.inv_t, c = a.c, slack = kBaseSlack / c;
 
   uint8_t* base = smem + group * group_smem<T, G>(K, plan.cells, C);
   GroupShared& sh = *reinterpret_cast<GroupShared*>(base);
@@ -360,7 +403,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
         }
       }
     }
-    sums.add<T>(w, largest, c, slack);
+    sums.add<T>(w, largest, c, slack, batch_fill<G>(b, v1, tid));
   });
   SoftState st = sums.wide ? soft_slowly<T, G>(vec, v0, v1, tid, c) : sums.state(c);
   if (edge >= 0) soft_add(st, edge_x, c);
@@ -596,19 +639,21 @@ struct GradShared {
 
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(TokenLogprobsBwdArgs a,
-                                                                      int pieces, int piece) {
+                                                                      FastDiv pieces, int piece,
+                                                                      FastDiv inner) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x % G, group = threadIdx.x / G;
   GradShared& sh = *(reinterpret_cast<GradShared*>(smem) + group);  // with a list only
-  const uint32_t unit = blockIdx.x * (kThreads / G) + group;
-  const int64_t row = unit / static_cast<uint32_t>(pieces);
+  int row32, nth, o, i;
+  pieces.divmod(static_cast<int>(blockIdx.x * (kThreads / G) + group), row32, nth);
+  const int64_t row = row32;
   if (row >= a.f.outer * a.f.inner) return;  // whole warps of the warp form
-  const int64_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.f.inner), i = row - o * a.f.inner;
+  inner.divmod(row32, o, i);
   const int V = static_cast<int>(a.f.V), K = a.g_top != nullptr ? static_cast<int>(a.f.K) : 0;
-  const int from = static_cast<int>(unit - static_cast<uint32_t>(row) * pieces) * piece, n = min(piece, V - from);
+  const int from = nth * piece, n = min(piece, V - from);
   const T* x = static_cast<const T*>(a.f.logits) + o * a.f.l_strides[0] + i * a.f.l_strides[1];
   T* d = static_cast<T*>(a.dlogits) + o * a.d_strides[0] + i * a.d_strides[1];
-  const float inv_t = 1.0f / a.f.temperature, c = kLog2e * inv_t;
+  const float inv_t = a.f.inv_t, c = a.f.c;
   const float m = a.f.stats[2 * row], ln_s = a.f.stats[2 * row + 1];
   const bool none = m == neg_inf();
   auto up = [&](const RowGrad& g) {
@@ -711,24 +756,27 @@ int launch_forward(const TokenLogprobsArgs& a, int cluster, cudaStream_t stream)
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, kern, a, plan);
+  cudaLaunchKernelEx(&cfg, kern, a, plan, FastDiv(static_cast<uint32_t>(a.inner)));
   return launch_check("token_logprobs launch");
 }
 
-template <typename T, int E>
-int launch_short(const TokenLogprobsArgs& a, cudaStream_t stream) {
-  const unsigned grid = static_cast<unsigned>((a.outer * a.inner + kWarps - 1) / kWarps);
-  if (a.K > 0) token_logprobs_short_kernel<T, E, true><<<grid, kThreads, 0, stream>>>(a);
-  else token_logprobs_short_kernel<T, E, false><<<grid, kThreads, 0, stream>>>(a);
+template <typename T, int L, int E>
+int launch_short(const TokenLogprobsArgs& a, const FastDiv& inner, cudaStream_t stream) {
+  const int64_t rows = a.outer * a.inner;
+  const int per = a.K > 0 ? kWarps : kThreads / L;
+  const unsigned grid = static_cast<unsigned>((rows + per - 1) / per);
+  if (a.K > 0) token_list_short_kernel<T, L * E / 32><<<grid, kThreads, 0, stream>>>(a, inner);
+  else token_logprobs_short_kernel<T, L, E><<<grid, kThreads, 0, stream>>>(a, inner);
   return launch_check("token_logprobs launch");
 }
 
 template <typename T>
 int forward_by_size(const TokenLogprobsArgs& a, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner, vecs = a.V / kVec<T>;
-  if (a.V <= 256) return launch_short<T, 8>(a, stream);
-  if (a.V <= 512) return launch_short<T, 16>(a, stream);
-  if (a.V <= kShort) return launch_short<T, 32>(a, stream);
+  const FastDiv inner(static_cast<uint32_t>(a.inner));
+  if (a.V <= 256) return launch_short<T, 8, 32>(a, inner, stream);
+  if (a.V <= 512) return launch_short<T, 16, 32>(a, inner, stream);
+  if (a.V <= kShort) return launch_short<T, 32, 32>(a, inner, stream);
   // Many rows of a middling length: a warp each.
   if (a.V <= kWarpRow && a.K <= kWarpList && rows >= kWarpRows * sm_count_here())
     return launch_forward<T, 32>(a, 1, stream);
@@ -744,9 +792,11 @@ template <typename T>
 int backward_by_size(const TokenLogprobsBwdArgs& a, cudaStream_t stream) {
   const int64_t rows = a.f.outer * a.f.inner;
   const size_t lists = a.g_top != nullptr && a.f.K > 0 ? sizeof(GradShared) : 0;
+  const FastDiv inner(static_cast<uint32_t>(a.f.inner));
   if (a.f.V <= 1024) {
     const unsigned grid = static_cast<unsigned>((rows + kWarps - 1) / kWarps);
-    token_logprobs_bwd_kernel<T, 32><<<grid, kThreads, kWarps * lists, stream>>>(a, 1, static_cast<int>(a.f.V));
+    token_logprobs_bwd_kernel<T, 32><<<grid, kThreads, kWarps * lists, stream>>>(
+        a, FastDiv(1), static_cast<int>(a.f.V), inner);
   } else {
     const int64_t pieces = (a.f.V + kPiece - 1) / kPiece;
     if (rows * pieces >= int64_t(1) << 31) {
@@ -754,7 +804,7 @@ int backward_by_size(const TokenLogprobsBwdArgs& a, cudaStream_t stream) {
       return BDH_ERR_INVALID;
     }
     token_logprobs_bwd_kernel<T, kThreads><<<static_cast<unsigned>(rows * pieces), kThreads, lists, stream>>>(
-        a, static_cast<int>(pieces), kPiece);
+        a, FastDiv(static_cast<uint32_t>(pieces)), kPiece, inner);
   }
   return launch_check("token_logprobs_bwd launch");
 }
