@@ -894,7 +894,7 @@ int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
   int cluster = 1;
   while (cluster < kMaxCluster &&
          ((a.dlogits != nullptr && bytes > static_cast<int64_t>(cluster) * kSliceBytes) ||
-          (rows * cluster < 4 * sm_count(dev) && bytes >= cluster * int64_t(32768))))
+          (2 * rows * cluster <= 4 * sm_count(dev) && bytes >= cluster * int64_t(32768))))
     cluster *= 2;
   if (rows * cluster >= int64_t(1) << 31) {
     set_error("distill_topk: too many rows for this vocabulary");

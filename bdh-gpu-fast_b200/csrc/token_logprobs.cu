@@ -83,7 +83,7 @@ __device__ __forceinline__ uint64_t list_bound(int K, uint32_t lo, uint32_t hi, 
 }
 
 struct ForwardPlan {
-  int cells, cell_vecs;  // per thread, and vectors in a cell: one, or a number of batches
+  int cells, cell_shift;  // per thread, and log2 of the vectors in a cell: one, or some batches
   int cluster;
 };
 
@@ -296,11 +296,12 @@ __global__ void __launch_bounds__(kThreads) token_list_short_kernel(TokenLogprob
 // ------------------------------------------- a warp, a CTA or a cluster for longer rows
 // Shared memory of one group of G threads; with a list its cells, candidates, lists and queue follow.
 struct GroupShared {
-  SoftState part[kMaxCluster];
+  SoftState part[kMaxCluster];  // of the cluster's CTAs, in the first
   SoftState warp_part[kWarps];
   uint64_t best[kWarps];
   uint64_t bound;
-  int found, queued;
+  int found, queued, kept;
+  float m, ln_s;                // the row's
 };
 // The list's bound is searched among the cells themselves in a warp's row, and among the threads'
 // largest cells in a CTA's.
@@ -310,17 +311,20 @@ __host__ __device__ constexpr int bound_items(int cells) {
 }
 // Candidates and queue; the items' indices, which are needed before them, take their place.
 template <typename T, int G>
-__host__ __device__ constexpr size_t candidate_smem(int K, int cells) {
-  const size_t cand = static_cast<size_t>(candidate_room<T>(K)) * (sizeof(uint64_t) + sizeof(int));
+__host__ __device__ constexpr size_t candidate_smem(int K, int cells, int cluster) {
+  size_t n = static_cast<size_t>(candidate_room<T>(K)) * (sizeof(uint64_t) + sizeof(int));
   const size_t at = static_cast<size_t>(bound_items<G>(cells)) * sizeof(int);
-  return ((cand > at ? cand : at) + 7) & ~size_t(7);
+  const size_t all = static_cast<size_t>(cluster) * K * sizeof(uint64_t);  // what the slices' lists leave
+  if (n < at) n = at;
+  if (n < all) n = all;
+  return (n + 7) & ~size_t(7);
 }
 constexpr size_t kGroupShared = (sizeof(GroupShared) + 7) & ~size_t(7);
 template <typename T, int G>
 __host__ __device__ constexpr size_t group_smem(int K, int cells, int cluster) {
   size_t n = kGroupShared;
   if (K > 0)
-    n += candidate_smem<T, G>(K, cells) + static_cast<size_t>(cluster) * K * sizeof(uint64_t) +
+    n += candidate_smem<T, G>(K, cells, cluster) + static_cast<size_t>(cluster) * K * sizeof(uint64_t) +
          sizeof(int) * (static_cast<size_t>(cells + 1) * G + (G == 32 ? 0 : G));
   return (n + 15) & ~size_t(15);
 }
@@ -330,8 +334,11 @@ __device__ __forceinline__ void group_sync() {
   else __syncthreads();
 }
 
+template <int G>
+constexpr int cta_threads = G == 32 ? kThreads : G;  // groups of a warp share a CTA
+
 template <typename T, int G, bool TOP>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsArgs a,
+__global__ void __launch_bounds__(cta_threads<G>) token_logprobs_kernel(TokenLogprobsArgs a,
                                                                   ForwardPlan plan, FastDiv inner) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int kV = kVec<T>, U = kUnroll;
@@ -339,7 +346,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
   const int C = G == 32 ? 1 : plan.cluster;
   const uint32_t rank = C > 1 ? cta_rank() : 0;
   const int tid = threadIdx.x % G, group = threadIdx.x / G;
-  const uint32_t row32 = G == 32 ? blockIdx.x * (kThreads / G) + group : blockIdx.x / static_cast<uint32_t>(C);
+  const uint32_t row32 = G == 32 ? blockIdx.x * (cta_threads<G> / G) + group : blockIdx.x / static_cast<uint32_t>(C);
   const int64_t row = row32;
   if (row >= a.outer * a.inner) return;  // whole warps of the warp form
   if (C > 1) cluster_arrive();  // every CTA's shared memory may be written once all have started
@@ -353,7 +360,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
   uint64_t* cand = reinterpret_cast<uint64_t*>(base + kGroupShared);
   int* queue = reinterpret_cast<int*>(cand + candidate_room<T>(K));  // cells to look at again
   uint32_t* item_at = reinterpret_cast<uint32_t*>(cand);  // where a value's first element is
-  uint64_t* lists = reinterpret_cast<uint64_t*>(base + kGroupShared + candidate_smem<T, G>(K, plan.cells));
+  uint64_t* lists = reinterpret_cast<uint64_t*>(base + kGroupShared + candidate_smem<T, G>(K, plan.cells, C));
   uint32_t* cells = reinterpret_cast<uint32_t*>(lists + C * K);  // [cell][thread]: largest value key
   uint32_t* items = cells + (plan.cells + 1) * G;                // threads' largest (not for a warp)
 
@@ -365,11 +372,14 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
   uint4 first[U];
   load_batch<T, G>(first, vec, v0, v1, tid);
   Token tok = {false, true, 0.0f};
-  if (tid == 0 && rank == 0 && a.tokens != nullptr) tok = load_token(a, x, o, i);
+  // One warp (the second of a CTA, while the first is at the list's bound) has the row's figures.
+  const bool figurer = G == 32 || (threadIdx.x >> 5) == 1;
+  if (figurer && (threadIdx.x & 31) == 0 && rank == 0 && a.tokens != nullptr) tok = load_token(a, x, o, i);
   int edge = -1;  // this thread's element of the row's ends
   if (rank == 0 && tid < span.head) edge = tid;
   if (rank == C - 1 && tid >= 8 && tid - 8 < span.tail) edge = V - span.tail + tid - 8;
   const float edge_x = edge >= 0 ? logit_at<T>(x, edge) : neg_inf();
+  const int cell_vecs = 1 << plan.cell_shift;
   SoftSums<true> sums;
 
   int cell = 0, in_cell = 0;          // TOP: cells written, vectors in the open one
@@ -382,7 +392,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
   };
   stream<T, G>(first, vec, v0, v1, tid, [&](const uint4 (&w)[U], int b) {
     float largest;
-    if (TOP && plan.cell_vecs == 1) {
+    if (TOP && cell_vecs == 1) {
       largest = neg_inf();
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -396,7 +406,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
       if (TOP) {
         cell_max = max_nan(cell_max, largest);
         in_cell += U;
-        if (in_cell == plan.cell_vecs || b + G * U >= v1) {
+        if (in_cell == cell_vecs || b + G * U >= v1) {
           put_cell(cell_max, b + (U - in_cell) * G + tid < v1);
           in_cell = 0;
           cell_max = neg_inf();
@@ -408,38 +418,53 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
   SoftState st = sums.wide ? soft_slowly<T, G>(vec, v0, v1, tid, c) : sums.state(c);
   if (edge >= 0) soft_add(st, edge_x, c);
   st = soft_join(st, c);
-  if (G > 32) {
-    if ((threadIdx.x & 31) == 0) sh.warp_part[threadIdx.x >> 5] = st;
-    __syncthreads();
-    st = soft_join((threadIdx.x & 31) < kWarps ? sh.warp_part[threadIdx.x & 31] : soft_empty(), c);
-  }
+  if (G > 32 && (threadIdx.x & 31) == 0) sh.warp_part[threadIdx.x >> 5] = st;
 
-  if (TOP) {
+  auto figures = [&](const SoftState& row_st) {
+    const float ln_s = ln_sum(row_st);
+    if ((threadIdx.x & 31) == 0) {
+      sh.m = row_st.m;
+      sh.ln_s = ln_s;
+      write_figures(a, row, row_st, ln_s, inv_t, tok);
+    }
+  };
+  auto join_warps = [&] {
+    if (!figurer) return;
+    if (G > 32) st = soft_join((threadIdx.x & 31) < G / 32 ? sh.warp_part[threadIdx.x & 31] : soft_empty(), c);
+    if (C == 1) figures(st);
+  };
+  if (!TOP) {
+    group_sync<G>();
+    join_warps();
+  } else {
     const uint32_t edge_key = edge >= 0 ? value_key(edge_x) : 0u;
     cells[cell * G + tid] = edge_key;  // the last cell: the row's ends
     own = max(own, edge_key);
-    const int n_items = G == 32 ? (cell + 1) * 32 : G;
     if (G > 32) items[tid] = own;
-    if (tid == 0) sh.found = sh.queued = 0;
+    if (tid == 0) sh.found = sh.queued = sh.kept = 0;
     group_sync<G>();
+    join_warps();
     const uint32_t* keys = G == 32 ? cells : items;
-    const int most = K + top_slack(K);
+    constexpr int kItems = G == 32 ? kWarpCells + 1 : G / 32;  // per lane of the searching warp
+    const int n_items = G == 32 ? (cell + 1) * 32 : G, most = K + top_slack(K);
     // First by value (one warp): at least K items at or above lo, as a rule not many more.
     if (tid < 32) {
-      uint32_t lo = 0xffffffffu, hi = 0;
+      uint32_t mine[kItems], lo = 0xffffffffu, hi = 0;
       int some = 0;
-      for (int n = tid; n < n_items; n += 32) {
-        const uint32_t k = keys[n];
-        if (k != 0) lo = min(lo, k);
-        hi = max(hi, k);
-        some += k != 0 ? 1 : 0;
+#pragma unroll
+      for (int n = 0; n < kItems; ++n) {
+        mine[n] = n * 32 + tid < n_items ? keys[n * 32 + tid] : 0u;
+        if (mine[n] != 0) lo = min(lo, mine[n]);
+        hi = max(hi, mine[n]);
+        some += mine[n] != 0 ? 1 : 0;
       }
       lo = __reduce_min_sync(0xffffffffu, lo);
       hi = __reduce_max_sync(0xffffffffu, hi);
       some = __reduce_add_sync(0xffffffffu, some);
       auto from = [&](uint32_t v) {
         int n = 0;
-        for (int k = tid; k < n_items; k += 32) n += keys[k] >= v ? 1 : 0;
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) n += mine[k] >= v ? 1 : 0;
         return static_cast<int>(__reduce_add_sync(0xffffffffu, n));
       };
       uint64_t bound = 0;  // fewer than K items: every element is a candidate
@@ -467,8 +492,8 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
     uint32_t last = 0xffffffffu;  // of elements with value lo, those up to this index
     auto first_at = [&](int q) {  // the first element with value lo of this thread's cell q
       if (q == cell) return static_cast<uint32_t>(edge);
-      for (int n = 0; n < plan.cell_vecs; ++n) {
-        const int v = v0 + (q * plan.cell_vecs + n) * G + tid;
+      for (int n = 0; n < cell_vecs; ++n) {
+        const int v = v0 + (q * cell_vecs + n) * G + tid;
         if (v >= v1) break;
         float part[kV];
         unpack(__ldg(vec + v), part);
@@ -525,7 +550,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
     if (own >= lo)
       for (int q = 0; q < cell; ++q) {
         const uint32_t k = cells[q * G + tid];
-        const int v = v0 + q * plan.cell_vecs * G + tid;
+        const int v = v0 + q * cell_vecs * G + tid;
         if (k < lo || v >= v1 || (k == lo && static_cast<uint32_t>(span.head + v * kV) > last)) continue;
         const int n = atomicAdd(&sh.queued, 1);
         if (n < room) queue[n] = v;
@@ -534,8 +559,8 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
     // All threads on the queued cells' vectors, one each, so that their loads are under way together.
     const int queued = sh.queued;
     if (queued <= room)
-      for (int n = tid; n < queued * plan.cell_vecs; n += G) {
-        const int v = queue[n / plan.cell_vecs] + n % plan.cell_vecs * G;
+      for (int n = tid; n < queued * cell_vecs; n += G) {
+        const int v = queue[n >> plan.cell_shift] + (n & (cell_vecs - 1)) * G;
         if (v >= v1) continue;
         float part[kV];
         unpack(__ldg(vec + v), part);
@@ -575,7 +600,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
           __syncthreads();
           if ((threadIdx.x & 31) == 0) sh.best[threadIdx.x >> 5] = best;
           __syncthreads();
-          for (int w = 0; w < kWarps; ++w) best = sh.best[w] > best ? sh.best[w] : best;
+          for (int w = 0; w < G / 32; ++w) best = sh.best[w] > best ? sh.best[w] : best;
         }
         if (tid == 0) list[k] = best;
         before = best;
@@ -586,7 +611,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
 
   if (C > 1) {
     cluster_wait();
-    if (tid == 0) {
+    if (figurer && (threadIdx.x & 31) == 0) {
       const uint32_t to = peer_smem(&sh.part[rank], 0);
       peer_store(to, st.m);
       peer_store(to + 4, st.s);
@@ -597,30 +622,39 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(TokenLogprobsA
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
-    st = soft_join((threadIdx.x & 31) < C ? sh.part[threadIdx.x & 31] : soft_empty(), c);
+    if (figurer) figures(soft_join((threadIdx.x & 31) < C ? sh.part[threadIdx.x & 31] : soft_empty(), c));
   }
 
-  const float ln_s = ln_sum(st);
-  if (tid == 0) write_figures(a, row, st, ln_s, inv_t, tok);
   if (TOP) {
-    for (int n = tid; n < C * K; n += G) {
-      const uint64_t mine = lists[n];
-      if (mine == 0) continue;  // a slice shorter than K
-      int place = n % K;
-      for (int r = 0; r < C; ++r) {  // and how many of the other slices' lists come before it
-        if (r == n / K) continue;
-        int left = 0, right = K;
-        while (left < right) {
-          const int mid = (left + right) / 2;
-          if (lists[r * K + mid] > mine) left = mid + 1;
-          else right = mid;
-        }
-        place += left;
+    const uint64_t* sorted = lists;
+    int n_sorted = K;
+    if (C > 1) {
+      // Of the slices' lists, what is not below the largest of their last entries (at least K are
+      // not): few more than K. A slice shorter than K has zeros at its list's end.
+      uint64_t floor = 1;
+      for (int r = 0; r < C; ++r) floor = max(floor, lists[r * K + K - 1]);
+      for (int n = tid; n < C * K; n += G) {
+        const uint64_t mine = lists[n];
+        if (mine < floor) continue;
+        cand[atomicAdd(&sh.kept, 1)] = mine;  // (room for C K: candidate_smem)
+      }
+      __syncthreads();
+      sorted = cand;
+      n_sorted = sh.kept;
+    }
+    const SoftState row_st = {sh.m, 0.0f, 0.0f};
+    const float ln_s = sh.ln_s;
+    for (int n = tid; n < n_sorted; n += G) {
+      const uint64_t mine = sorted[n];
+      int place = n;
+      if (C > 1) {
+        place = 0;
+        for (int q = 0; q < n_sorted; ++q) place += cand[q] > mine ? 1 : 0;
       }
       if (place < K) {
         a.top_index[row * K + place] = key_index(mine);
         a.top_logprob[row * K + place] =
-            logprob_of(key_value(static_cast<uint32_t>(mine >> 32)), st, ln_s, inv_t);
+            logprob_of(key_value(static_cast<uint32_t>(mine >> 32)), row_st, ln_s, inv_t);
       }
     }
   }
@@ -730,11 +764,12 @@ int launch_forward(const TokenLogprobsArgs& a, int cluster, cudaStream_t stream)
   // vectors that a thread reads of its slice; a cell for each in a warp's row while they are few
   const int64_t mine = std::max<int64_t>(1, ((a.V / kVec<T> + cluster - 1) / cluster + G - 1) / G);
   const int64_t batches = (mine + kUnroll - 1) / kUnroll;
-  plan.cell_vecs = G == 32 && mine <= kWarpCells
-                       ? 1
-                       : static_cast<int>((batches + kMaxCells - 1) / kMaxCells) * kUnroll;
-  plan.cells = static_cast<int>((mine + plan.cell_vecs - 1) / plan.cell_vecs);
-  constexpr int kGroups = kThreads / G;
+  plan.cell_shift = 0;
+  if (G != 32 || mine > kWarpCells)
+    for (plan.cell_shift = 2; (batches * kUnroll) >> plan.cell_shift > kMaxCells;) ++plan.cell_shift;
+  static_assert(kUnroll == 4, "a cell is some batches");
+  plan.cells = static_cast<int>((mine + (int64_t(1) << plan.cell_shift) - 1) >> plan.cell_shift);
+  constexpr int kGroups = cta_threads<G> / G;
   const size_t smem = kGroups * group_smem<T, G>(static_cast<int>(a.K), plan.cells, cluster);
   auto* kern = a.K > 0 ? token_logprobs_kernel<T, G, true> : token_logprobs_kernel<T, G, false>;
   if (smem > 48 * 1024) {
@@ -747,7 +782,7 @@ int launch_forward(const TokenLogprobsArgs& a, int cluster, cudaStream_t stream)
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(G == 32 ? (rows + kGroups - 1) / kGroups : rows * cluster));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(cta_threads<G>);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -782,7 +817,7 @@ int forward_by_size(const TokenLogprobsArgs& a, cudaStream_t stream) {
     return launch_forward<T, 32>(a, 1, stream);
   // Few rows: split each until there are some CTAs for every SM or a slice is one batch.
   int cluster = 1;
-  while (cluster < kMaxCluster && rows * cluster < 4 * sm_count_here() &&
+  while (cluster < kMaxCluster && 2 * rows * cluster <= 4 * sm_count_here() &&
          vecs / (2 * cluster) >= kThreads * kUnroll)
     cluster *= 2;
   return launch_forward<T, kThreads>(a, cluster, stream);

@@ -596,6 +596,38 @@ std::optional<BesideRows> token_rows(const LogitRows& x, const std::optional<at:
   return BesideRows(x, *tokens, at::kLong, -1, "tokens");
 }
 
+// The outputs of one call in one allocation: a small call spends most of its host time on them.
+// Each is a tensor of its own (not a view of another) at a 16-byte boundary of the shared storage.
+class Outputs {
+ public:
+  void add(at::Tensor* out, at::IntArrayRef shape, at::ScalarType dtype) {
+    int64_t n = 1;
+    for (int64_t d : shape) n *= d;
+    parts_.push_back({out, shape.vec(), dtype, bytes_});
+    bytes_ += (n * static_cast<int64_t>(c10::elementSize(dtype)) + 15) / 16 * 16;
+  }
+  void make(const c10::Device& device) {
+    const at::Tensor slab = at::detail::empty_cuda({bytes_}, at::kByte, device, std::nullopt);
+    for (const Part& p : parts_) {
+      at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+          c10::Storage(slab.storage()), slab.key_set(), c10::scalarTypeToTypeMeta(p.dtype));
+      t.unsafeGetTensorImpl()->set_sizes_contiguous(p.shape);
+      t.unsafeGetTensorImpl()->set_storage_offset(p.at / static_cast<int64_t>(c10::elementSize(p.dtype)));
+      *p.out = std::move(t);
+    }
+  }
+
+ private:
+  struct Part {
+    at::Tensor* out;
+    std::vector<int64_t> shape;
+    at::ScalarType dtype;
+    int64_t at;
+  };
+  std::vector<Part> parts_;
+  int64_t bytes_ = 0;
+};
+
 void check_temperature(double temperature, const char* what) {
   if (!(temperature > 0.0) || !(temperature < 1e30) || !(temperature > 1e-30))
     TORCH_CHECK_VALUE(false, std::string(what) + ": temperature must be positive and finite, got " +
@@ -609,6 +641,7 @@ std::vector<int64_t> with_entries(const LogitRows& x, int64_t k) {
 }
 
 using MaybeTensor = std::optional<at::Tensor>;
+MaybeTensor maybe(const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : std::nullopt; }
 
 // A new tensor on the logits' device from the caching allocator (of the current stream), without
 // at::empty's dispatch: a small call spends most of its host time on its outputs.
@@ -627,24 +660,27 @@ token_logprobs(const at::Tensor& logits, const MaybeTensor& tokens, int64_t top_
   check_temperature(temperature, "token_logprobs");
   const std::optional<BesideRows> tok = token_rows(x, tokens, "token_logprobs");
   const c10::cuda::CUDAGuard guard(x.t.device());
-  MaybeTensor logprob, top_logprob, top_index, stats;
-  if (tok.has_value()) logprob = fresh(x, x.lead, at::kFloat);
-  at::Tensor entropy = fresh(x, x.lead, at::kFloat), lse = fresh(x, x.lead, at::kFloat);
+  at::Tensor logprob, entropy, lse, top_logprob, top_index, stats;
+  Outputs outputs;
+  if (tok.has_value()) outputs.add(&logprob, x.lead, at::kFloat);
+  outputs.add(&entropy, x.lead, at::kFloat);
+  outputs.add(&lse, x.lead, at::kFloat);
   if (top_k > 0) {
-    top_logprob = fresh(x, with_entries(x, top_k), at::kFloat);
-    top_index = fresh(x, with_entries(x, top_k), at::kLong);
+    outputs.add(&top_logprob, with_entries(x, top_k), at::kFloat);
+    outputs.add(&top_index, with_entries(x, top_k), at::kLong);
   }
-  if (want_stats) stats = fresh(x, {x.rows(), 2}, at::kFloat);
-  auto fp = [](const MaybeTensor& t) { return t.has_value() ? t->data_ptr<float>() : nullptr; };
+  if (want_stats) outputs.add(&stats, {x.rows(), 2}, at::kFloat);
+  outputs.make(x.t.device());
+  auto fp = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
   check_rc(bdh_token_logprobs(
                x.t.data_ptr(), dtype_code(x.t), x.strides,
                tok.has_value() ? tok->t.data_ptr<int64_t>() : nullptr, strides_of(tok),
                ignore_index, fp(logprob), lse.data_ptr<float>(), entropy.data_ptr<float>(),
                fp(stats), fp(top_logprob),
-               top_index.has_value() ? top_index->data_ptr<int64_t>() : nullptr, x.outer, x.inner,
+               top_index.defined() ? top_index.data_ptr<int64_t>() : nullptr, x.outer, x.inner,
                x.V, top_k, static_cast<float>(temperature), stream_of(x.t)),
            "token_logprobs");
-  return {logprob, entropy, lse, top_logprob, top_index, stats};
+  return {maybe(logprob), entropy, lse, maybe(top_logprob), maybe(top_index), maybe(stats)};
 }
 
 at::Tensor token_logprobs_bwd(const at::Tensor& logits, const MaybeTensor& tokens,
@@ -762,7 +798,6 @@ at::Tensor distill_topk_bwd(const at::Tensor& logits, const at::Tensor& index,
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-MaybeTensor maybe(const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : std::nullopt; }
 at::Tensor defined_or_not(const MaybeTensor& t) { return t.value_or(at::Tensor()); }
 
 variable_list once(variable_list grads, const at::Tensor& logits) {
