@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(32 * kWarpsHeld, 10) distill_warp_kernel(Disti
       const int v = b + u * 32 + lane;
       wv[u] = v < span.vecs ? hvec[v] : void_vec<T>();
     }
-    sums.add<T>(wv, max_of(wv, T()), c, slack, batch_fill<32>(b, span.vecs, lane));
+    sums.template add<T>(wv, max_of(wv, T()), c, slack, batch_fill<32>(b, span.vecs, lane), [](int) {});
   }
   SoftState rest = sums.wide ? soft_slowly<T, 32>(hvec, 0, span.vecs, lane, c) : sums.state(c);
   if (edge >= 0) soft_add(rest, logit_at<T>(held, edge), c);
@@ -609,13 +609,15 @@ __device__ __forceinline__ void write_slice(uint4 (&next)[kUnroll], const uint4*
                                             int tid, const RowMap& f) {
   constexpr int kV = kVec<T>;
   const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
-  stream<T, G>(next, vec, v0, v1, tid, [&](const uint4 (&wv)[kUnroll], int b) {
+  stream_early<T, G>(next, vec, v0, v1, tid, [&](const uint4 (&wv)[kUnroll], int b, auto fill, auto refill) {
+    constexpr bool kWhole = !std::is_same<decltype(fill), int>::value;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int v = b + u * G + tid;
-      if (v >= v1) break;
       float xs[kV], ds[kV];
       unpack(wv[u], xs);
+      refill(u);
+      if (!kWhole && v >= v1) continue;
 #pragma unroll
       for (int e = 0; e < kV; ++e) ds[e] = ex2(fmaf(xs[e], f.c, -f.b)) * f.k0;
       if (aligned) {
@@ -755,14 +757,14 @@ __global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTo
   SoftSums<false> sums;
   const float slack = kBaseSlack / c;
   const uint32_t* my_bits = bits + tid;
-  stream<T, kThreads>(next, vec, v0, v1, tid, [&](uint4 (&wv)[kUnroll], int b) {
+  stream_early<T, kThreads>(next, vec, v0, v1, tid, [&](uint4 (&wv)[kUnroll], int, auto fill, auto refill) {
     const uint32_t struck = *my_bits;
     my_bits += kThreads;
     if (struck != 0) {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) strike(wv[u], struck >> 8 * u, T());
     }
-    sums.add<T>(wv, max_of(wv, T()), c, slack, batch_fill<kThreads>(b, v1, tid));
+    sums.template add<T>(wv, max_of(wv, T()), c, slack, fill, refill);
   });
   if (d != nullptr) load_batch<T, kThreads>(next, vec, v0, v1, tid);  // again, for the gradient
   SoftState rest = soft_empty();

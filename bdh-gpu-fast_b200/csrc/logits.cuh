@@ -17,6 +17,7 @@
 #pragma once
 
 #include <cstdint>
+#include <type_traits>
 
 #include "bdh_sm100.h"
 #include "common.cuh"
@@ -132,6 +133,19 @@ __device__ __forceinline__ float max_of(const uint4 (&w)[N], uint16_t) {
     m = max_bf16x2(m, max_bf16x2(max_bf16x2(w[u].x, w[u].y), max_bf16x2(w[u].z, w[u].w)));
   return max_nan(bf16x2_lo(m), bf16x2_hi(m));
 }
+// A vector with what is below kLeast raised to it: the least logit of an entropy's sum, whose
+// exponential is 0 (the base is within kWide / c of 0) and times which 0 is 0.
+constexpr float kLeast = -1267650600228229401496703205376.0f;  // -2^100
+__device__ __forceinline__ uint4 at_least(const uint4& w, float) {
+  return make_uint4(__float_as_uint(max_nan(__uint_as_float(w.x), kLeast)),
+                    __float_as_uint(max_nan(__uint_as_float(w.y), kLeast)),
+                    __float_as_uint(max_nan(__uint_as_float(w.z), kLeast)),
+                    __float_as_uint(max_nan(__uint_as_float(w.w), kLeast)));
+}
+__device__ __forceinline__ uint4 at_least(const uint4& w, uint16_t) {
+  constexpr uint32_t kTwo = 0xf180f180u;  // -2^100 twice
+  return make_uint4(max_bf16x2(w.x, kTwo), max_bf16x2(w.y, kTwo), max_bf16x2(w.z, kTwo), max_bf16x2(w.w, kTwo));
+}
 // A vector of -inf: what a place past the end of a row counts as.
 template <typename T>
 __device__ __forceinline__ uint4 void_vec();
@@ -151,31 +165,54 @@ template <int G>
 __device__ __forceinline__ int batch_fill(int b, int v1, int tid) {
   return (v1 - b - (tid & ~31) + G - 1) / G;  // may be more than there are
 }
-// A group of G threads over the vectors [v0, v1): f(w, b) for every batch w of its kUnroll vectors
-// b + u G + tid (-inf past the end), with the next batch's loads under way meanwhile. `next` is the
-// batch at v0, asked for by the caller (load_batch) as early as it can.
+// A group of G threads over the vectors [v0, v1): f(w, b, fill, refill) for every batch w of its kUnroll
+// vectors b + u G + tid (-inf past the end). f calls refill(u) as soon as it has taken vector u out of
+// its register, so that the next batch's loads are under way while this one is worked on, without
+// registers of their own. `w` is asked for by the caller (load_batch) as early as it can. While this
+// batch and the next are whole (fill: the constant kUnroll), nothing is checked per vector.
 template <typename T, int G>
 __device__ __forceinline__ void load_batch(uint4 (&w)[kUnroll], const uint4* vec, int b, int v1, int tid) {
-  if (b + G * kUnroll <= v1) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) w[u] = __ldg(vec + b + u * G + tid);
-  } else {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int v = b + u * G + tid;
-      w[u] = v < v1 ? __ldg(vec + v) : void_vec<T>();
-    }
-  }
+  for (int u = 0; u < kUnroll; ++u)
+    if (b < v1) w[u] = __ldg(vec + min(b + u * G + tid, v1 - 1));  // (a vector past the end: any inside)
 }
 template <typename T, int G, typename F>
-__device__ __forceinline__ void stream(uint4 (&next)[kUnroll], const uint4* vec, int v0, int v1, int tid, F f) {
+__device__ __forceinline__ void stream(uint4 (&w)[kUnroll], const uint4* vec, int v0, int v1, int tid, F f) {
+  constexpr int kStep = G * kUnroll;
+  int b = v0;
+  const uint4* next = vec + v0 + kStep + tid;
+  for (; b + 2 * kStep <= v1; b += kStep, next += kStep)
+    f(w, b, std::integral_constant<int, kUnroll>(), [&](int u) { w[u] = __ldg(next + u * G); });
+  for (; b < v1; b += kStep) {
+    if (b + kStep > v1) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (b + u * G + tid >= v1) w[u] = void_vec<T>();
+    }
+    f(w, b, batch_fill<G>(b, v1, tid),
+      [&](int u) { w[u] = __ldg(vec + min(b + kStep + u * G + tid, v1 - 1)); });
+  }
+}
+
+// The same with the next batch in registers of its own, asked for before this one is looked at: more
+// instructions (the copies), and loads that are under way longer. For the two passes of a clustered row,
+// whose CTAs wait for each other and have little else in flight (2048 rows of 131072 in bf16: 229 us so,
+// 236 us with refills); the single pass over such rows is better off with the refills (163 against 167 us).
+template <typename T, int G, typename F>
+__device__ __forceinline__ void stream_early(uint4 (&next)[kUnroll], const uint4* vec, int v0, int v1, int tid,
+                                             F f) {
   constexpr int kStep = G * kUnroll;
   for (int b = v0; b < v1; b += kStep) {
     uint4 w[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) w[u] = next[u];
-    if (b + kStep < v1) load_batch<T, G>(next, vec, b + kStep, v1, tid);
-    f(w, b);
+    load_batch<T, G>(next, vec, b + kStep, v1, tid);
+    if (b + kStep > v1) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (b + u * G + tid >= v1) w[u] = void_vec<T>();
+    }
+    f(w, b, batch_fill<G>(b, v1, tid), [](int) {});
   }
 }
 
@@ -292,24 +329,28 @@ struct SoftSums {
     m = largest;
     limit = largest + slack;
   }
-  // N vectors whose largest element is `largest`; of a row's last ones, `fill` of them.
-  template <typename T, int N>
-  __device__ __forceinline__ void add(const uint4 (&w)[N], float largest, float c, float slack, int fill) {
+  // N vectors whose largest element is `largest`; of a row's last ones, `fill` of them. taken(u): vector
+  // u is out of its register.
+  template <typename T, int N, typename Fill, typename Taken>
+  __device__ __forceinline__ void add(const uint4 (&w)[N], float largest, float c, float slack, Fill fill,
+                                      Taken taken) {
     if (!(largest <= limit)) raise(largest, c, slack);  // a NaN too
-    if (wide || m == neg_inf()) return;
+    const bool sum = !wide && m != neg_inf();
     float ps[2] = {0.0f, 0.0f}, pa[2] = {0.0f, 0.0f};  // (a batch's own sums: fewer terms in a row)
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      if (u > 0 && u >= fill) break;
       float x[kVec<T>];
-      unpack(w[u], x);
+      unpack(ENTROPY ? at_least(w[u], T()) : w[u], x);
+      taken(u);
+      if (u > 0 && u >= fill) continue;
 #pragma unroll
       for (int i = 0; i < kVec<T>; ++i) {
         const float t = fmaf(x[i], c, -base), e = ex2(t);
         ps[i % 2] += e;
-        if (ENTROPY) pa[i % 2] = fmaf(e, max_nan(t, kExpFloor), pa[i % 2]);
+        if (ENTROPY) pa[i % 2] = fmaf(e, t, pa[i % 2]);
       }
     }
+    if (!sum) return;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       s[i] += ps[i];

@@ -338,7 +338,7 @@ template <int G>
 constexpr int cta_threads = G == 32 ? kThreads : G;  // groups of a warp share a CTA
 
 template <typename T, int G, bool TOP>
-__global__ void __launch_bounds__(cta_threads<G>) token_logprobs_kernel(TokenLogprobsArgs a,
+__global__ void __launch_bounds__(cta_threads<G>, TOP && G > 32 ? 5 : 4) token_logprobs_kernel(TokenLogprobsArgs a,
                                                                   ForwardPlan plan, FastDiv inner) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int kV = kVec<T>, U = kUnroll;
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(cta_threads<G>) token_logprobs_kernel(TokenLog
     cells[cell++ * G + tid] = k;
     own = max(own, k);
   };
-  stream<T, G>(first, vec, v0, v1, tid, [&](const uint4 (&w)[U], int b) {
+  stream<T, G>(first, vec, v0, v1, tid, [&](const uint4 (&w)[U], int b, auto fill, auto refill) {
     float largest;
     if (TOP && cell_vecs == 1) {
       largest = neg_inf();
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(cta_threads<G>) token_logprobs_kernel(TokenLog
         }
       }
     }
-    sums.add<T>(w, largest, c, slack, batch_fill<G>(b, v1, tid));
+    sums.template add<T>(w, largest, c, slack, fill, refill);
   });
   SoftState st = sums.wide ? soft_slowly<T, G>(vec, v0, v1, tid, c) : sums.state(c);
   if (edge >= 0) soft_add(st, edge_x, c);
