@@ -526,6 +526,21 @@ class BDH(nn.Module):
             x = self._ln(x + self._ln(y_mlp))
         return x
 
+    @torch.no_grad()
+    def score(self, idx: torch.Tensor, *, top_k: int = 0, temperature: float = 1.0,
+              ignore_index: int = -100):
+        """Log probabilities of the tokens ``idx[:, 1:]`` under this model, each given those before
+        it, with entropies and the ``top_k`` alternatives of every position: a
+        ``kernels.TokenLogprobs`` of (B, T - 1) figures (see ``kernels.token_logprobs``; a token
+        equal to ``ignore_index`` is fed to the model as token 0 and scores 0). The native kernels
+        read the (B, T, V) logits once, through the shifted view; CUDA only."""
+        from kernels import token_logprobs
+
+        fed = idx.masked_fill(idx == ignore_index, 0)
+        logits, _ = self(fed)
+        return token_logprobs(logits[:, :-1], idx[:, 1:], top_k=top_k, temperature=temperature,
+                              ignore_index=ignore_index)
+
     def graphed_forward(self, batch: int, seq_len: int,
                         amp_dtype: Optional[torch.dtype] = torch.bfloat16) -> "GraphedForward":
         """This model's no-grad prefill for one (batch, seq_len) captured as a CUDA graph (see

@@ -16,8 +16,7 @@
 // way: every slot writes its number in place of its token's logit and reads it back.
 // A longer row is streamed by a CTA, or by a cluster whose CTAs take a slice each and exchange their
 // sums through distributed shared memory; a bit per element in shared memory says what is listed (and
-// was set twice for a repeated token). For the gradient the slice is streamed again: the slices in
-// flight are 64 KB for each of some 600 CTAs, so that the second read finds them in L2.
+// was set twice for a repeated token). For the gradient the slice is streamed again, from L2.
 // Where a token is repeated its masses are added up by a search (K^2 comparisons, seldom needed).
 // The backward from stored statistics has nothing to sum.
 #include <algorithm>
@@ -36,11 +35,15 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kPiece = 16384;             // elements of a row per CTA of the streaming backward
-constexpr int kWarpRowBytes = 24 * 1024;  // longest row that a warp takes
-constexpr int kWarpRows = 8;               // rows for every SM from which it does
-constexpr int kWarpsHeld = 4;              // rows of a CTA then
-constexpr int kSliceBytes = 68 * 1024;    // of a row per CTA, while the cluster may grow
-
+// A warp takes rows up to kWarpRowBytes where there are kWarpRows for every SM (kWarpsHeld a CTA, each
+// held in shared memory). 8192 rows of 2048 in bf16: 25 us, against 80 us by CTAs; fewer rows leave
+// warps idle.
+constexpr int kWarpRowBytes = 24 * 1024, kWarpRows = 8, kWarpsHeld = 4;
+// With a gradient, a row longer than this is split over a cluster: the slices of some 600 CTAs in flight
+// are read again from L2. 2048 rows of 131072 in bf16: 128 KB slices 213 us, 64 KB 228 us (two CTAs more
+// to wait for), whole rows of 256 KB 249 us (they no longer fit L2). Without the L2 policies 232, 224 and
+// 255 us: the DRAM reads of 128 KB slices are then 0.98 GB, of 64 KB slices 0.54 GB.
+constexpr int kSliceBytes = 136 * 1024;
 
 constexpr int kStats = 8;  // floats per row: see RowStats
 
@@ -606,10 +609,10 @@ __device__ __forceinline__ SoftState soft_slowly_struck(const uint4* vec, int v0
 // wide row).
 template <typename T, int G>
 __device__ __forceinline__ void write_slice(uint4 (&next)[kUnroll], const uint4* vec, T* out, int v0, int v1,
-                                            int tid, const RowMap& f) {
+                                            int tid, uint64_t drop, const RowMap& f) {
   constexpr int kV = kVec<T>;
   const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
-  stream_early<T, G>(next, vec, v0, v1, tid, [&](const uint4 (&wv)[kUnroll], int b, auto fill, auto refill) {
+  stream_early<T, G>(next, vec, v0, v1, tid, drop, [&](const uint4 (&wv)[kUnroll], int b, auto fill, auto refill) {
     constexpr bool kWhole = !std::is_same<decltype(fill), int>::value;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -621,7 +624,7 @@ __device__ __forceinline__ void write_slice(uint4 (&next)[kUnroll], const uint4*
 #pragma unroll
       for (int e = 0; e < kV; ++e) ds[e] = ex2(fmaf(xs[e], f.c, -f.b)) * f.k0;
       if (aligned) {
-        store_vec(out + static_cast<int64_t>(v) * kV, ds);
+        st_global_v4_hint(out + static_cast<int64_t>(v) * kV, pack(ds), drop);
       } else {
 #pragma unroll
         for (int e = 0; e < kV; ++e) logit_put(out, static_cast<int64_t>(v) * kV + e, ds[e]);
@@ -662,12 +665,16 @@ __global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTo
   const int from = span.head + v0 * kV - head, n = head + (v1 - v0) * kV + tail;
   const float inv_t = a.inv_t, c = a.c;
 
+  // The first pass's lines stay in L2 for the second, which lets go of them, as the gradient's do.
+  const uint64_t drop = l2_policy_evict_first();
+  const uint64_t keep = d != nullptr ? l2_policy_evict_last() : drop;
+
   uint4 next[kUnroll];
   int edge = -1;
   float edge_x = neg_inf();
   int slot_at[kTopMax / 32];  // the lister's slots
   if (!lister) {
-    load_batch<T, kThreads>(next, vec, v0, v1, tid);
+    load_batch<kThreads>(next, vec, v0, v1, tid, keep);
     edge = tid < head ? from + tid : tid - head < tail ? V - tail + tid - head : -1;
     if (edge >= 0) edge_x = logit_at<T>(x, edge);
     for (int k = tid; k < slice_batches<T>(V, C) * kThreads; k += kThreads) bits[k] = 0;
@@ -757,7 +764,7 @@ __global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTo
   SoftSums<false> sums;
   const float slack = kBaseSlack / c;
   const uint32_t* my_bits = bits + tid;
-  stream_early<T, kThreads>(next, vec, v0, v1, tid, [&](uint4 (&wv)[kUnroll], int, auto fill, auto refill) {
+  stream_early<T, kThreads>(next, vec, v0, v1, tid, keep, [&](uint4 (&wv)[kUnroll], int, auto fill, auto refill) {
     const uint32_t struck = *my_bits;
     my_bits += kThreads;
     if (struck != 0) {
@@ -766,7 +773,7 @@ __global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTo
     }
     sums.template add<T>(wv, max_of(wv, T()), c, slack, fill, refill);
   });
-  if (d != nullptr) load_batch<T, kThreads>(next, vec, v0, v1, tid);  // again, for the gradient
+  if (d != nullptr) load_batch<kThreads>(next, vec, v0, v1, tid, drop);  // again, for the gradient
   SoftState rest = soft_empty();
   if (!sums.wide) rest = sums.state(c);
   else rest = soft_slowly_struck<T, kThreads>(vec, v0, v1, tid, c, bits);
@@ -798,7 +805,7 @@ __global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTo
   if (f.wide || none) {
     map_row<T, kThreads>(x + from + head, d + from + head, n - head - tail, tid, none, f);
   } else {
-    write_slice<T, kThreads>(next, vec, d + span.head, v0, v1, tid, f);
+    write_slice<T, kThreads>(next, vec, d + span.head, v0, v1, tid, drop, f);
   }
   if (!none) __syncthreads();
 }

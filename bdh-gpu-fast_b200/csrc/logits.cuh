@@ -100,13 +100,18 @@ __device__ __forceinline__ void unpack(const uint4& u, float (&x)[8]) {
     x[2 * i + 1] = bf16x2_hi(w[i]);
   }
 }
-// The other way, to a 16-byte aligned place.
-__device__ __forceinline__ void store_vec(float* p, const float (&x)[4]) {
-  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+// The other way, and to a 16-byte aligned place.
+__device__ __forceinline__ uint4 pack(const float (&x)[4]) {
+  return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                    __float_as_uint(x[3]));
 }
-__device__ __forceinline__ void store_vec(uint16_t* p, const float (&x)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(cvt_bf16x2(x[0], x[1]), cvt_bf16x2(x[2], x[3]),
-                                            cvt_bf16x2(x[4], x[5]), cvt_bf16x2(x[6], x[7]));
+__device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+  return make_uint4(cvt_bf16x2(x[0], x[1]), cvt_bf16x2(x[2], x[3]), cvt_bf16x2(x[4], x[5]),
+                    cvt_bf16x2(x[6], x[7]));
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
+  *reinterpret_cast<uint4*>(p) = pack(x);
 }
 // The largest element of N vectors (bf16 in pairs, where one instruction compares two).
 template <int N>
@@ -194,19 +199,32 @@ __device__ __forceinline__ void stream(uint4 (&w)[kUnroll], const uint4* vec, in
   }
 }
 
-// The same with the next batch in registers of its own, asked for before this one is looked at: more
-// instructions (the copies), and loads that are under way longer. For the two passes of a clustered row,
-// whose CTAs wait for each other and have little else in flight (2048 rows of 131072 in bf16: 229 us so,
-// 236 us with refills); the single pass over such rows is better off with the refills (163 against 167 us).
+// The same for a slice that is read twice: with an L2 cache policy on its loads, and with the next batch
+// in registers of its own, asked for before this one is looked at, which costs the copies but has the
+// loads under way longer (f's refill does nothing).
+__device__ __forceinline__ uint4 ld_vec(const uint4* p, uint64_t policy) {
+  uint4 r;
+  asm volatile("ld.global.nc.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p), "l"(policy));
+  return r;
+}
+template <int G>
+__device__ __forceinline__ void load_batch(uint4 (&w)[kUnroll], const uint4* vec, int b, int v1, int tid,
+                                           uint64_t policy) {
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u)
+    if (b < v1) w[u] = ld_vec(vec + min(b + u * G + tid, v1 - 1), policy);
+}
 template <typename T, int G, typename F>
 __device__ __forceinline__ void stream_early(uint4 (&next)[kUnroll], const uint4* vec, int v0, int v1, int tid,
-                                             F f) {
+                                             uint64_t policy, F f) {
   constexpr int kStep = G * kUnroll;
   for (int b = v0; b < v1; b += kStep) {
     uint4 w[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) w[u] = next[u];
-    load_batch<T, G>(next, vec, b + kStep, v1, tid);
+    load_batch<G>(next, vec, b + kStep, v1, tid, policy);
     if (b + kStep > v1) {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u)

@@ -25,10 +25,10 @@ int check_rows(const char* what, int dtype, int64_t outer, int64_t inner, int64_
   if (dtype != BDH_DTYPE_F32 && dtype != BDH_DTYPE_BF16)
     return refuse(what, "dtype must be f32 or bf16");
   if (outer < 0 || inner < 0 || V < 0 || K < 0) return refuse(what, "negative size");
-  const int64_t most = (int64_t(1) << 31) - 1;
+  const int64_t most = (int64_t(1) << 31) - 1024;  // (rows are rounded up to whole CTAs in 32 bits)
   if (V < 1 || V > (int64_t(1) << 30)) return refuse(what, "vocabulary must be 1 to 2^30 wide");
   if (outer > most || inner > most || (inner > 0 && outer > most / inner))
-    return refuse(what, "at most 2^31 - 1 rows");
+    return refuse(what, "at most 2^31 - 1024 rows");
   if (K > BDH_TOP_MAX) return refuse(what, "at most BDH_TOP_MAX entries in a row's list");
   if (!(temperature > 1e-30f && temperature < 1e30f))  // so that 1 / temperature has room as well
     return refuse(what, "temperature must be positive and finite");

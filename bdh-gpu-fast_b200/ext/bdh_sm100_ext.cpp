@@ -800,6 +800,18 @@ using torch::autograd::variable_list;
 
 at::Tensor defined_or_not(const MaybeTensor& t) { return t.value_or(at::Tensor()); }
 
+// What backward needs of a constant input: saved as a variable (so that a later change in place is
+// noticed), or, where it was made in inference mode, which cannot be, beside the variables.
+at::Tensor constant(AutogradContext* ctx, const char* name, const at::Tensor& t) {
+  if (!t.defined() || !t.is_inference()) return t;
+  ctx->saved_data[name] = t;
+  return at::Tensor();
+}
+at::Tensor constant_back(AutogradContext* ctx, const char* name, const at::Tensor& saved) {
+  const auto it = ctx->saved_data.find(name);
+  return it == ctx->saved_data.end() ? saved : it->second.toTensor();
+}
+
 variable_list once(variable_list grads, const at::Tensor& logits) {
   if (!at::GradMode::is_enabled()) return grads;
   // beside the logits, so that a second derivative by anything they come from finds the error
@@ -816,7 +828,8 @@ struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
     auto [logprob, entropy, lse, top_logprob, top_index, stats] =
         token_logprobs(logits, tokens, top_k, temperature, ignore_index, true);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({logits, defined_or_not(tokens), *stats, entropy, defined_or_not(top_index)});
+    ctx->save_for_backward({logits, constant(ctx, "tokens", defined_or_not(tokens)), *stats, entropy,
+                            defined_or_not(top_index)});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["ignore_index"] = ignore_index;
     variable_list out = {entropy, lse};  // the figures asked for: a node has no undefined outputs
@@ -830,7 +843,8 @@ struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     variable_list out(5);
-    const variable_list saved = ctx->get_saved_variables();
+    variable_list saved = ctx->get_saved_variables();
+    saved[1] = constant_back(ctx, "tokens", saved[1]);
     const size_t top = saved[1].defined() ? 3 : 2;
     const at::Tensor g_logprob = saved[1].defined() ? g[2] : at::Tensor(),
                      g_top = saved[4].defined() ? g[top] : at::Tensor();
@@ -862,7 +876,8 @@ struct DistillTopkFn : torch::autograd::Function<DistillTopkFn> {
                             const at::Tensor& teacher, const MaybeTensor& weight,
                             double temperature, bool tail) {
     auto [loss, d, stats] = distill_topk(logits, index, teacher, weight, temperature, tail, false, true);
-    ctx->save_for_backward({logits, index, teacher, defined_or_not(weight), *stats});
+    ctx->save_for_backward({logits, constant(ctx, "index", index), constant(ctx, "teacher", teacher),
+                            constant(ctx, "weight", defined_or_not(weight)), *stats});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["tail"] = tail;
     return loss;
@@ -870,7 +885,9 @@ struct DistillTopkFn : torch::autograd::Function<DistillTopkFn> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const variable_list saved = ctx->get_saved_variables();
     variable_list out(6);
-    out[0] = distill_topk_bwd(saved[0], saved[1], saved[2], maybe(saved[3]), saved[4], g[0],
+    out[0] = distill_topk_bwd(saved[0], constant_back(ctx, "index", saved[1]),
+                              constant_back(ctx, "teacher", saved[2]),
+                              maybe(constant_back(ctx, "weight", saved[3])), saved[4], g[0],
                               ctx->saved_data["temperature"].toDouble(),
                               ctx->saved_data["tail"].toBool());
     return once(out, saved[0]);

@@ -49,13 +49,26 @@ def _once(d: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
 
 
 # The autograd nodes of the ctypes binding; the extension has its own (a tenth of the host time).
+def _save(ctx, constants: dict, **variables) -> None:
+    """save_for_backward, with constant inputs that were made in inference mode (and so cannot be
+    saved) kept beside it."""
+    ctx.beside = {k: t for k, t in constants.items() if t is not None and t.is_inference()}
+    ctx.names = list(constants) + list(variables)
+    ctx.save_for_backward(*(None if k in ctx.beside else t for k, t in constants.items()),
+                          *variables.values())
+
+
+def _saved(ctx) -> dict:
+    return {**dict(zip(ctx.names, ctx.saved_tensors)), **ctx.beside}
+
+
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top_k, temperature, ignore_index):
         logprob, entropy, lse, top, index, stats = _ops().token_logprobs(
             logits, tokens, top_k, temperature, ignore_index, True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, tokens, stats, entropy, index)
+        _save(ctx, {"tokens": tokens}, logits=logits, stats=stats, entropy=entropy, top_index=index)
         ctx.opts = (temperature, ignore_index)
         if index is not None:
             ctx.mark_non_differentiable(index)
@@ -65,10 +78,12 @@ class _TokenLogprobsFn(torch.autograd.Function):
     def backward(ctx, g_logprob, g_entropy, g_lse, g_top, _):
         if g_logprob is None and g_entropy is None and g_lse is None and g_top is None:
             return (None,) * 5
-        logits, tokens, stats, entropy, index = ctx.saved_tensors
-        d = _ops().token_logprobs_bwd(logits, tokens, stats, entropy, index, g_logprob, g_entropy,
-                                      g_lse, g_top, *ctx.opts)
-        return _once(d, logits), None, None, None, None
+        temperature, ignore_index = ctx.opts
+        saved = _saved(ctx)
+        d = _ops().token_logprobs_bwd(**saved, g_logprob=g_logprob, g_entropy=g_entropy, g_lse=g_lse,
+                                      g_top=g_top, temperature=temperature,
+                                      ignore_index=ignore_index)
+        return _once(d, saved["logits"]), None, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top_k: int = 0,
@@ -100,15 +115,17 @@ class _DistillTopkFn(torch.autograd.Function):
     def forward(ctx, logits, index, teacher, weight, temperature, tail):
         loss, _, stats = _ops().distill_topk(logits, index, teacher, weight, temperature, tail,
                                              False, True)
-        ctx.save_for_backward(logits, index, teacher, weight, stats)
+        _save(ctx, {"teacher_index": index, "teacher_logprob": teacher, "weight": weight},
+              logits=logits, stats=stats)
         ctx.opts = (temperature, tail)
         return loss
 
     @staticmethod
     def backward(ctx, g_loss):
-        logits, index, teacher, weight, stats = ctx.saved_tensors
-        d = _ops().distill_topk_bwd(logits, index, teacher, weight, stats, g_loss, *ctx.opts)
-        return _once(d, logits), None, None, None, None, None
+        temperature, tail = ctx.opts
+        saved = _saved(ctx)
+        d = _ops().distill_topk_bwd(**saved, g_loss=g_loss, temperature=temperature, tail=tail)
+        return _once(d, saved["logits"]), None, None, None, None, None
 
 
 def _constant_teacher(teacher_logprob, weight) -> None:

@@ -593,3 +593,22 @@ def test_logits_changed_after_the_forward_are_noticed():
     y.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         r.logprob.sum().backward()
+
+
+@pytest.mark.parametrize("binding", ["ext", "ctypes"])
+def test_lists_and_tokens_made_in_inference_mode(binding, monkeypatch):
+    """A teacher's pass is often made there; its tensors cannot be saved as variables."""
+    monkeypatch.setenv("BDH_SM100_EXT", "1" if binding == "ext" else "0")
+    x = make((4,), 500, torch.float32)
+    with torch.inference_mode():
+        tok = tokens((4,), 500).cuda()
+        top = kernels.token_logprobs(x, tok, top_k=6)
+        w = torch.rand(4, device="cuda")
+    z = (x + 0.1 * torch.randn_like(x)).requires_grad_(True)
+    loss = kernels.distill_topk_loss(z, top.top_index, top.top_logprob, weight=w, tail=True)
+    r = kernels.token_logprobs(z, tok)
+    (d,) = torch.autograd.grad(loss.sum() + r.logprob.sum(), z)
+    zc = z.detach().cpu()
+    ref = L.distill_grad(zc, top.top_index.cpu(), top.top_logprob.cpu(), w.cpu(), 1.0, True)
+    ref = ref + L.token_logprobs_grad(zc, tok.cpu(), g_logprob=torch.ones(4))
+    check_grad(d, ref, 2 * w.cpu() + 1, 500, torch.float32)
