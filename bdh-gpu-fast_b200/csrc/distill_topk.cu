@@ -7,7 +7,8 @@
 //   loss  = w [ sum_j q_j (ln q_j - ln p[token_j]) + r (ln r - ln s) ]
 //   dx_i  = w/temperature [ p_i (sum_j q_j + r) - r (p_i / s) [i unlisted] - sum_j q_j [i = token_j] ]
 //
-// A slot with token < 0 is empty; a repeated token's masses add; a row of weight 0 is not read.
+// A slot with token < 0 is empty; a repeated token's masses add; a row of weight 0 counts for nothing,
+// whatever it holds.
 // The unlisted tokens are summed by themselves, so that s keeps its digits when the list holds
 // nearly everything.
 //
@@ -19,6 +20,13 @@
 // was set twice for a repeated token). For the gradient the slice is streamed again, from L2.
 // Where a token is repeated its masses are added up by a search (K^2 comparisons, seldom needed).
 // The backward from stored statistics has nothing to sum.
+//
+// What bounds it: of long rows with a gradient neither memory nor the issue slots alone (66% and 0.63 of
+// them in use): 2048 rows of 131072 in bf16 with K = 64 take 213 us, 5.0 TB/s of the 1.07 GB that must be
+// read and written (DRAM moves 1.14: nearly all of the second pass comes from L2); warps wait for loads,
+// and between the passes for one another. The loss alone of 600 rows of 100003 takes 27 us, 4.5 TB/s:
+// one wave of CTAs, each with its list to fetch. Short rows with their lists are latency: 16384 rows of
+// 256 with K = 16 take 9 us with their gradient.
 #include <algorithm>
 #include <string>
 
@@ -34,13 +42,17 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kPiece = 16384;             // elements of a row per CTA of the streaming backward
+// The backward from stored statistics: elements of a row per CTA, and the longest of many rows that are
+// a warp's each. The bytes that it moves bound it, as the log probabilities' (measured there): 89 us for
+// 1024 rows of 131072 in bf16, 6.0 TB/s; 6.3 us for 16384 rows of 256 by 8 lanes each.
+constexpr int kPiece = 16384, kWarpGradBytes = 8 * 1024;
 // A warp takes rows up to kWarpRowBytes where there are kWarpRows for every SM (kWarpsHeld a CTA, each
-// held in shared memory). 8192 rows of 2048 in bf16: 25 us, against 80 us by CTAs; fewer rows leave
-// warps idle.
+// held in shared memory). Loss and gradient of 8192 rows in bf16, by warps against by CTAs: 2048 long 19
+// and 83 us, 8192 long 73 and 96, 16384 long 259 and 132 (four such rows fill more than half of an SM's
+// shared memory); of 592 rows of 8192 11.9 and 8.7 us.
 constexpr int kWarpRowBytes = 24 * 1024, kWarpRows = 8, kWarpsHeld = 4;
 // With a gradient, a row longer than this is split over a cluster: the slices of some 600 CTAs in flight
-// are read again from L2. 2048 rows of 131072 in bf16: 128 KB slices 213 us, 64 KB 228 us (two CTAs more
+// are read again from L2, with policies that keep them there until then. 2048 rows of 131072 in bf16: 128 KB slices 213 us, 64 KB 228 us (two CTAs more
 // to wait for), whole rows of 256 KB 249 us (they no longer fit L2). Without the L2 policies 232, 224 and
 // 255 us: the DRAM reads of 128 KB slices are then 0.98 GB, of 64 KB slices 0.54 GB.
 constexpr int kSliceBytes = 136 * 1024;
@@ -135,7 +147,8 @@ __device__ __forceinline__ float row_weight(const DistillTopkArgs& a, int64_t o,
 // Rows of at most kShort elements: the slots and the row's elements stay in registers, S slots and E
 // elements (and up to two of its unaligned ends) in each of the L lanes that have a row; the row passes
 // through shared memory for the slots to find their logits. With few lanes a row the shuffles and the
-// row's own figures serve several rows at once (a byte model's 256: 4 rows a warp).
+// row's own figures serve several rows at once (a byte model's 256: 4 rows a warp; 16384 such rows with
+// their gradient 9.0 us, 14.8 with a warp each).
 constexpr int kShort = 1024;
 
 template <typename T, int L, int E, int S>
@@ -836,7 +849,7 @@ __global__ void __launch_bounds__(kThreads) distill_topk_bwd_kernel(DistillTopkA
   const RowGradient g = row_gradient(st, a.tail, inv_t, w * up);
   map_row<T, G>(x + from, d + from, n, tid, g.none, g.unlisted(c));
   if (g.none) return;
-  if (G == 32) __syncwarp();
+  if (G <= 32) __syncwarp();
   else __syncthreads();
   // the listed tokens of this piece, over what the formula for the others left there
   const int64_t* index = a.index + o * a.i_strides[0] + i * a.i_strides[1];
@@ -903,7 +916,7 @@ int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
   int cluster = 1;
   while (cluster < kMaxCluster &&
          ((a.dlogits != nullptr && bytes > static_cast<int64_t>(cluster) * kSliceBytes) ||
-          (2 * rows * cluster <= 4 * sm_count(dev) && bytes >= cluster * int64_t(32768))))
+          (2 * rows * cluster <= 3 * sm_count(dev) && bytes >= cluster * int64_t(32768))))
     cluster *= 2;
   if (rows * cluster >= int64_t(1) << 31) {
     set_error("distill_topk: too many rows for this vocabulary");
@@ -926,23 +939,30 @@ int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
   return launch_check("distill_topk launch", cudaLaunchKernelEx(&cfg, kern, a, cluster, inner));
 }
 
+template <typename T, int G>
+int launch_backward(const DistillTopkArgs& a, int64_t pieces, int piece, cudaStream_t stream) {
+  constexpr int kGroups = kThreads / G;
+  const int64_t grid = (a.outer * a.inner * pieces + kGroups - 1) / kGroups;
+  if (grid * kGroups >= int64_t(1) << 31) {
+    set_error("distill_topk_bwd: too many rows for this vocabulary");
+    return BDH_ERR_INVALID;
+  }
+  distill_topk_bwd_kernel<T, G><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
+      a, FastDiv(static_cast<uint32_t>(pieces)), piece, FastDiv(static_cast<uint32_t>(a.inner)));
+  return launch_check("distill_topk_bwd launch", cudaSuccess);
+}
+
 template <typename T>
 int backward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
-  const int64_t rows = a.outer * a.inner;
-  const FastDiv inner(static_cast<uint32_t>(a.inner));
-  if (a.V <= kShort) {
-    const unsigned grid = static_cast<unsigned>((rows + kWarps - 1) / kWarps);
-    distill_topk_bwd_kernel<T, 32><<<grid, kThreads, 0, stream>>>(a, FastDiv(1), static_cast<int>(a.V), inner);
-  } else {
-    const int64_t pieces = (a.V + kPiece - 1) / kPiece;
-    if (rows * pieces >= int64_t(1) << 31) {
-      set_error("distill_topk_bwd: too many rows for this vocabulary");
-      return BDH_ERR_INVALID;
-    }
-    distill_topk_bwd_kernel<T, kThreads><<<static_cast<unsigned>(rows * pieces), kThreads, 0, stream>>>(
-        a, FastDiv(static_cast<uint32_t>(pieces)), kPiece, inner);
-  }
-  return launch_check("distill_topk_bwd launch", cudaSuccess);
+  const int64_t rows = a.outer * a.inner, bytes = a.V * static_cast<int64_t>(sizeof(T));
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (a.V <= 256) return launch_backward<T, 8>(a, 1, 256, stream);
+  if (a.V <= 512) return launch_backward<T, 16>(a, 1, 512, stream);
+  if (a.V <= kShort) return launch_backward<T, 32>(a, 1, kShort, stream);
+  if (bytes <= kWarpGradBytes && rows >= kWarpRows * sm_count(dev))
+    return launch_backward<T, 32>(a, 1, static_cast<int>(a.V), stream);
+  return launch_backward<T, kThreads>(a, (a.V + kPiece - 1) / kPiece, kPiece, stream);
 }
 
 }  // namespace

@@ -418,11 +418,15 @@ struct RowMap {
     return ex2(t) * (with_log ? fmaf(k1, max_nan(t, kExpFloor), k0) : k0);
   }
 };
+template <int G>
+__device__ __forceinline__ float row_map(const RowMap& map, float x) {
+  return G <= 32 ? map.plain(x) : map.of(x);
+}
 // d = map(x) for n elements of a row by a group of G threads. A warp's rows are short and do not wait
 // for arithmetic: the plain form, in which a single token's probability is exactly 1.
 template <typename T, int G>
 __device__ __forceinline__ void map_row(const T* x, T* d, int n, int tid, bool zero, const RowMap& map) {
-  if (G == 32) {
+  if (G <= 32) {
     map_row<T, G>(x, d, n, tid, zero, [&](float v) { return map.plain(v); });
   } else if (map.wide && !zero) {
 #pragma unroll 1

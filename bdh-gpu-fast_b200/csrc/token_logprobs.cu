@@ -5,12 +5,20 @@
 //   dx_i = 1/temperature [ p_i (g_lse - g_logprob - sum_j g_top_j - g_entropy (ln p_i + entropy))
 //                          + [i = token] g_logprob + sum_j [i = top_j] g_top_j ]
 //
-// The forward reads a row once. A group of threads (a warp for short rows and lists, else a CTA of
-// 256 threads, else a cluster of up to 8 CTAs with a slice of the row each) keeps a softmax state
-// per thread and joins them at the end, through distributed shared memory in a cluster. For the top
-// list it keeps the maximum of every batch of vectors that a thread reads (a cell); the K-th largest
-// of the threads' own maxima bounds the K-th largest logit from below, so that only cells above it
-// are looked at again, a few cache lines, and the few candidates are put in order by counting.
+// The forward reads a row once. A group of threads (8 to 32 lanes for a short row, a warp for many rows
+// of a middling length, else a CTA of 256 threads, or a cluster of up to 8 with a slice of the row each)
+// keeps a softmax state per thread and joins them at the end, through distributed shared memory in a
+// cluster. For the top list it keeps the maximum of every batch of vectors that a thread reads (a cell);
+// the K-th largest of the threads' own maxima bounds the K-th largest logit from below, so that only cells
+// above it are looked at again, a few cache lines, and the few candidates are put in order by counting.
+//
+// What bounds it: without a list, memory, with the exponentials close behind. 4096 rows of 131072 in bf16
+// take 162 us, 6.6 TB/s; the exponential's unit is then busy 76% of the time and 0.67 of the issue slots
+// are used (7.2 instructions an element; run for seconds, at the clocks that the power limit leaves, 173).
+// With a list the issue slots (0.73 used): 2048 rows of 65536 with K = 64 take 66 us, 4.1 TB/s, of which
+// the search after the stream is 13, half of it the second look at the cells above the bound. A single
+// row of 131072 with K = 20 takes 8.7 us, the latencies of some ten steps that wait for one another.
+// The backward reads and writes at 6.2 to 6.6 TB/s: 81 us for 1024 rows of 131072 in bf16.
 #include <algorithm>
 #include <string>
 
@@ -26,12 +34,23 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kWarpTop = 16;     // longest list that a short row bounds by its lanes' maxima
-constexpr int kWarpRow = 8192;   // longest row that a warp reads
-constexpr int kWarpRows = 16;    // rows for every SM from which a warp takes a row
+// Steps that bring this bound close where K > 8: with 24 of 32 lanes' maxima above it 45 of 256 elements
+// are, with 16 of them 22. 16384 rows of 256 with K = 16: 18.9 us, 21 without; with K = 5 16 and 15.5.
+constexpr int kClose = 10;
+// A warp takes a row of up to this size where there are this many rows for every SM: no thread waits for
+// another warp, and the loads of 32 rows are in flight on an SM. 8192 rows in bf16, by warps against by
+// CTAs: 4096 long 13 and 38 us (with K = 20 32 and 70), 16384 long 47 and 64 us (63 and 102), 32768 long
+// 97 and 99 (158 and 140). 592 rows of 8192 and 4096, 4 an SM: 5.4 and 4.9, 4.1 and 4.7 us (K = 20: 11 and
+// 8, 10 and 8).
+constexpr int kWarpRowBytes = 32 * 1024, kWarpRows = 8;
 constexpr int kWarpList = 32;    // longest list of a warp's row (its candidates' room)
 constexpr int kWarpCells = 16;   // vectors per lane up to which each is a cell in a warp's row
 constexpr int kMaxCells = 48;    // cells per thread; longer rows put more batches into a cell
 constexpr int kMaxCluster = 8;
+// A row by itself is split over a cluster in slices of at least 16 KB, but not one of 32 KB or less, which
+// a CTA has read before a cluster has met: one row of 16384 in bf16 3.3 us whole and 3.5 split, of 65536
+// 4.8 whole, 3.7 split, of 131072 8.2 and 4.1.
+constexpr int kUnsplitBytes = 32 * 1024, kSliceBytes = 16 * 1024;
 
 // Threads' maxima that may lie above the bound besides the K wanted: the search for it ends early.
 __host__ __device__ constexpr int top_slack(int K) { return K / 4 + 4; }
@@ -45,14 +64,15 @@ constexpr int candidate_room(int K) {
 // A key that at least K of a group's items are at or above, and as a rule few more, by bisection:
 // first over the values' keys, [lo, hi] holding all of them, then, where more items share the value
 // found than may be taken, over the index up to which they count. from(v): items with value key >= v;
-// tied(v, i): items with value key v and an index up to i.
+// tied(v, i): items with value key v and an index up to i. The first `close` steps are taken even where
+// there are few more than K.
 template <typename From, typename Tied>
-__device__ __forceinline__ uint64_t list_bound(int K, uint32_t lo, uint32_t hi, int V, From from,
-                                               Tied tied) {
+__device__ __forceinline__ uint64_t list_bound(int K, uint32_t lo, uint32_t hi, int V, int close,
+                                               From from, Tied tied) {
   const int most = K + top_slack(K);
   int n = 0x7fffffff;
   ++hi;  // at least K items from lo, fewer than K from hi
-  while (hi - lo > 1 && n > most) {
+  while (hi - lo > 1 && n > (--close >= 0 ? K : most)) {
     const uint32_t mid = lo + (hi - lo) / 2;
     const int now = from(mid);
     if (now >= K) {
@@ -132,7 +152,8 @@ __device__ __forceinline__ void write_figures(const TokenLogprobsArgs& a, int64_
 // ------------------------------------------------------------------ lanes for a short row
 // Rows of at most kShort elements stay in registers: L lanes hold E elements each of a row, and one or
 // two of its unaligned ends; the maximum first, then the sums. With few lanes a row the shuffles and
-// the row's own figures serve several rows at once (a byte model's 256: 4 rows a warp).
+// the row's own figures serve several rows at once (a byte model's 256: 4 rows a warp; 16352 such rows
+// in bf16 take 4.1 us, 7.0 with a warp each). 2 us are the launch; the rest is the row's latencies.
 constexpr int kShort = 1024;
 
 template <typename T, int L, int E>
@@ -244,12 +265,13 @@ __global__ void __launch_bounds__(kThreads) token_list_short_kernel(TokenLogprob
   if (K <= kWarpTop && __popc(__ballot_sync(0xffffffffu, own != 0)) >= K) {
     const uint32_t lo = __reduce_min_sync(0xffffffffu, own != 0 ? own : 0xffffffffu);
     bound = list_bound(
-        K, lo, hi, V, [&](uint32_t v) { return __popc(__ballot_sync(0xffffffffu, own >= v)); },
+        K, lo, hi, V, K > 8 ? kClose : 0, [&](uint32_t v) { return __popc(__ballot_sync(0xffffffffu, own >= v)); },
         [&](uint32_t v, uint32_t at) { return __popc(__ballot_sync(0xffffffffu, own == v && own_at <= at)); });
     by_element = false;
   }
+  uint32_t least = 0, last = 0;  // the bound's value, and of elements with it the last index
   auto above = [&](uint32_t k, int at) {
-    return k != 0 && ((static_cast<uint64_t>(k) << 32) | (0xffffffffu - static_cast<uint32_t>(at))) >= bound;
+    return k > least || (k == least && static_cast<uint32_t>(at) <= last);  // (an empty place's key is 0)
   };
   auto count = [&](auto in) {
     int n = in(edge_key, edge) ? 1 : 0;
@@ -259,28 +281,40 @@ __global__ void __launch_bounds__(kThreads) token_list_short_kernel(TokenLogprob
       for (int e = 0; e < kV; ++e) n += in(keys[u * kV + e], index_of(u, e)) ? 1 : 0;
     return static_cast<int>(__reduce_add_sync(0xffffffffu, n));
   };
-  if (!by_element) by_element = count(above) > kShortRoom;
-  if (by_element) {
+  uint32_t bits = 0;  // this lane's candidates in its vectors
+  bool at_edge = false;
+  int n = kShortRoom + 1;  // the row's candidates
+  auto mark = [&] {
+    least = static_cast<uint32_t>(bound >> 32);
+    last = key_index(bound);
+    bits = 0;
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+      for (int e = 0; e < kV; ++e) bits |= above(keys[u * kV + e], index_of(u, e)) ? 1u << (u * kV + e) : 0u;
+    at_edge = above(edge_key, edge);
+    n = __reduce_add_sync(0xffffffffu, __popc(bits) + (at_edge ? 1 : 0));
+  };
+  if (!by_element) mark();
+  if (n > kShortRoom) {
     bound = list_bound(
-        K, 1u, hi, V, [&](uint32_t v) { return count([&](uint32_t k, int) { return k >= v; }); },
+        K, 1u, hi, V, 0, [&](uint32_t v) { return count([&](uint32_t k, int) { return k >= v; }); },
         [&](uint32_t v, uint32_t at) {
           return count([&](uint32_t k, int j) { return k == v && static_cast<uint32_t>(j) <= at; });
         });
+    mark();
   }
   if (lane == 0) found[warp] = 0;
   __syncwarp();
-  auto offer = [&](uint32_t k, int at) {
-    if (!above(k, at)) return;
-    const int n = atomicAdd(&found[warp], 1);
-    if (n < kShortRoom) cand[n] = (static_cast<uint64_t>(k) << 32) | (0xffffffffu - static_cast<uint32_t>(at));
-  };
-  offer(edge_key, edge);
-#pragma unroll
-  for (int u = 0; u < kVecs; ++u)
-#pragma unroll
-    for (int e = 0; e < kV; ++e) offer(keys[u * kV + e], index_of(u, e));
+  if (bits != 0 || at_edge) {
+    int to = atomicAdd(&found[warp], __popc(bits) + (at_edge ? 1 : 0));
+    if (at_edge) cand[to++] = top_key(r.x[E], edge);
+    for (; bits != 0; bits &= bits - 1) {
+      const int q = __ffs(bits) - 1, at = index_of(q / kV, q % kV);
+      cand[to++] = top_key(logit_at<T>(x, at), at);  // (from L1: registers have no index)
+    }
+  }
   __syncwarp();
-  const int n = found[warp];
   for (int j = lane; j < n; j += 32) {
     const uint64_t mine = cand[j];
     int place = 0;
@@ -330,8 +364,31 @@ __host__ __device__ constexpr size_t group_smem(int K, int cells, int cluster) {
 }
 template <int G>
 __device__ __forceinline__ void group_sync() {
-  if (G == 32) __syncwarp();
+  if (G <= 32) __syncwarp();
   else __syncthreads();
+}
+
+// f(key, its place) for n different keys, by counting those above each: more than a warp's are shared
+// out to two or four threads each while the CTA has them.
+template <int G, typename F>
+__device__ __forceinline__ void rank_by_counting(const uint64_t* keys, int n, int tid, F f) {
+  if (G > 32 && n > 32 && 2 * n <= G) {
+    const int split = 4 * n <= G ? 4 : 2, part = tid & (split - 1), k = tid / split;
+    if ((tid & ~31) / split >= n) return;  // whole warps
+    const uint64_t mine = keys[min(k, n - 1)];
+    int place = 0;
+    for (int q = part; q < n; q += split) place += keys[q] > mine ? 1 : 0;
+    place += __shfl_xor_sync(0xffffffffu, place, 1);
+    if (split > 2) place += __shfl_xor_sync(0xffffffffu, place, 2);
+    if (part == 0 && k < n) f(mine, place);
+    return;
+  }
+  for (int k = tid; k < n; k += G) {
+    const uint64_t mine = keys[k];
+    int place = 0;
+    for (int q = 0; q < n; ++q) place += keys[q] > mine ? 1 : 0;
+    f(mine, place);
+  }
 }
 
 template <int G>
@@ -557,27 +614,31 @@ __global__ void __launch_bounds__(cta_threads<G>, TOP && G > 32 ? 5 : 4) token_l
       }
     group_sync<G>();
     // All threads on the queued cells' vectors, one each, so that their loads are under way together.
+    // What is not below the bound's value (NaN is not) is looked at by its key.
     const int queued = sh.queued;
+    const float least = key_value(lo);
     if (queued <= room)
       for (int n = tid; n < queued * cell_vecs; n += G) {
         const int v = queue[n >> plan.cell_shift] + (n & (cell_vecs - 1)) * G;
         if (v >= v1) continue;
         float part[kV];
         unpack(__ldg(vec + v), part);
+        uint32_t some = 0;
 #pragma unroll
-        for (int e = 0; e < kV; ++e) offer(part[e], span.head + v * kV + e);
+        for (int e = 0; e < kV; ++e) some |= !(part[e] < least) ? 1u << e : 0u;
+        for (; some != 0; some &= some - 1) {
+          const int at = span.head + v * kV + __ffs(some) - 1;
+          offer(logit_at<T>(x, at), at);  // (from L1: registers have no index)
+        }
       }
     uint64_t* list = lists + rank * K;  // this slice's K largest in order
     for (int k = tid; k < K; k += G) list[k] = 0;
     group_sync<G>();
     const int found = queued <= room ? sh.found : room + 1;
     if (found <= room) {
-      for (int n = tid; n < found; n += G) {
-        const uint64_t mine = cand[n];
-        int place = 0;
-        for (int q = 0; q < found; ++q) place += cand[q] > mine ? 1 : 0;
+      rank_by_counting<G>(cand, found, tid, [&](uint64_t mine, int place) {
         if (place < K) list[place] = mine;
-      }
+      });
     } else {
       // More elements above the bound than there is room for: large values that keep to few
       // cells. K rounds of "the largest below the last one" over the slice.
@@ -661,10 +722,15 @@ __global__ void __launch_bounds__(cta_threads<G>, TOP && G > 32 ? 5 : 4) token_l
 }
 
 // The gradient writes as many bytes as it reads and needs nothing of a row but its two statistics, so
-// a row is cut into pieces of kPiece elements for the CTAs (short rows: a warp each). The token and
-// the list get their own terms in the CTA whose piece they lie in: the element is computed again with
-// its term added, so that it is rounded once.
+// a row is cut into pieces of kPiece elements for the CTAs. The token and the list get their own terms in
+// the CTA whose piece they lie in: the element is computed again with its term added, so that it is
+// rounded once. 1024 rows of 131072 in bf16: 82 us, with pieces of 8192 91 and of 32768 85 us (in fp32
+// 163, 158 and 168).
 constexpr int kPiece = 16384;
+// Many rows of up to this size are a warp's each (8192 rows in bf16, by warps against by CTAs: 2048 long
+// 12.5 and 28.7 us, 4096 long 26 and 37, 8192 long 47 and 50; 1184 rows of 8192 9.1 and 8.0), short ones
+// of fewer lanes (16384 rows of 256: 5.1 us by 8 lanes, 8.9 by warps).
+constexpr int kWarpGradBytes = 8 * 1024;
 
 struct GradShared {
   int index[kTopMax + 1];
@@ -710,8 +776,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(TokenLogpr
       sh.index[k] = k == 0 ? tok : static_cast<int>(a.f.top_index[row * K + k - 1]);
       sh.add[k] = k == 0 ? g_tok : a.g_top[row * K + k - 1];
     }
-    if (G == 32) __syncwarp();
-    else __syncthreads();
+    group_sync<G>();
     for (int k = 1; k <= K; ++k) sum -= sh.add[k];
   }
   // p (sum - g_entropy (ln p + entropy)) / temperature
@@ -721,13 +786,11 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(TokenLogpr
   if (none) return;
   if (K == 0) {
     if (tok < from || tok >= from + n) return;
-    if (G == 32) __syncwarp();
-    else __syncthreads();
-    if (tid == 0) logit_put(d, tok, fmaf(g_tok, inv_t, (G == 32 ? dense.plain(logit_at<T>(x, tok)) : dense.of(logit_at<T>(x, tok)))));
+    group_sync<G>();
+    if (tid == 0) logit_put(d, tok, fmaf(g_tok, inv_t, row_map<G>(dense, logit_at<T>(x, tok))));
     return;
   }
-  if (G == 32) __syncwarp();
-  else __syncthreads();
+  group_sync<G>();
   for (int k = tid; k <= K; k += G) {
     const int at = sh.index[k];
     bool mine = at >= from && at < from + n;
@@ -737,7 +800,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(TokenLogpr
         mine = j > k;
         add += sh.add[j];
       }
-    if (mine) logit_put(d, at, fmaf(add, inv_t, (G == 32 ? dense.plain(logit_at<T>(x, at)) : dense.of(logit_at<T>(x, at)))));
+    if (mine) logit_put(d, at, fmaf(add, inv_t, row_map<G>(dense, logit_at<T>(x, at))));
   }
 }
 
@@ -807,41 +870,47 @@ int launch_short(const TokenLogprobsArgs& a, const FastDiv& inner, cudaStream_t 
 
 template <typename T>
 int forward_by_size(const TokenLogprobsArgs& a, cudaStream_t stream) {
-  const int64_t rows = a.outer * a.inner, vecs = a.V / kVec<T>;
+  const int64_t rows = a.outer * a.inner, bytes = a.V * static_cast<int64_t>(sizeof(T));
   const FastDiv inner(static_cast<uint32_t>(a.inner));
   if (a.V <= 256) return launch_short<T, 8, 32>(a, inner, stream);
   if (a.V <= 512) return launch_short<T, 16, 32>(a, inner, stream);
   if (a.V <= kShort) return launch_short<T, 32, 32>(a, inner, stream);
   // Many rows of a middling length: a warp each.
-  if (a.V <= kWarpRow && a.K <= kWarpList && rows >= kWarpRows * sm_count_here())
+  if (bytes <= kWarpRowBytes && a.K <= kWarpList && rows >= kWarpRows * sm_count_here())
     return launch_forward<T, 32>(a, 1, stream);
-  // Few rows: split each until there are some CTAs for every SM or a slice is one batch.
+  // Few rows: split each in two while that leaves at most three CTAs for every SM. 296 rows of 131072 in
+  // bf16: 13.4 us whole, 14.2 in two; 200: 13.3 whole, 11.5 in two; 64: 8.6 whole, 6.6 in four, 7.0 in eight.
   int cluster = 1;
-  while (cluster < kMaxCluster && 2 * rows * cluster <= 4 * sm_count_here() &&
-         vecs / (2 * cluster) >= kThreads * kUnroll)
-    cluster *= 2;
+  if (bytes > kUnsplitBytes)
+    while (cluster < kMaxCluster && 2 * rows * cluster <= 3 * sm_count_here() &&
+           bytes >= 2 * cluster * kSliceBytes)
+      cluster *= 2;
   return launch_forward<T, kThreads>(a, cluster, stream);
+}
+
+template <typename T, int G>
+int launch_backward(const TokenLogprobsBwdArgs& a, int64_t pieces, int piece, cudaStream_t stream) {
+  constexpr int kGroups = kThreads / G;
+  const int64_t grid = (a.f.outer * a.f.inner * pieces + kGroups - 1) / kGroups;
+  if (grid * kGroups >= int64_t(1) << 31) {
+    set_error("token_logprobs_bwd: too many rows for this vocabulary");
+    return BDH_ERR_INVALID;
+  }
+  const size_t lists = a.g_top != nullptr && a.f.K > 0 ? kGroups * sizeof(GradShared) : 0;
+  token_logprobs_bwd_kernel<T, G><<<static_cast<unsigned>(grid), kThreads, lists, stream>>>(
+      a, FastDiv(static_cast<uint32_t>(pieces)), piece, FastDiv(static_cast<uint32_t>(a.f.inner)));
+  return launch_check("token_logprobs_bwd launch");
 }
 
 template <typename T>
 int backward_by_size(const TokenLogprobsBwdArgs& a, cudaStream_t stream) {
-  const int64_t rows = a.f.outer * a.f.inner;
-  const size_t lists = a.g_top != nullptr && a.f.K > 0 ? sizeof(GradShared) : 0;
-  const FastDiv inner(static_cast<uint32_t>(a.f.inner));
-  if (a.f.V <= 1024) {
-    const unsigned grid = static_cast<unsigned>((rows + kWarps - 1) / kWarps);
-    token_logprobs_bwd_kernel<T, 32><<<grid, kThreads, kWarps * lists, stream>>>(
-        a, FastDiv(1), static_cast<int>(a.f.V), inner);
-  } else {
-    const int64_t pieces = (a.f.V + kPiece - 1) / kPiece;
-    if (rows * pieces >= int64_t(1) << 31) {
-      set_error("token_logprobs_bwd: too many rows for this vocabulary");
-      return BDH_ERR_INVALID;
-    }
-    token_logprobs_bwd_kernel<T, kThreads><<<static_cast<unsigned>(rows * pieces), kThreads, lists, stream>>>(
-        a, FastDiv(static_cast<uint32_t>(pieces)), kPiece, inner);
-  }
-  return launch_check("token_logprobs_bwd launch");
+  const int64_t rows = a.f.outer * a.f.inner, V = a.f.V, bytes = V * static_cast<int64_t>(sizeof(T));
+  if (V <= 256) return launch_backward<T, 8>(a, 1, 256, stream);
+  if (V <= 512) return launch_backward<T, 16>(a, 1, 512, stream);
+  if (V <= kShort) return launch_backward<T, 32>(a, 1, kShort, stream);
+  if (bytes <= kWarpGradBytes && rows >= kWarpRows * sm_count_here())
+    return launch_backward<T, 32>(a, 1, static_cast<int>(V), stream);
+  return launch_backward<T, kThreads>(a, (V + kPiece - 1) / kPiece, kPiece, stream);
 }
 
 }  // namespace

@@ -148,7 +148,7 @@ def distill_topk_loss(logits: torch.Tensor, teacher_index: torch.Tensor,
     other token" one more class, with the probability the list leaves over. An index below 0 is an
     empty slot, one past the vocabulary makes the position NaN, the masses of a repeated one add.
     ``weight``: a tensor of the leading shape or with no dimension; a position of weight 0 gives
-    exactly 0 and its logits are not read. Multiply by temperature ** 2 in the weight where that
+    exactly 0, whatever it holds. Multiply by temperature ** 2 in the weight where that
     convention is wanted. Differentiable with respect to the logits.
     """
     _constant_teacher(teacher_logprob, weight)

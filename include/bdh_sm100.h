@@ -382,7 +382,9 @@ int bdh_decoder_f32(const float* x, int64_t ldx, const float* w, int64_t ldw, fl
  * loss and its sampling with torch: bdh.py:680-728, :1066-1072). Rows are (outer, inner) pairs of
  * V logits with unit stride over V and any {outer, inner} strides in elements (a shifted view
  * [:, :-1] is read in place); statistics are fp32 whatever the logits' dtype (f32 or bf16). Rows
- * start at any element: nothing needs to be aligned beyond the element size.
+ * start at any element: nothing needs to be aligned beyond the element size. Outputs do not overlap
+ * inputs: a row is read again where its gradient is written. No scratch, no atomics on global memory;
+ * the same inputs give the same bits.
  *
  * bdh_token_logprobs: with z = x / temperature and lse = ln sum_i exp(z_i), per row
  *   logprob = z[token] - lse (0 for token == ignore_index, NaN for any other token outside
@@ -423,13 +425,14 @@ int bdh_token_logprobs_bwd(const void* logits, int dtype, const int64_t l_stride
  *   loss = w [ sum_j q_j (ln q_j - ln p[index_j]) + r (ln r - ln s) ]
  *   dx_i = w/temperature [ p_i (sum_j q_j + r) - r p_i / s [i unlisted] - sum_j q_j [i = index_j] ]
  * index < 0: an empty slot; index >= V: the row's loss and gradient are NaN; a repeated token's
- * masses add. weight null: 1; a row of weight 0 gives exact zeros and its logits are not read.
+ * masses add. weight null: 1; a row of weight 0 gives exact zeros, whatever its logits and list hold.
  * When the list holds every token there is no other class (r = 0). A row with no logit above -inf
  * has loss +inf and gradient 0.
  * bdh_distill_topk writes the loss per row and, with dlogits, the gradient of the sum of the losses
- * in the same call (the logits are read from memory once); stats (8 floats per row, 16-byte aligned, may be null) is
- * what bdh_distill_topk_bwd reads, which multiplies the gradient of each row by g_loss. A bit per
- * token is held in the shared memory of up to 8 CTAs, so V is at most BDH_DISTILL_VOCAB_MAX.
+ * in the same call (a second look at a row is served by the caches as far as they reach); stats (8
+ * floats per row, 16-byte aligned, may be null) is what bdh_distill_topk_bwd reads, which multiplies the
+ * gradient of each row by g_loss. A bit per token is held in the shared memory of up to 8 CTAs, so V is
+ * at most BDH_DISTILL_VOCAB_MAX.
  */
 #define BDH_DISTILL_VOCAB_MAX 2097152
 int bdh_distill_topk(const void* logits, int dtype, const int64_t l_strides[2],

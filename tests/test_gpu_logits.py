@@ -612,3 +612,57 @@ def test_lists_and_tokens_made_in_inference_mode(binding, monkeypatch):
     ref = L.distill_grad(zc, top.top_index.cpu(), top.top_logprob.cpu(), w.cpu(), 1.0, True)
     ref = ref + L.token_logprobs_grad(zc, tok.cpu(), g_logprob=torch.ones(4))
     check_grad(d, ref, 2 * w.cpu() + 1, 500, torch.float32)
+
+
+# ------------------------------------------------------ many rows, which warps take one each
+def many_rows():
+    return 8 * torch.cuda.get_device_properties(0).multi_processor_count + 5
+
+
+@pytest.mark.parametrize("dtype,V", [("f32", 1025), ("f32", 3001), ("f32", 8190), ("bf16", 1030), ("bf16", 4096),
+                                     ("bf16", 9001), ("bf16", 16384), ("bf16", 16390)])
+def test_forward_of_many_rows(V, dtype):
+    n = many_rows()
+    x = make((n,), V, DT[dtype], seed=V, offset=V % 4)
+    rows = torch.stack(list(patterns(V, DT[dtype]).values())).to(DT[dtype])
+    x[100:100 + rows.size(0)] = rows.cuda()
+    for k in (0, 1, 9, 32, 40):
+        check_forward(x, tokens((n,), V), k, 0.9)
+
+
+@pytest.mark.parametrize("dtype,V", [("f32", 200), ("f32", 512), ("bf16", 999), ("f32", 1025), ("f32", 2048),
+                                     ("f32", 2049), ("bf16", 1031), ("bf16", 4096), ("bf16", 4099)])
+def test_logprob_gradient_of_many_rows(V, dtype):
+    n, T, k = many_rows(), 1.3, 7
+    x = make((n,), V, DT[dtype], seed=V, offset=V % 5).requires_grad_(True)
+    tok = tokens((n,), V)
+    tok[::50] = -100
+    g = torch.Generator().manual_seed(4)
+    up = {name: torch.randn(n, generator=g) for name in ("logprob", "entropy")}
+    up_top = torch.randn(n, k, generator=g)
+    xc = x.detach().float().cpu()
+    for with_list in (False, True):
+        r = kernels.token_logprobs(x, tok.cuda(), top_k=k if with_list else 0, temperature=T)
+        outs, ups = [r.logprob, r.entropy], [up["logprob"], up["entropy"]]
+        more = {}
+        if with_list:
+            outs.append(r.top_logprob)
+            ups.append(up_top)
+            more = {"g_top": up_top, "top_index": L.order(xc, k)}
+        (d,) = torch.autograd.grad(outs, x, [u.cuda() for u in ups])
+        ref = L.token_logprobs_grad(xc, tok, T, g_logprob=up["logprob"], g_entropy=up["entropy"], **more)
+        size = sum(u.abs() if u.dim() == 1 else u.abs().sum(-1) for u in ups) / T
+        check_grad(d, ref, size, V, x.dtype)
+
+
+@pytest.mark.parametrize("dtype,V,k", [("f32", 200, 16), ("bf16", 512, 20), ("f32", 1025, 24), ("bf16", 1031, 100),
+                                       ("bf16", 4096, 64), ("f32", 6144, 30), ("f32", 6149, 30), ("bf16", 9001, 24)])
+def test_distill_of_many_rows(V, k, dtype):
+    n = many_rows()
+    x = make((n,), V, DT[dtype], seed=V, offset=V % 4)
+    index, lp = lists((n,), V, k)
+    index[7::20, 1] = index[7::20, 0]  # a token twice
+    w = torch.rand(n, generator=torch.Generator().manual_seed(2)) + 0.1
+    w[::30] = 0.0
+    check_distill(x, index, lp, None, 2.0, False)
+    check_distill(x, index, lp, w, 0.8, True)
