@@ -52,9 +52,11 @@ constexpr int kPiece = 16384, kWarpGradBytes = 8 * 1024;
 // shared memory); of 592 rows of 8192 11.9 and 8.7 us.
 constexpr int kWarpRowBytes = 24 * 1024, kWarpRows = 8, kWarpsHeld = 4;
 // With a gradient, a row longer than this is split over a cluster: the slices of some 600 CTAs in flight
-// are read again from L2, with policies that keep them there until then. 2048 rows of 131072 in bf16: 128 KB slices 213 us, 64 KB 228 us (two CTAs more
-// to wait for), whole rows of 256 KB 249 us (they no longer fit L2). Without the L2 policies 232, 224 and
-// 255 us: the DRAM reads of 128 KB slices are then 0.98 GB, of 64 KB slices 0.54 GB.
+// are read again from L2, with policies that keep them there until then. 2048 rows of 131072 in bf16:
+// 128 KB slices 213 us, 64 KB 228 us (two CTAs more to wait for), whole rows of 256 KB 249 us (they no
+// longer fit L2). Without the L2 policies 232, 224 and 255 us: the DRAM reads of 128 KB slices are then
+// 0.98 GB, of 64 KB slices 0.54 GB. Few rows are split further, to three CTAs for every SM and 16 KB (one
+// row of 131072 with its gradient: 20 us whole, 7.0 in eight; 128 rows 22 whole, 18 in two).
 constexpr int kSliceBytes = 136 * 1024;
 
 constexpr int kStats = 8;  // floats per row: see RowStats
@@ -625,8 +627,10 @@ __device__ __forceinline__ void write_slice(uint4 (&next)[kUnroll], const uint4*
                                             int tid, uint64_t drop, const RowMap& f) {
   constexpr int kV = kVec<T>;
   const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
-  stream_early<T, G>(next, vec, v0, v1, tid, drop, [&](const uint4 (&wv)[kUnroll], int b, auto fill, auto refill) {
+  stream_early<T, G>(next, vec, v0, v1, tid, drop, [&](const uint4 (&wv)[kUnroll], int b, auto fill,
+                                                       auto refill) {
     constexpr bool kWhole = !std::is_same<decltype(fill), int>::value;
+    T* to = out + static_cast<int64_t>(b + tid) * kV;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int v = b + u * G + tid;
@@ -637,10 +641,10 @@ __device__ __forceinline__ void write_slice(uint4 (&next)[kUnroll], const uint4*
 #pragma unroll
       for (int e = 0; e < kV; ++e) ds[e] = ex2(fmaf(xs[e], f.c, -f.b)) * f.k0;
       if (aligned) {
-        st_global_v4_hint(out + static_cast<int64_t>(v) * kV, pack(ds), drop);
+        st_global_v4_hint(to + u * G * kV, pack(ds), drop);
       } else {
 #pragma unroll
-        for (int e = 0; e < kV; ++e) logit_put(out, static_cast<int64_t>(v) * kV + e, ds[e]);
+        for (int e = 0; e < kV; ++e) logit_put(to, u * G * kV + e, ds[e]);
       }
     }
   });
@@ -648,7 +652,8 @@ __device__ __forceinline__ void write_slice(uint4 (&next)[kUnroll], const uint4*
 
 // kThreads threads stream; one warp more has the list.
 template <typename T>
-__global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTopkArgs a, int C, FastDiv inner) {
+__global__ void __launch_bounds__(kThreads + 32, 4)
+    distill_cta_kernel(DistillTopkArgs a, int C, FastDiv inner) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int kV = kVec<T>, kStep = kThreads * kUnroll;
   CtaShared& sh = *reinterpret_cast<CtaShared*>(smem);
@@ -777,12 +782,14 @@ __global__ void __launch_bounds__(kThreads + 32, 4) distill_cta_kernel(DistillTo
   SoftSums<false> sums;
   const float slack = kBaseSlack / c;
   const uint32_t* my_bits = bits + tid;
-  stream_early<T, kThreads>(next, vec, v0, v1, tid, keep, [&](uint4 (&wv)[kUnroll], int, auto fill, auto refill) {
+  stream_early<T, kThreads>(next, vec, v0, v1, tid, keep, [&](uint4 (&wv)[kUnroll], int, auto fill,
+                                                              auto refill) {
     const uint32_t struck = *my_bits;
     my_bits += kThreads;
     if (struck != 0) {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) strike(wv[u], struck >> 8 * u, T());
+      for (int u = 0; u < kUnroll; ++u)
+        if (struck >> 8 * u & 0xff) strike(wv[u], struck >> 8 * u, T());
     }
     sums.template add<T>(wv, max_of(wv, T()), c, slack, fill, refill);
   });

@@ -15,7 +15,7 @@
 // What bounds it: without a list, memory, with the exponentials close behind. 4096 rows of 131072 in bf16
 // take 162 us, 6.6 TB/s; the exponential's unit is then busy 76% of the time and 0.67 of the issue slots
 // are used (7.2 instructions an element; run for seconds, at the clocks that the power limit leaves, 173).
-// With a list the issue slots (0.73 used): 2048 rows of 65536 with K = 64 take 66 us, 4.1 TB/s, of which
+// With a list the issue slots (0.75 used): 2048 rows of 65536 with K = 64 take 66 us, 4.1 TB/s, of which
 // the search after the stream is 13, half of it the second look at the cells above the bound. A single
 // row of 131072 with K = 20 takes 8.7 us, the latencies of some ten steps that wait for one another.
 // The backward reads and writes at 6.2 to 6.6 TB/s: 81 us for 1024 rows of 131072 in bf16.
@@ -33,18 +33,24 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kWarpTop = 16;     // longest list that a short row bounds by its lanes' maxima
+constexpr int kWarpTop = 16;     // longest list that a warp bounds by its lanes' largest
 // Steps that bring this bound close where K > 8: with 24 of 32 lanes' maxima above it 45 of 256 elements
 // are, with 16 of them 22. 16384 rows of 256 with K = 16: 18.9 us, 21 without; with K = 5 16 and 15.5.
 constexpr int kClose = 10;
 // A warp takes a row of up to this size where there are this many rows for every SM: no thread waits for
 // another warp, and the loads of 32 rows are in flight on an SM. 8192 rows in bf16, by warps against by
-// CTAs: 4096 long 13 and 38 us (with K = 20 32 and 70), 16384 long 47 and 64 us (63 and 102), 32768 long
-// 97 and 99 (158 and 140). 592 rows of 8192 and 4096, 4 an SM: 5.4 and 4.9, 4.1 and 4.7 us (K = 20: 11 and
-// 8, 10 and 8).
+// CTAs: 4096 long 13 and 38 us (with K = 20 26 and 73), 16384 long 47 and 63 us (63 and 103), 32768 long
+// 97 and 99 (158 and 140). 592 rows, 4 an SM: 4096 long 4.1 and 4.7 us (8.6 and 7.8), 8192 long 5.4 and
+// 4.9 (11 and 8).
 constexpr int kWarpRowBytes = 32 * 1024, kWarpRows = 8;
 constexpr int kWarpList = 32;    // longest list of a warp's row (its candidates' room)
-constexpr int kWarpCells = 16;   // vectors per lane up to which each is a cell in a warp's row
+// Cells are batches of vectors, or single vectors in a warp's row whose batches would be fewer than four
+// for every entry of the list. 8192 rows in bf16, by batches and by vectors: 1500 long with K = 4 15.7 and
+// 16.9 us, with K = 32 34 and 25; 1025 long with K = 32 229 (more candidates than there is room for) and
+// 22. In a CTA's longer rows the stream pays more than the search saves: 2048 rows of 65536 66 and 83 us.
+// What a warp's bound is searched among, of a lane: its cells' largest in so many groups. (8192 rows of
+// 2048 with K = 32: 24.5 us, with every cell by itself 28.)
+constexpr int kLaneItems = 4;
 constexpr int kMaxCells = 48;    // cells per thread; longer rows put more batches into a cell
 constexpr int kMaxCluster = 8;
 // A row by itself is split over a cluster in slices of at least 16 KB, but not one of 32 KB or less, which
@@ -162,7 +168,9 @@ struct ShortRow {
   RowSpan span;
   int end[kEnds];  // elements of the row's ends, or -1
   float x[kN];     // the vectors', then the ends'; -inf where there is none
-  __device__ __forceinline__ int index(int u, int e, int lane) const { return span.head + (u * L + lane) * kV + e; }
+  __device__ __forceinline__ int index(int u, int e, int lane) const {
+    return span.head + (u * L + lane) * kV + e;
+  }
   __device__ __forceinline__ bool has(int u, int lane) const { return u * L + lane < span.vecs; }
   __device__ __forceinline__ void place(const T* p, int V, int lane) {
     span = row_span(p, V);
@@ -265,7 +273,8 @@ __global__ void __launch_bounds__(kThreads) token_list_short_kernel(TokenLogprob
   if (K <= kWarpTop && __popc(__ballot_sync(0xffffffffu, own != 0)) >= K) {
     const uint32_t lo = __reduce_min_sync(0xffffffffu, own != 0 ? own : 0xffffffffu);
     bound = list_bound(
-        K, lo, hi, V, K > 8 ? kClose : 0, [&](uint32_t v) { return __popc(__ballot_sync(0xffffffffu, own >= v)); },
+        K, lo, hi, V, K > 8 ? kClose : 0,
+        [&](uint32_t v) { return __popc(__ballot_sync(0xffffffffu, own >= v)); },
         [&](uint32_t v, uint32_t at) { return __popc(__ballot_sync(0xffffffffu, own == v && own_at <= at)); });
     by_element = false;
   }
@@ -337,17 +346,15 @@ struct GroupShared {
   int found, queued, kept;
   float m, ln_s;                // the row's
 };
-// The list's bound is searched among the cells themselves in a warp's row, and among the threads'
-// largest cells in a CTA's.
+// The list's bound is searched among the threads' largest cells; in a warp's row among kLaneItems of a
+// lane, and for a list of up to kWarpTop among the lanes' largest.
 template <int G>
-__host__ __device__ constexpr int bound_items(int cells) {
-  return G == 32 ? (cells + 1) * 32 : G;
-}
+constexpr int bound_items = G == 32 ? 32 * kLaneItems : G;
 // Candidates and queue; the items' indices, which are needed before them, take their place.
 template <typename T, int G>
 __host__ __device__ constexpr size_t candidate_smem(int K, int cells, int cluster) {
   size_t n = static_cast<size_t>(candidate_room<T>(K)) * (sizeof(uint64_t) + sizeof(int));
-  const size_t at = static_cast<size_t>(bound_items<G>(cells)) * sizeof(int);
+  const size_t at = bound_items<G> * sizeof(int);
   const size_t all = static_cast<size_t>(cluster) * K * sizeof(uint64_t);  // what the slices' lists leave
   if (n < at) n = at;
   if (n < all) n = all;
@@ -394,16 +401,19 @@ __device__ __forceinline__ void rank_by_counting(const uint64_t* keys, int n, in
 template <int G>
 constexpr int cta_threads = G == 32 ? kThreads : G;  // groups of a warp share a CTA
 
+// Four CTAs an SM; with a list five, 48 registers a thread: while some search, others read (2048 rows of
+// 65536 with K = 64: 74 us with four, 69 with five).
 template <typename T, int G, bool TOP>
-__global__ void __launch_bounds__(cta_threads<G>, TOP && G > 32 ? 5 : 4) token_logprobs_kernel(TokenLogprobsArgs a,
-                                                                  ForwardPlan plan, FastDiv inner) {
+__global__ void __launch_bounds__(cta_threads<G>, TOP && G > 32 ? 5 : 4)
+    token_logprobs_kernel(TokenLogprobsArgs a, ForwardPlan plan, FastDiv inner) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int kV = kVec<T>, U = kUnroll;
   const int K = static_cast<int>(a.K), V = static_cast<int>(a.V);
   const int C = G == 32 ? 1 : plan.cluster;
   const uint32_t rank = C > 1 ? cta_rank() : 0;
   const int tid = threadIdx.x % G, group = threadIdx.x / G;
-  const uint32_t row32 = G == 32 ? blockIdx.x * (cta_threads<G> / G) + group : blockIdx.x / static_cast<uint32_t>(C);
+  const uint32_t row32 =
+      G == 32 ? blockIdx.x * (cta_threads<G> / G) + group : blockIdx.x / static_cast<uint32_t>(C);
   const int64_t row = row32;
   if (row >= a.outer * a.inner) return;  // whole warps of the warp form
   if (C > 1) cluster_arrive();  // every CTA's shared memory may be written once all have started
@@ -501,16 +511,22 @@ __global__ void __launch_bounds__(cta_threads<G>, TOP && G > 32 ? 5 : 4) token_l
     if (tid == 0) sh.found = sh.queued = sh.kept = 0;
     group_sync<G>();
     join_warps();
-    const uint32_t* keys = G == 32 ? cells : items;
-    constexpr int kItems = G == 32 ? kWarpCells + 1 : G / 32;  // per lane of the searching warp
-    const int n_items = G == 32 ? (cell + 1) * 32 : G, most = K + top_slack(K);
+    constexpr int kItems = G == 32 ? kLaneItems : G / 32;  // per lane of the searching warp
+    const bool few = G == 32 && K <= kWarpTop;
+    const int most = K + top_slack(K);
     // First by value (one warp): at least K items at or above lo, as a rule not many more.
     if (tid < 32) {
       uint32_t mine[kItems], lo = 0xffffffffu, hi = 0;
       int some = 0;
 #pragma unroll
+      for (int n = 0; n < kItems; ++n) mine[n] = G > 32 ? items[n * 32 + tid] : few && n == 0 ? own : 0u;
+      if (G == 32 && !few)
+        for (int q = 0; q <= cell; q += kItems)
+#pragma unroll
+          for (int n = 0; n < kItems; ++n)
+            if (q + n <= cell) mine[n] = max(mine[n], cells[(q + n) * 32 + tid]);
+#pragma unroll
       for (int n = 0; n < kItems; ++n) {
-        mine[n] = n * 32 + tid < n_items ? keys[n * 32 + tid] : 0u;
         if (mine[n] != 0) lo = min(lo, mine[n]);
         hi = max(hi, mine[n]);
         some += mine[n] != 0 ? 1 : 0;
@@ -519,6 +535,7 @@ __global__ void __launch_bounds__(cta_threads<G>, TOP && G > 32 ? 5 : 4) token_l
       hi = __reduce_max_sync(0xffffffffu, hi);
       some = __reduce_add_sync(0xffffffffu, some);
       auto from = [&](uint32_t v) {
+        if (few) return __popc(__ballot_sync(0xffffffffu, mine[0] >= v));
         int n = 0;
 #pragma unroll
         for (int k = 0; k < kItems; ++k) n += mine[k] >= v ? 1 : 0;
@@ -526,9 +543,9 @@ __global__ void __launch_bounds__(cta_threads<G>, TOP && G > 32 ? 5 : 4) token_l
       };
       uint64_t bound = 0;  // fewer than K items: every element is a candidate
       if (some >= K) {
-        int n = some;
+        int n = some, close = few && K > 8 ? kClose : 0;
         ++hi;
-        while (hi - lo > 1 && n > most) {
+        while (hi - lo > 1 && n > (--close >= 0 ? K : most)) {
           const uint32_t mid = lo + (hi - lo) / 2;
           const int now = from(mid);
           if (now >= K) {
@@ -563,18 +580,17 @@ __global__ void __launch_bounds__(cta_threads<G>, TOP && G > 32 ? 5 : 4) token_l
     if (static_cast<uint32_t>(bound) != 0) {
       // Then, where too many items share the value, by the index of its first element in each.
       const int above = static_cast<int>(static_cast<uint32_t>(bound)) - 1;
-      if (G == 32) {
-        for (int q = 0; q <= cell; ++q)
-          item_at[q * 32 + tid] = cells[q * 32 + tid] == lo ? first_at(q) : 0xffffffffu;
-      } else {
+      const int groups = G == 32 && !few ? kLaneItems : 1;
+      for (int n = 0; n < groups; ++n) {
         uint32_t at = 0xffffffffu;
-        if (own == lo)
-          for (int q = 0; q <= cell; ++q)
+        if (own >= lo)
+          for (int q = n; q <= cell; q += groups)
             if (cells[q * G + tid] == lo) at = min(at, first_at(q));
-        item_at[tid] = at;
+        item_at[n * G + tid] = at;
       }
       group_sync<G>();
       if (tid < 32) {
+        const int n_items = groups * G;
         uint32_t left = 0, right = static_cast<uint32_t>(V);
         int n = n_items;
         while (left < right && n > most - above) {
@@ -824,11 +840,11 @@ int launch_forward(const TokenLogprobsArgs& a, int cluster, cudaStream_t stream)
   const int64_t rows = a.outer * a.inner;
   ForwardPlan plan;
   plan.cluster = cluster;
-  // vectors that a thread reads of its slice; a cell for each in a warp's row while they are few
+  // vectors that a thread reads of its slice
   const int64_t mine = std::max<int64_t>(1, ((a.V / kVec<T> + cluster - 1) / cluster + G - 1) / G);
   const int64_t batches = (mine + kUnroll - 1) / kUnroll;
   plan.cell_shift = 0;
-  if (G != 32 || mine > kWarpCells)
+  if (G != 32 || 32 * batches >= 4 * a.K)
     for (plan.cell_shift = 2; (batches * kUnroll) >> plan.cell_shift > kMaxCells;) ++plan.cell_shift;
   static_assert(kUnroll == 4, "a cell is some batches");
   plan.cells = static_cast<int>((mine + (int64_t(1) << plan.cell_shift) - 1) >> plan.cell_shift);

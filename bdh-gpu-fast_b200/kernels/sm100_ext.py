@@ -2,7 +2,8 @@
 of the reference's native module ``bdh_cuda_ext`` (csrc/tril_attn_bind.cpp:25-40:
 ``tril_score_v``, ``tril_decode``, ``has_cuda``), plus ``tril_score_v_bwd``, ``rope_rotate``,
 ``rope_tril_score_v``, ``rope_tril_decode`` and the fused layer's ``latent_encode``,
-``latent_gate_dec``, ``layer_norm`` and ``residual_layer_norm``.
+``latent_gate_dec``, ``layer_norm`` and ``residual_layer_norm``, and the operators on logits
+(``token_logprobs``, ``distill_topk``, their gradients and their autograd forms).
 
 The extension is a C++ module built in-tree next to the library
 (``python bdh-gpu-fast_b200/build_lib.py --ext``; ``__graft_entry__.build()`` does it). It calls
