@@ -15,9 +15,9 @@
 // A row that a warp takes passes through shared memory: the listed tokens are struck out there (-inf),
 // the rest is summed from it and turned into the gradient from it. Repeated tokens are found on the
 // way: every slot writes its number in place of its token's logit and reads it back.
-// A longer row is streamed by a CTA, or by a cluster whose CTAs take a slice each and exchange their
-// sums through distributed shared memory; a bit per element in shared memory says what is listed (and
-// was set twice for a repeated token). For the gradient the slice is streamed again, from L2.
+// A longer row is streamed by a CTA of 128 or 256 threads, or by a cluster whose CTAs take a slice each and
+// exchange their sums through distributed shared memory; a bit per element in shared memory says what is
+// listed (and was set twice for a repeated token). For the gradient the slice is streamed again, from L2.
 // Where a token is repeated its masses are added up by a search (K^2 comparisons, seldom needed).
 // The backward from stored statistics has nothing to sum.
 //
@@ -58,6 +58,12 @@ constexpr int kWarpRowBytes = 24 * 1024, kWarpRows = 8, kWarpsHeld = 4;
 // 0.98 GB, of 64 KB slices 0.54 GB. Few rows are split further, to three CTAs for every SM and 16 KB (one
 // row of 131072 with its gradient: 20 us whole, 7.0 in eight; 128 rows 22 whole, 18 in two).
 constexpr int kSliceBytes = 136 * 1024;
+// Rows of up to this size that are not split are streamed by 128 threads instead of 256: more rows' lists
+// and waits pass at a time, until the slices in flight outgrow L2. 8192 rows in bf16 by 128 and by 256
+// threads: the loss of 16384 long ones 66 and 85 us, of 50021 141 and 160, of 65536 174 and 183 (1184
+// rows 38 and 31); loss and gradient of 16384 long ones 115 and 130, of 20000 136 and 154, of 32768 204 and
+// 205 (1184 rows 40 and 33).
+constexpr int kHalfBytes = 112 * 1024, kHalfGradBytes = 48 * 1024;
 
 constexpr int kStats = 8;  // floats per row: see RowStats
 
@@ -580,10 +586,9 @@ struct CtaShared {
 __host__ __device__ constexpr size_t bits_at(int K) {
   return (sizeof(CtaShared) + list_bytes(K) + 15) & ~size_t(15);
 }
-template <typename T>
+template <typename T, int G>
 __host__ __device__ constexpr int slice_batches(int64_t V, int cluster) {
-  return static_cast<int>(((V / kVec<T> + cluster - 1) / cluster + kThreads * kUnroll - 1) /
-                          (kThreads * kUnroll));
+  return static_cast<int>(((V / kVec<T> + cluster - 1) / cluster + G * kUnroll - 1) / (G * kUnroll));
 }
 static_assert(kUnroll == 4, "a batch's bytes make a word");
 
@@ -650,15 +655,15 @@ __device__ __forceinline__ void write_slice(uint4 (&next)[kUnroll], const uint4*
   });
 }
 
-// kThreads threads stream; one warp more has the list.
-template <typename T>
-__global__ void __launch_bounds__(kThreads + 32, 4)
+// G threads stream; one warp more has the list.
+template <typename T, int G>
+__global__ void __launch_bounds__(G + 32, G == kThreads ? 4 : 7)
     distill_cta_kernel(DistillTopkArgs a, int C, FastDiv inner) {
   extern __shared__ __align__(16) uint8_t smem[];
-  constexpr int kV = kVec<T>, kStep = kThreads * kUnroll;
+  constexpr int kV = kVec<T>, kStep = G * kUnroll;
   CtaShared& sh = *reinterpret_cast<CtaShared*>(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const bool lister = warp == kWarps;
+  const bool lister = warp == G / 32;
   const int V = static_cast<int>(a.V), K = static_cast<int>(a.K);
   const List l = list_at(smem + sizeof(CtaShared), K);
   uint32_t* bits = reinterpret_cast<uint32_t*>(smem + bits_at(K));
@@ -692,10 +697,10 @@ __global__ void __launch_bounds__(kThreads + 32, 4)
   float edge_x = neg_inf();
   int slot_at[kTopMax / 32];  // the lister's slots
   if (!lister) {
-    load_batch<kThreads>(next, vec, v0, v1, tid, keep);
+    load_batch<G>(next, vec, v0, v1, tid, keep);
     edge = tid < head ? from + tid : tid - head < tail ? V - tail + tid - head : -1;
     if (edge >= 0) edge_x = logit_at<T>(x, edge);
-    for (int k = tid; k < slice_batches<T>(V, C) * kThreads; k += kThreads) bits[k] = 0;
+    for (int k = tid; k < slice_batches<T, G>(V, C) * G; k += G) bits[k] = 0;
     if (tid == 0) sh.edge_bits = 0;
   } else {
 #pragma unroll
@@ -711,7 +716,7 @@ __global__ void __launch_bounds__(kThreads + 32, 4)
   }
   if (w == 0.0f) {  // the whole cluster; a batch of the row was on its way
     if (!lister && d != nullptr)
-      map_row<T, kThreads>(x + from, d + from, n, tid, true, Nothing());
+      map_row<T, G>(x + from, d + from, n, tid, true, Nothing());
     if (tid == 0 && rank == 0) a.loss[row] = 0.0f;
     if (C > 1) cluster_wait();
     return;
@@ -731,8 +736,8 @@ __global__ void __launch_bounds__(kThreads + 32, 4)
         before = atomicOr(&sh.edge_bits, bit);
       } else {
         const int in_batch = v % kStep;
-        bit = 1u << (in_batch / kThreads * 8 + e % kV);
-        before = atomicOr(&bits[v / kStep * kThreads + in_batch % kThreads], bit);
+        bit = 1u << (in_batch / G * 8 + e % kV);
+        before = atomicOr(&bits[v / kStep * G + in_batch % G], bit);
       }
       repeated |= (before & bit) != 0;
     }
@@ -759,7 +764,7 @@ __global__ void __launch_bounds__(kThreads + 32, 4)
     repeated = __any_sync(0xffffffffu, lane < C && sh.repeated[lane] != 0);
     if (repeated) list_state(sh.row, l, K, V, lane, c, true);  // in every CTA of the cluster
     SoftState rest = soft_empty();
-    for (int k = lane; k < C * kWarps; k += 32)
+    for (int k = lane; k < C * (G / 32); k += 32)
       rest = soft_merge(rest, {sh.part[k].x, sh.part[k].y, 0.0f}, c);
     rest = soft_join(rest, c);
     __syncwarp();
@@ -782,10 +787,10 @@ __global__ void __launch_bounds__(kThreads + 32, 4)
   SoftSums<false> sums;
   const float slack = kBaseSlack / c;
   const uint32_t* my_bits = bits + tid;
-  stream_early<T, kThreads>(next, vec, v0, v1, tid, keep, [&](uint4 (&wv)[kUnroll], int, auto fill,
+  stream_early<T, G>(next, vec, v0, v1, tid, keep, [&](uint4 (&wv)[kUnroll], int, auto fill,
                                                               auto refill) {
     const uint32_t struck = *my_bits;
-    my_bits += kThreads;
+    my_bits += G;
     if (struck != 0) {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u)
@@ -793,10 +798,10 @@ __global__ void __launch_bounds__(kThreads + 32, 4)
     }
     sums.template add<T>(wv, max_of(wv, T()), c, slack, fill, refill);
   });
-  if (d != nullptr) load_batch<kThreads>(next, vec, v0, v1, tid, drop);  // again, for the gradient
+  if (d != nullptr) load_batch<G>(next, vec, v0, v1, tid, drop);  // again, for the gradient
   SoftState rest = soft_empty();
   if (!sums.wide) rest = sums.state(c);
-  else rest = soft_slowly_struck<T, kThreads>(vec, v0, v1, tid, c, bits);
+  else rest = soft_slowly_struck<T, G>(vec, v0, v1, tid, c, bits);
   if (edge >= 0 && (sh.edge_bits >> tid & 1) == 0) soft_add(rest, edge_x, c);
   {
     const float m = warp_max(rest.m);
@@ -806,7 +811,7 @@ __global__ void __launch_bounds__(kThreads + 32, 4)
   if (C > 1) {  // every warp's state to every CTA of the cluster
     cluster_wait();
     if (lane < C) {
-      const uint32_t to = peer_smem(&sh.part[rank * kWarps + warp], lane);
+      const uint32_t to = peer_smem(&sh.part[rank * (G / 32) + warp], lane);
       peer_store(to, rest.m);
       peer_store(to + 4, rest.s);
     }
@@ -823,9 +828,9 @@ __global__ void __launch_bounds__(kThreads + 32, 4)
   const RowMap f = g.unlisted(c);
   if (edge >= 0) logit_put(d, edge, none ? 0.0f : f.of(edge_x));
   if (f.wide || none) {
-    map_row<T, kThreads>(x + from + head, d + from + head, n - head - tail, tid, none, f);
+    map_row<T, G>(x + from + head, d + from + head, n - head - tail, tid, none, f);
   } else {
-    write_slice<T, kThreads>(next, vec, d + span.head, v0, v1, tid, drop, f);
+    write_slice<T, G>(next, vec, d + span.head, v0, v1, tid, drop, f);
   }
   if (!none) __syncthreads();
 }
@@ -903,6 +908,27 @@ int allow_smem(const void* kern, size_t smem) {
   return e == cudaSuccess ? BDH_OK : launch_check("distill_topk shared memory", e);
 }
 
+template <typename T, int G>
+int launch_cta(const DistillTopkArgs& a, int cluster, const FastDiv& inner, cudaStream_t stream) {
+  const int64_t rows = a.outer * a.inner;
+  const size_t smem =
+      bits_at(static_cast<int>(a.K)) + static_cast<size_t>(slice_batches<T, G>(a.V, cluster)) * G * kUnroll;
+  auto* kern = distill_cta_kernel<T, G>;
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * cluster));
+  cfg.blockDim = dim3(G + 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  return launch_check("distill_topk launch", cudaLaunchKernelEx(&cfg, kern, a, cluster, inner));
+}
+
 template <typename T>
 int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
   const FastDiv inner(static_cast<uint32_t>(a.inner));
@@ -929,21 +955,9 @@ int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
     set_error("distill_topk: too many rows for this vocabulary");
     return BDH_ERR_INVALID;
   }
-  const size_t smem = bits_at(K) + static_cast<size_t>(slice_batches<T>(a.V, cluster)) * kThreads * kUnroll;
-  auto* kern = distill_cta_kernel<T>;
-  if (int rc = allow_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * cluster));
-  cfg.blockDim = dim3(kThreads + 32);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return launch_check("distill_topk launch", cudaLaunchKernelEx(&cfg, kern, a, cluster, inner));
+  if (cluster == 1 && bytes <= (a.dlogits != nullptr ? kHalfGradBytes : kHalfBytes))
+    return launch_cta<T, kThreads / 2>(a, 1, inner, stream);
+  return launch_cta<T, kThreads>(a, cluster, inner, stream);
 }
 
 template <typename T, int G>

@@ -6,8 +6,8 @@
 //                          + [i = token] g_logprob + sum_j [i = top_j] g_top_j ]
 //
 // The forward reads a row once. A group of threads (8 to 32 lanes for a short row, a warp for many rows
-// of a middling length, else a CTA of 256 threads, or a cluster of up to 8 with a slice of the row each)
-// keeps a softmax state per thread and joins them at the end, through distributed shared memory in a
+// of a middling length, else a CTA of 128 or 256 threads, or a cluster of up to 8 with a slice of the row
+// each) keeps a softmax state per thread and joins them at the end, through distributed shared memory in a
 // cluster. For the top list it keeps the maximum of every batch of vectors that a thread reads (a cell);
 // the K-th largest of the threads' own maxima bounds the K-th largest logit from below, so that only cells
 // above it are looked at again, a few cache lines, and the few candidates are put in order by counting.
@@ -43,7 +43,13 @@ constexpr int kClose = 10;
 // 97 and 99 (158 and 140). 592 rows, 4 an SM: 4096 long 4.1 and 4.7 us (8.6 and 7.8), 8192 long 5.4 and
 // 4.9 (11 and 8).
 constexpr int kWarpRowBytes = 32 * 1024, kWarpRows = 8;
-constexpr int kWarpList = 32;    // longest list of a warp's row (its candidates' room)
+constexpr int kWarpList = 32;    // longest list of a warp's or a half CTA's row (what bounds it is few)
+// Rows of up to this size that are not split are read by CTAs of 128 threads: more rows' loads, joins and
+// searches pass at a time. 8192 rows in bf16 by 128 and by 256 threads: 20000 long 60 and 76 us (with
+// K = 20 93 and 123), 50021 long 129 and 141 (168 and 189), 65536 long 167 and 170 (203 and 210); 2048 rows
+// of 100003 74 and 72 us (91 and 86). (By 64 threads 20000 long 59, with K = 32 89 and 96 by 128; 50021
+// long 132, with K = 32 228 and 172.)
+constexpr int kHalfBytes = 112 * 1024;
 // Cells are batches of vectors, or single vectors in a warp's row whose batches would be fewer than four
 // for every entry of the list. 8192 rows in bf16, by batches and by vectors: 1500 long with K = 4 15.7 and
 // 16.9 us, with K = 32 34 and 25; 1025 long with K = 32 229 (more candidates than there is room for) and
@@ -401,10 +407,10 @@ __device__ __forceinline__ void rank_by_counting(const uint64_t* keys, int n, in
 template <int G>
 constexpr int cta_threads = G == 32 ? kThreads : G;  // groups of a warp share a CTA
 
-// Four CTAs an SM; with a list five, 48 registers a thread: while some search, others read (2048 rows of
-// 65536 with K = 64: 74 us with four, 69 with five).
+// Threads of an SM: 1024; with a list 1280, 48 registers each: while some search, others read (2048 rows
+// of 65536 with K = 64: 74 us with 1024, 69 with 1280).
 template <typename T, int G, bool TOP>
-__global__ void __launch_bounds__(cta_threads<G>, TOP && G > 32 ? 5 : 4)
+__global__ void __launch_bounds__(cta_threads<G>, (TOP && G > 32 ? 1280 : 1024) / cta_threads<G>)
     token_logprobs_kernel(TokenLogprobsArgs a, ForwardPlan plan, FastDiv inner) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int kV = kVec<T>, U = kUnroll;
@@ -901,6 +907,8 @@ int forward_by_size(const TokenLogprobsArgs& a, cudaStream_t stream) {
     while (cluster < kMaxCluster && 2 * rows * cluster <= 3 * sm_count_here() &&
            bytes >= 2 * cluster * kSliceBytes)
       cluster *= 2;
+  if (cluster == 1 && bytes <= kHalfBytes && a.K <= kWarpList)
+    return launch_forward<T, kThreads / 2>(a, 1, stream);
   return launch_forward<T, kThreads>(a, cluster, stream);
 }
 

@@ -666,3 +666,22 @@ def test_distill_of_many_rows(V, k, dtype):
     w[::30] = 0.0
     check_distill(x, index, lp, None, 2.0, False)
     check_distill(x, index, lp, w, 0.8, True)
+
+
+@pytest.mark.parametrize("dtype,V", [("f32", 8200), ("f32", 12001), ("f32", 28672), ("bf16", 16400), ("bf16", 40001),
+                                     ("bf16", 57344)])
+def test_rows_of_a_cta_each(V, dtype):
+    """Too many rows to be split over clusters, too long for a warp."""
+    n = 2 * torch.cuda.get_device_properties(0).multi_processor_count + 3
+    x = make((n,), V, DT[dtype], seed=V, offset=V % 4)
+    rows = torch.stack(list(patterns(V, DT[dtype]).values())).to(DT[dtype])
+    x[50:50 + rows.size(0)] = rows.cuda()
+    for k in (0, 1, 12, 32, 33, 128):
+        check_forward(x, tokens((n,), V), k, 1.1)
+    x = make((n,), V, DT[dtype], seed=V + 1, offset=V % 3)
+    index, lp = lists((n,), V, 40)
+    index[7::20, 1] = index[7::20, 0]  # a token twice
+    w = torch.rand(n, generator=torch.Generator().manual_seed(2)) + 0.1
+    w[::30] = 0.0
+    check_distill(x, index, lp, None, 2.0, False)
+    check_distill(x, index, lp, w, 0.8, True)
