@@ -17,7 +17,7 @@
 // are used (7.2 instructions an element; run for seconds, at the clocks that the power limit leaves, 173).
 // With a list the issue slots (0.75 used): 2048 rows of 65536 with K = 64 take 66 us, 4.1 TB/s, of which
 // the search after the stream is 13, half of it the second look at the cells above the bound. A single
-// row of 131072 with K = 20 takes 8.7 us, the latencies of some ten steps that wait for one another.
+// row of 131072 with K = 20 takes 8.2 us (with K = 128 13), the latencies of some ten steps that wait for one another.
 // The backward reads and writes at 6.2 to 6.6 TB/s: 81 us for 1024 rows of 131072 in bf16.
 #include <algorithm>
 #include <string>
@@ -34,16 +34,20 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kWarpTop = 16;     // longest list that a warp bounds by its lanes' largest
-// Steps that bring this bound close where K > 8: with 24 of 32 lanes' maxima above it 45 of 256 elements
-// are, with 16 of them 22. 16384 rows of 256 with K = 16: 18.9 us, 21 without; with K = 5 16 and 15.5.
-constexpr int kClose = 10;
+// Steps that bring the bound close where the list is more than a quarter of the items that it is searched
+// among: with 24 of 32 lanes' largest above it 45 of 256 elements are, with 16 of them 22. 16384 rows of
+// 256 with K = 16: 18.9 us, 21 without; with K = 5 16 and 15.5. 8192
+// rows of 4096 with K = 128 (of 256 items): 135 us, 156 without.
+__host__ __device__ constexpr int close_steps(int K, int items) { return 4 * K > items ? 10 : 0; }
 // A warp takes a row of up to this size where there are this many rows for every SM: no thread waits for
 // another warp, and the loads of 32 rows are in flight on an SM. 8192 rows in bf16, by warps against by
 // CTAs: 4096 long 13 and 38 us (with K = 20 26 and 73), 16384 long 47 and 63 us (63 and 103), 32768 long
 // 97 and 99 (158 and 140). 592 rows, 4 an SM: 4096 long 4.1 and 4.7 us (8.6 and 7.8), 8192 long 5.4 and
 // 4.9 (11 and 8).
 constexpr int kWarpRowBytes = 32 * 1024, kWarpRows = 8;
-constexpr int kWarpList = 32;    // longest list of a warp's or a half CTA's row (what bounds it is few)
+// Longest list of a warp's or a half CTA's row (half of their items). 8192 rows of 4096 with K = 64: 61 us by
+// warps, 94 by CTAs; with K = 100 by a warp 1550 us, its items no longer bound it.
+constexpr int kWarpList = 64;
 // Rows of up to this size that are not split are read by CTAs of 128 threads: more rows' loads, joins and
 // searches pass at a time. 8192 rows in bf16 by 128 and by 256 threads: 20000 long 60 and 76 us (with
 // K = 20 93 and 123), 50021 long 129 and 141 (168 and 189), 65536 long 167 and 170 (203 and 210); 2048 rows
@@ -279,7 +283,7 @@ __global__ void __launch_bounds__(kThreads) token_list_short_kernel(TokenLogprob
   if (K <= kWarpTop && __popc(__ballot_sync(0xffffffffu, own != 0)) >= K) {
     const uint32_t lo = __reduce_min_sync(0xffffffffu, own != 0 ? own : 0xffffffffu);
     bound = list_bound(
-        K, lo, hi, V, K > 8 ? kClose : 0,
+        K, lo, hi, V, close_steps(K, 32),
         [&](uint32_t v) { return __popc(__ballot_sync(0xffffffffu, own >= v)); },
         [&](uint32_t v, uint32_t at) { return __popc(__ballot_sync(0xffffffffu, own == v && own_at <= at)); });
     by_element = false;
@@ -349,7 +353,7 @@ struct GroupShared {
   SoftState warp_part[kWarps];
   uint64_t best[kWarps];
   uint64_t bound;
-  int found, queued, kept;
+  int found, queued, close, kept;
   float m, ln_s;                // the row's
 };
 // The list's bound is searched among the threads' largest cells; in a warp's row among kLaneItems of a
@@ -379,6 +383,38 @@ template <int G>
 __device__ __forceinline__ void group_sync() {
   if (G <= 32) __syncwarp();
   else __syncthreads();
+}
+
+// The K largest of n > K different keys, none below lo, and at most top_slack(K) more (one warp); how many.
+// Counting places takes n^2 comparisons, so it is worth the steps where there are many: 8192 rows of 1025
+// with K = 128, where nearly every element is a candidate, 220 us, 1270 without.
+__device__ __forceinline__ int keep_largest(const uint64_t* keys, int n, int K, uint64_t lo, uint64_t* out,
+                                            int lane) {
+  uint64_t hi = 0;
+  for (int k = lane; k < n; k += 32) hi = max(hi, keys[k]);
+  hi = warp_max_key(hi) + 1;
+  int above = n;
+  while (hi - lo > 1 && above > K + top_slack(K)) {
+    const uint64_t mid = lo + (hi - lo) / 2;
+    int now = 0;
+    for (int k = lane; k < n; k += 32) now += keys[k] >= mid ? 1 : 0;
+    now = __reduce_add_sync(0xffffffffu, now);
+    if (now >= K) {
+      lo = mid;
+      above = now;
+    } else {
+      hi = mid;
+    }
+  }
+  int kept = 0;
+  for (int from = 0; from < n; from += 32) {
+    const uint64_t mine = from + lane < n ? keys[from + lane] : 0;
+    const bool in = mine >= lo && from + lane < n;
+    const uint32_t who = __ballot_sync(0xffffffffu, in);
+    if (in) out[kept + __popc(who & ((1u << lane) - 1))] = mine;
+    kept += __popc(who);
+  }
+  return kept;
 }
 
 // f(key, its place) for n different keys, by counting those above each: more than a warp's are shared
@@ -549,7 +585,7 @@ __global__ void __launch_bounds__(cta_threads<G>, (TOP && G > 32 ? 1280 : 1024) 
       };
       uint64_t bound = 0;  // fewer than K items: every element is a candidate
       if (some >= K) {
-        int n = some, close = few && K > 8 ? kClose : 0;
+        int n = some, close = close_steps(K, few ? 32 : bound_items<G>);
         ++hi;
         while (hi - lo > 1 && n > (--close >= 0 ? K : most)) {
           const uint32_t mid = lo + (hi - lo) / 2;
@@ -658,7 +694,19 @@ __global__ void __launch_bounds__(cta_threads<G>, (TOP && G > 32 ? 1280 : 1024) 
     group_sync<G>();
     const int found = queued <= room ? sh.found : room + 1;
     if (found <= room) {
-      rank_by_counting<G>(cand, found, tid, [&](uint64_t mine, int place) {
+      int n = found;
+      const uint64_t* keys = cand;
+      if (found > 2 * K + 32) {  // many more than wanted: one warp looks for a bound among them
+        uint64_t* few_keys = reinterpret_cast<uint64_t*>(queue);  // (done with, and room for K + slack)
+        if (tid < 32) {
+          const int kept = keep_largest(cand, found, K, bound, few_keys, tid);
+          if (tid == 0) sh.close = kept;
+        }
+        group_sync<G>();
+        n = sh.close;
+        keys = few_keys;
+      }
+      rank_by_counting<G>(keys, n, tid, [&](uint64_t mine, int place) {
         if (place < K) list[place] = mine;
       });
     } else {
@@ -712,10 +760,16 @@ __global__ void __launch_bounds__(cta_threads<G>, (TOP && G > 32 ? 1280 : 1024) 
     const uint64_t* sorted = lists;
     int n_sorted = K;
     if (C > 1) {
-      // Of the slices' lists, what is not below the largest of their last entries (at least K are
-      // not): few more than K. A slice shorter than K has zeros at its list's end.
-      uint64_t floor = 1;
-      for (int r = 0; r < C; ++r) floor = max(floor, lists[r * K + K - 1]);
+      // Of the slices' lists, what is not below the largest of their last entries nor below the least of
+      // their K/C-th (at least K are not): few more than K (by the last entries alone a row of 131072 with
+      // K = 128 kept some 900 and took 45 us, not 13). A slice shorter than K has zeros at its list's end.
+      const int share = (K + C - 1) / C;
+      uint64_t floor = 1, least = ~0ull;
+      for (int r = 0; r < C; ++r) {
+        floor = max(floor, lists[r * K + K - 1]);
+        least = min(least, lists[r * K + share - 1]);
+      }
+      floor = max(floor, least);
       for (int n = tid; n < C * K; n += G) {
         const uint64_t mine = lists[n];
         if (mine < floor) continue;

@@ -685,3 +685,15 @@ def test_rows_of_a_cta_each(V, dtype):
     w[::30] = 0.0
     check_distill(x, index, lp, None, 2.0, False)
     check_distill(x, index, lp, w, 0.8, True)
+
+
+@pytest.mark.parametrize("dtype,V", [("bf16", 1025), ("f32", 1040), ("bf16", 1600), ("f32", 2500), ("bf16", 6000)])
+def test_long_lists_of_middling_rows(V, dtype):
+    """Lists that hold a good part of what their search can tell apart."""
+    for n in (3, many_rows()):
+        x = make((n,), V, DT[dtype], seed=V, offset=V % 3)
+        if n > 100:
+            rows = torch.stack(list(patterns(V, DT[dtype]).values())).to(DT[dtype])
+            x[50:50 + rows.size(0)] = rows.cuda()
+        for k in (33, 64, 65, 100, 128):
+            check_forward(x, None, k, 1.0)
