@@ -17,8 +17,8 @@
 // are used (7.2 instructions an element; run for seconds, at the clocks that the power limit leaves, 173).
 // With a list the issue slots (0.75 used): 2048 rows of 65536 with K = 64 take 66 us, 4.1 TB/s, of which
 // the search after the stream is 13, half of it the second look at the cells above the bound. A single
-// row of 131072 with K = 20 takes 8.2 us (with K = 128 13), the latencies of some ten steps that wait for one another.
-// The backward reads and writes at 6.2 to 6.6 TB/s: 81 us for 1024 rows of 131072 in bf16.
+// row of 131072 with K = 20 takes 8.2 us (with K = 128 13), the latencies of some ten steps that wait for
+// one another. The backward reads and writes at 6.2 to 6.6 TB/s: 81 us for 1024 rows of 131072 in bf16.
 #include <algorithm>
 #include <string>
 
@@ -36,8 +36,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kWarpTop = 16;     // longest list that a warp bounds by its lanes' largest
 // Steps that bring the bound close where the list is more than a quarter of the items that it is searched
 // among: with 24 of 32 lanes' largest above it 45 of 256 elements are, with 16 of them 22. 16384 rows of
-// 256 with K = 16: 18.9 us, 21 without; with K = 5 16 and 15.5. 8192
-// rows of 4096 with K = 128 (of 256 items): 135 us, 156 without.
+// 256 with K = 16, a warp each: 18.9 us, 21 without; with K = 5 16 and 15.5. 8192 rows of 4096 with K = 128 (of 256
+// items): 135 us, 156 without.
 __host__ __device__ constexpr int close_steps(int K, int items) { return 4 * K > items ? 10 : 0; }
 // A warp takes a row of up to this size where there are this many rows for every SM: no thread waits for
 // another warp, and the loads of 32 rows are in flight on an SM. 8192 rows in bf16, by warps against by
@@ -229,8 +229,9 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_short_kernel(TokenLog
 }
 
 // With a list, a warp for a row: the elements' keys. Lists up to kWarpTop are bounded by the lanes'
-// largest keys, where that leaves no more candidates than there is room for; longer ones by the
-// elements' own.
+// largest keys, where enough lanes have any and that leaves no more candidates than there is room for;
+// longer ones by the elements' own. (16384 rows of 100 with K = 12, which 13 to 16 lanes hold: 22 us by the
+// elements, 31 by the lanes; 200 with K = 16 20 by the lanes.)
 constexpr int kShortRoom = kTopMax + top_slack(kTopMax) + 1;
 
 template <typename T, int E>
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(kThreads) token_list_short_kernel(TokenLogprob
   const uint32_t hi = __reduce_max_sync(0xffffffffu, own);
   uint64_t bound = 0;
   bool by_element = true;
-  if (K <= kWarpTop && __popc(__ballot_sync(0xffffffffu, own != 0)) >= K) {
+  if (K <= kWarpTop && 2 * __popc(__ballot_sync(0xffffffffu, own != 0)) >= 3 * K) {
     const uint32_t lo = __reduce_min_sync(0xffffffffu, own != 0 ? own : 0xffffffffu);
     bound = list_bound(
         K, lo, hi, V, close_steps(K, 32),
@@ -339,6 +340,197 @@ __global__ void __launch_bounds__(kThreads) token_list_short_kernel(TokenLogprob
     int place = 0;
     for (int q = 0; q < n; ++q) place += cand[q] > mine ? 1 : 0;
     if (place < K) {
+      a.top_index[row * K + place] = key_index(mine);
+      a.top_logprob[row * K + place] =
+          logprob_of(key_value(static_cast<uint32_t>(mine >> 32)), st, ln_s, inv_t);
+    }
+  }
+}
+
+// Over each L neighbouring lanes (all lanes take part).
+template <int L, typename F>
+__device__ __forceinline__ uint32_t lanes_reduce(uint32_t v, F f) {
+#pragma unroll
+  for (int d = L / 2; d > 0; d >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+template <int L>
+__device__ __forceinline__ int lanes_sum(int v) {
+  return static_cast<int>(lanes_reduce<L>(static_cast<uint32_t>(v), [](uint32_t x, uint32_t y) { return x + y; }));
+}
+
+// The lanes' values below this one.
+template <int L>
+__device__ __forceinline__ int lanes_before(int v, int lane) {
+  int to = v;
+#pragma unroll
+  for (int d = 1; d < L; d *= 2) {
+    const int before = __shfl_up_sync(0xffffffffu, to, d, L);
+    if (lane >= d) to += before;
+  }
+  return to - v;
+}
+
+// Many short rows with a short list: L lanes a row, as without a list. The bound is searched among the
+// largest of every four of a lane's elements, for the warp's rows in step; what is not below it goes to
+// the row's places in shared memory, where counting puts it in order. Bound by the issue slots. 16384 rows
+// of 256 in bf16: K = 1 10.8 us, K = 5 11.8, K = 16 16.3; with a warp a row 15.4, 16.0 and 19.1; but 1200
+// rows with K = 5 5.8 against 4.4 (K = 16: 8.1 and 5.1), and where a list is more than a sixteenth of the
+// row, so that the bound lets much of it through, 25 against 22 (16384 rows of 100 with K = 16).
+constexpr int kLanesRoom = 64;
+constexpr int kLanesRows = 32;  // for every SM
+
+template <typename T, int L, int E>
+__global__ void __launch_bounds__(kThreads, 3) token_list_lanes_kernel(TokenLogprobsArgs a, FastDiv inner) {
+  using Row = ShortRow<T, L, E>;
+  constexpr int kV = Row::kV, kVecs = Row::kVecs, kEnds = Row::kEnds, kCells = E / 4;
+  static_assert(E <= 32 && kV % 4 == 0, "a bit for each of a lane's elements; a cell is of one vector");
+  __shared__ uint64_t room[kThreads / L][kLanesRoom];
+  const int lane = threadIdx.x % L;
+  const int rows = static_cast<int>(a.outer * a.inner);
+  int row32 = static_cast<int>(blockIdx.x * (kThreads / L) + threadIdx.x / L);
+  const bool live = row32 < rows;
+  if (!__any_sync(0xffffffffu, live)) return;
+  if (!live) row32 = rows - 1;  // (the warp's other rows need these lanes)
+  int o, i;
+  inner.divmod(row32, o, i);
+  const int64_t row = row32;
+  const int V = static_cast<int>(a.V), K = static_cast<int>(a.K), most = K + top_slack(K);
+  const T* x = static_cast<const T*>(a.logits) + o * a.l_strides[0] + i * a.l_strides[1];
+  Row r;
+  r.place(x, V, lane);
+  Token tok = {false, true, 0.0f};
+  if (lane == 0 && a.tokens != nullptr) tok = load_token(a, x, o, i);
+  r.load(x, lane);
+  const float inv_t = a.inv_t;
+  const SoftState st = soft_of_lanes<true, L>(r.x, a.c);
+  const float ln_s = ln_sum(st);
+  if (lane == 0 && live) write_figures(a, row, st, ln_s, inv_t, tok);
+
+  auto high = [](uint32_t p, uint32_t q) { return max(p, q); };
+  uint32_t cells[kCells + 1], lo = 0xffffffffu, hi = 0;
+  int some = 0;
+  cells[kCells] = 0;
+#pragma unroll
+  for (int e = 0; e < kEnds; ++e)
+    if (r.end[e] >= 0) cells[kCells] = max(cells[kCells], value_key(r.x[E + e]));
+#pragma unroll
+  for (int q = 0; q < kCells; ++q) {
+    const float m = max_nan(max_nan(r.x[4 * q], r.x[4 * q + 1], r.x[4 * q + 2]), r.x[4 * q + 3]);
+    cells[q] = r.has(4 * q / kV, lane) ? value_key(m) : 0u;
+  }
+#pragma unroll
+  for (int q = 0; q <= kCells; ++q) {
+    if (cells[q] != 0) lo = min(lo, cells[q]);
+    hi = max(hi, cells[q]);
+    some += cells[q] != 0 ? 1 : 0;
+  }
+  lo = lanes_reduce<L>(lo, [](uint32_t p, uint32_t q) { return min(p, q); });
+  hi = lanes_reduce<L>(hi, high);
+  some = lanes_sum<L>(some);
+  const uint32_t top = hi++;
+  for (int n = some;;) {
+    const bool go = some >= K && hi - lo > 1 && n > most;
+    if (!__any_sync(0xffffffffu, go)) break;
+    const uint32_t mid = lo + (hi - lo) / 2;
+    int now = 0;
+#pragma unroll
+    for (int q = 0; q <= kCells; ++q) now += cells[q] >= mid ? 1 : 0;
+    now = lanes_sum<L>(now);
+    if (!go) continue;
+    if (now >= K) {
+      lo = mid;
+      n = now;
+    } else {
+      hi = mid;
+    }
+  }
+  if (some < K) lo = 1;  // fewer cells than entries: every element
+
+  uint32_t there = 0;  // this lane's elements
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u)
+    if (r.has(u, lane)) there |= ((1u << kV) - 1) << (u * kV);
+  uint32_t bits = 0, ends = 0;  // the candidates among them; nothing at or above the bound is left out
+  const float least = key_value(lo);
+#pragma unroll
+  for (int e = 0; e < E; ++e) bits |= !(r.x[e] < least) ? 1u << e : 0u;
+  bits &= there;
+#pragma unroll
+  for (int e = 0; e < kEnds; ++e) ends |= r.end[e] >= 0 && !(r.x[E + e] < least) ? 1u << e : 0u;
+  int held = __popc(bits) + __popc(ends), n = lanes_sum<L>(held);
+  uint64_t* cand = room[threadIdx.x / L];
+  const bool wide = n > kLanesRoom;
+  if (__any_sync(0xffffffffu, wide)) {
+    // Equal values, or large ones close together: the bound among the elements themselves, by value and
+    // where needed by index.
+    auto each = [&](auto f) {
+#pragma unroll 1
+      for (int at = lane; at < V; at += L) f(value_key(logit_at<T>(x, at)), at);
+    };
+    auto count = [&](auto in) {
+      int now = 0;
+      each([&](uint32_t k, int at) { now += in(k, at) ? 1 : 0; });
+      return lanes_sum<L>(now);
+    };
+    int from = V, right = V;
+    hi = wide ? top + 1 : hi;
+    for (;;) {
+      const bool go = wide && hi - lo > 1 && from > kLanesRoom;
+      if (!__any_sync(0xffffffffu, go)) break;
+      const uint32_t mid = lo + (hi - lo) / 2;
+      const int now = count([&](uint32_t k, int) { return k >= mid; });
+      if (!go) continue;
+      if (now >= K) {
+        lo = mid;
+        from = now;
+      } else {
+        hi = mid;
+      }
+    }
+    const int above = count([&](uint32_t k, int) { return k > lo; });
+    for (int left = 0, tied = V;;) {
+      const bool go = wide && from > kLanesRoom && left < right && above + tied > kLanesRoom;
+      if (!__any_sync(0xffffffffu, go)) break;
+      const int mid = left + (right - left) / 2;
+      const int now = count([&](uint32_t k, int at) { return k == lo && at <= mid; });
+      if (!go) continue;
+      if (now >= K - above) {
+        right = mid;
+        tied = now;
+      } else {
+        left = mid + 1;
+      }
+    }
+    if (wide) held = 0;
+    const uint64_t bound = (static_cast<uint64_t>(lo) << 32) | (0xffffffffu - static_cast<uint32_t>(right));
+    auto above_it = [&](uint32_t k, int at) {
+      return wide && ((static_cast<uint64_t>(k) << 32) | (0xffffffffu - static_cast<uint32_t>(at))) >= bound;
+    };
+    each([&](uint32_t k, int at) { held += above_it(k, at) ? 1 : 0; });
+    n = lanes_sum<L>(held);
+    int to = lanes_before<L>(held, lane);
+    each([&](uint32_t k, int at) {
+      if (above_it(k, at))
+        cand[to++] = (static_cast<uint64_t>(k) << 32) | (0xffffffffu - static_cast<uint32_t>(at));
+    });
+  }
+  int to = lanes_before<L>(held, lane);
+  if (!wide) {
+#pragma unroll
+    for (int e = 0; e < kEnds; ++e)
+      if (ends >> e & 1) cand[to++] = top_key(logit_at<T>(x, r.end[e]), r.end[e]);
+    for (; bits != 0; bits &= bits - 1) {  // (from L1: registers have no index)
+      const int e = __ffs(bits) - 1, at = r.index(e / kV, e % kV, lane);
+      cand[to++] = top_key(logit_at<T>(x, at), at);
+    }
+  }
+  __syncwarp();
+  for (int j = lane; j < n; j += L) {
+    const uint64_t mine = cand[j];
+    int place = 0;
+    for (int q = 0; q < n; ++q) place += cand[q] > mine ? 1 : 0;
+    if (place < K && live) {
       a.top_index[row * K + place] = key_index(mine);
       a.top_logprob[row * K + place] =
           logprob_of(key_value(static_cast<uint32_t>(mine >> 32)), st, ln_s, inv_t);
@@ -937,10 +1129,12 @@ int launch_forward(const TokenLogprobsArgs& a, int cluster, cudaStream_t stream)
 template <typename T, int L, int E>
 int launch_short(const TokenLogprobsArgs& a, const FastDiv& inner, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
-  const int per = a.K > 0 ? kWarps : kThreads / L;
+  const bool lanes = L < 32 && 16 * a.K <= a.V && a.K <= kWarpTop && rows >= kLanesRows * sm_count_here();
+  const int per = a.K == 0 || lanes ? kThreads / L : kWarps;
   const unsigned grid = static_cast<unsigned>((rows + per - 1) / per);
-  if (a.K > 0) token_list_short_kernel<T, L * E / 32><<<grid, kThreads, 0, stream>>>(a, inner);
-  else token_logprobs_short_kernel<T, L, E><<<grid, kThreads, 0, stream>>>(a, inner);
+  if (a.K == 0) token_logprobs_short_kernel<T, L, E><<<grid, kThreads, 0, stream>>>(a, inner);
+  else if (lanes) token_list_lanes_kernel<T, L < 32 ? L : 16, E><<<grid, kThreads, 0, stream>>>(a, inner);
+  else token_list_short_kernel<T, L * E / 32><<<grid, kThreads, 0, stream>>>(a, inner);
   return launch_check("token_logprobs launch");
 }
 

@@ -697,3 +697,19 @@ def test_long_lists_of_middling_rows(V, dtype):
             x[50:50 + rows.size(0)] = rows.cuda()
         for k in (33, 64, 65, 100, 128):
             check_forward(x, None, k, 1.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [17, 90, 200, 256, 257, 300, 511, 512])
+def test_lists_of_many_short_rows(V, dtype):
+    n = 32 * torch.cuda.get_device_properties(0).multi_processor_count + 3
+    x = make((n,), V, DT[dtype], seed=V, offset=V % 4)
+    rows = torch.stack(list(patterns(V, DT[dtype]).values())).to(DT[dtype])
+    x[1001:1001 + rows.size(0)] = rows.cuda()
+    x[2000:2100] = (x[2000:2100] * 2).round() / 2  # few values
+    x[2200] = -math.inf
+    x[2201, V // 2] = -math.inf
+    for k in (1, min(5, V // 16), V // 16, min(16, V // 16)):
+        check_forward(x, tokens((n,), V), k, 0.7)
+    x = x[:, : V - 1]  # rows at every alignment
+    check_forward(x, None, max(1, min(16, V // 16 - 1)), 1.0)
