@@ -36,8 +36,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kWarpTop = 16;     // longest list that a warp bounds by its lanes' largest
 // Steps that bring the bound close where the list is more than a quarter of the items that it is searched
 // among: with 24 of 32 lanes' largest above it 45 of 256 elements are, with 16 of them 22. 16384 rows of
-// 256 with K = 16, a warp each: 18.9 us, 21 without; with K = 5 16 and 15.5. 8192 rows of 4096 with K = 128 (of 256
-// items): 135 us, 156 without.
+// 256 with K = 16, a warp each: 18.9 us, 21 without; with K = 5 16 and 15.5. 8192 rows of 4096 with
+// K = 128 (of 256 items): 135 us, 156 without.
 __host__ __device__ constexpr int close_steps(int K, int items) { return 4 * K > items ? 10 : 0; }
 // A warp takes a row of up to this size where there are this many rows for every SM: no thread waits for
 // another warp, and the loads of 32 rows are in flight on an SM. 8192 rows in bf16, by warps against by
@@ -356,7 +356,8 @@ __device__ __forceinline__ uint32_t lanes_reduce(uint32_t v, F f) {
 }
 template <int L>
 __device__ __forceinline__ int lanes_sum(int v) {
-  return static_cast<int>(lanes_reduce<L>(static_cast<uint32_t>(v), [](uint32_t x, uint32_t y) { return x + y; }));
+  auto sum = [](uint32_t x, uint32_t y) { return x + y; };
+  return static_cast<int>(lanes_reduce<L>(static_cast<uint32_t>(v), sum));
 }
 
 // The lanes' values below this one.
