@@ -1130,7 +1130,8 @@ int launch_forward(const TokenLogprobsArgs& a, int cluster, cudaStream_t stream)
 template <typename T, int L, int E>
 int launch_short(const TokenLogprobsArgs& a, const FastDiv& inner, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
-  const bool lanes = L < 32 && 16 * a.K <= a.V && a.K <= kWarpTop && rows >= kLanesRows * sm_count_here();
+  const bool lanes = L < 32 && a.K > 0 && a.K <= kWarpTop && 16 * a.K <= a.V &&
+                     rows >= kLanesRows * sm_count_here();
   const int per = a.K == 0 || lanes ? kThreads / L : kWarps;
   const unsigned grid = static_cast<unsigned>((rows + per - 1) / per);
   if (a.K == 0) token_logprobs_short_kernel<T, L, E><<<grid, kThreads, 0, stream>>>(a, inner);

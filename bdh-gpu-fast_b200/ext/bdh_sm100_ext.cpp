@@ -24,6 +24,8 @@
 #include <torch/extension.h>
 
 #include <cstdint>
+#include <cstdlib>
+#include <cstring>
 #include <mutex>
 #include <optional>
 #include <string>
@@ -520,7 +522,7 @@ struct LogitRows {
   at::Tensor t;
   int64_t outer = 1, inner = 1, V = 0;
   int64_t strides[2] = {0, 0};
-  std::vector<int64_t> lead;  // the caller's leading shape
+  at::DimVector lead;  // the caller's leading shape
 
   LogitRows(const at::Tensor& x, const char* what) : t(x) {
     if (x.dim() < 1) TORCH_CHECK_VALUE(false, std::string(what) + ": logits must be (..., V)");
@@ -603,7 +605,7 @@ class Outputs {
   void add(at::Tensor* out, at::IntArrayRef shape, at::ScalarType dtype) {
     int64_t n = 1;
     for (int64_t d : shape) n *= d;
-    parts_.push_back({out, shape.vec(), dtype, bytes_});
+    parts_.push_back({out, at::DimVector(shape), dtype, bytes_});
     bytes_ += (n * static_cast<int64_t>(c10::elementSize(dtype)) + 15) / 16 * 16;
   }
   void make(const c10::Device& device) {
@@ -620,11 +622,11 @@ class Outputs {
  private:
   struct Part {
     at::Tensor* out;
-    std::vector<int64_t> shape;
+    at::DimVector shape;
     at::ScalarType dtype;
     int64_t at;
   };
-  std::vector<Part> parts_;
+  c10::SmallVector<Part, 6> parts_;
   int64_t bytes_ = 0;
 };
 
@@ -634,8 +636,8 @@ void check_temperature(double temperature, const char* what) {
                                  std::to_string(temperature));
 }
 
-std::vector<int64_t> with_entries(const LogitRows& x, int64_t k) {
-  std::vector<int64_t> s = x.lead;
+at::DimVector with_entries(const LogitRows& x, int64_t k) {
+  at::DimVector s = x.lead;
   s.push_back(k);
   return s;
 }
@@ -967,5 +969,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("logits"), py::arg("teacher_index"), py::arg("teacher_logprob"), py::arg("weight"),
         py::arg("temperature"), py::arg("tail"));
   m.def("abi_version", &bdh_abi_version, "ABI version of the loaded libbdh_sm100.so");
+  m.def("in_use", [] {
+    const char* v = std::getenv("BDH_SM100_EXT");
+    return v == nullptr || std::strcmp(v, "0") != 0;
+  }, "False where BDH_SM100_EXT is 0 (os.environ takes ten times as long to say so)");
   m.attr("has_cuda") = true;
 }

@@ -74,6 +74,8 @@ def model_ops() -> ModuleType:
     built and ``BDH_SM100_EXT`` is not ``0``, else the ctypes binding. Both call the same C-ABI
     entries with the same arguments (the same bits); the extension costs less host time per
     call, which is what an eager step of the model spends between its kernels."""
+    if _ext is not None and _ext.in_use():
+        return _ext
     import os
 
     if os.environ.get("BDH_SM100_EXT", "1") != "0":
