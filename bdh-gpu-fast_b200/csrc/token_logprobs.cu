@@ -555,7 +555,7 @@ template <int G>
 constexpr int bound_items = G == 32 ? 32 * kLaneItems : G;
 // Candidates and queue; the items' indices, which are needed before them, take their place.
 template <typename T, int G>
-__host__ __device__ constexpr size_t candidate_smem(int K, int cells, int cluster) {
+__host__ __device__ constexpr size_t candidate_smem(int K, int cluster) {
   size_t n = static_cast<size_t>(candidate_room<T>(K)) * (sizeof(uint64_t) + sizeof(int));
   const size_t at = bound_items<G> * sizeof(int);
   const size_t all = static_cast<size_t>(cluster) * K * sizeof(uint64_t);  // what the slices' lists leave
@@ -568,7 +568,7 @@ template <typename T, int G>
 __host__ __device__ constexpr size_t group_smem(int K, int cells, int cluster) {
   size_t n = kGroupShared;
   if (K > 0)
-    n += candidate_smem<T, G>(K, cells, cluster) + static_cast<size_t>(cluster) * K * sizeof(uint64_t) +
+    n += candidate_smem<T, G>(K, cluster) + static_cast<size_t>(cluster) * K * sizeof(uint64_t) +
          sizeof(int) * (static_cast<size_t>(cells + 1) * G + (G == 32 ? 0 : G));
   return (n + 15) & ~size_t(15);
 }
@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(cta_threads<G>, (TOP && G > 32 ? 1280 : 1024) 
   uint64_t* cand = reinterpret_cast<uint64_t*>(base + kGroupShared);
   int* queue = reinterpret_cast<int*>(cand + candidate_room<T>(K));  // cells to look at again
   uint32_t* item_at = reinterpret_cast<uint32_t*>(cand);  // where a value's first element is
-  uint64_t* lists = reinterpret_cast<uint64_t*>(base + kGroupShared + candidate_smem<T, G>(K, plan.cells, C));
+  uint64_t* lists = reinterpret_cast<uint64_t*>(base + kGroupShared + candidate_smem<T, G>(K, C));
   uint32_t* cells = reinterpret_cast<uint32_t*>(lists + C * K);  // [cell][thread]: largest value key
   uint32_t* items = cells + (plan.cells + 1) * G;                // threads' largest (not for a warp)
 
