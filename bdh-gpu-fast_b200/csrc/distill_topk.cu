@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(32 * kWarpsHeld, 10) distill_warp_kernel(Disti
       const int v = b + u * 32 + lane;
       wv[u] = v < span.vecs ? hvec[v] : void_vec<T>();
     }
-    sums.template add<T>(wv, max_of(wv, T()), c, slack, batch_fill<32>(b, span.vecs, lane), [](int) {});
+    sums.template add<T>(wv, max_of(wv, T()), c, slack, 0u, batch_fill<32>(b, span.vecs, lane), [](int) {});
   }
   SoftState rest = sums.wide ? soft_slowly<T, 32>(hvec, 0, span.vecs, lane, c) : sums.state(c);
   if (edge >= 0) soft_add(rest, logit_at<T>(held, edge), c);
@@ -791,7 +791,7 @@ __global__ void __launch_bounds__(G + 32, G == kThreads ? 4 : 7)
       for (int u = 0; u < kUnroll; ++u)
         if (struck >> 8 * u & 0xff) strike(wv[u], struck >> 8 * u, T());
     }
-    sums.template add<T>(wv, max_of(wv, T()), c, slack, fill, refill);
+    sums.template add<T>(wv, max_of(wv, T()), c, slack, 0u, fill, refill);
   });
   if (d != nullptr) load_batch<G>(next, vec, v0, v1, tid, drop);  // again, for the gradient
   SoftState rest = soft_empty();

@@ -309,6 +309,7 @@ int launch_state_decode(const StateDecodeArgs& a, float* partial, float* qrot, c
 
 // Operators on logits (token_logprobs.cu, distill_topk.cu). Rows are (outer, inner) pairs; strides
 // are in elements, {outer, inner} and, for lists, {outer, inner, entry}.
+constexpr float kWide = 4194304.0f;  // 2^22: exponents below it are taken from a whole-number base (logits.cuh)
 struct TokenLogprobsArgs {
   const void* logits = nullptr;  // (outer, inner, V), unit stride over V
   int dtype = BDH_DTYPE_F32;
@@ -318,6 +319,7 @@ struct TokenLogprobsArgs {
   int64_t ignore_index = -100;
   int64_t outer = 0, inner = 0, V = 0, K = 0;
   float inv_t = 1.0f, c = 1.0f;  // 1 / temperature, and times log2(e)
+  uint32_t least = 0;            // forward: the least logit of an entropy's sum (logits.cuh, at_least)
   // forward outputs, one per row in row order; top_* K per row; any but stats may be null
   float* logprob = nullptr;
   float* lse = nullptr;

@@ -21,6 +21,7 @@
 
 #include "bdh_sm100.h"
 #include "common.cuh"
+#include "internal.h"
 
 namespace bdh {
 
@@ -138,18 +139,20 @@ __device__ __forceinline__ float max_of(const uint4 (&w)[N], uint16_t) {
     m = max_bf16x2(m, max_bf16x2(max_bf16x2(w[u].x, w[u].y), max_bf16x2(w[u].z, w[u].w)));
   return max_nan(bf16x2_lo(m), bf16x2_hi(m));
 }
-// A vector with what is below kLeast raised to it: the least logit of an entropy's sum, whose
-// exponential is 0 (the base is within kWide / c of 0) and times which 0 is 0.
-constexpr float kLeast = -1267650600228229401496703205376.0f;  // -2^100
-__device__ __forceinline__ uint4 at_least(const uint4& w, float) {
-  return make_uint4(__float_as_uint(max_nan(__uint_as_float(w.x), kLeast)),
-                    __float_as_uint(max_nan(__uint_as_float(w.y), kLeast)),
-                    __float_as_uint(max_nan(__uint_as_float(w.z), kLeast)),
-                    __float_as_uint(max_nan(__uint_as_float(w.w), kLeast)));
+// A vector with what is below `least` raised to it. An entropy's sum multiplies an element's exponential by
+// its exponent, so that a masked one must not have an infinite exponent: -2 kWide / c (from the host, in the
+// logits' type, bf16 twice) has an exponential of 0 beside every base, which is above -kWide, and -2 kWide as
+// its exponent, at every temperature.
+__device__ __forceinline__ uint4 at_least(const uint4& w, float, uint32_t least) {
+  const float to = __uint_as_float(least);
+  return make_uint4(__float_as_uint(max_nan(__uint_as_float(w.x), to)),
+                    __float_as_uint(max_nan(__uint_as_float(w.y), to)),
+                    __float_as_uint(max_nan(__uint_as_float(w.z), to)),
+                    __float_as_uint(max_nan(__uint_as_float(w.w), to)));
 }
-__device__ __forceinline__ uint4 at_least(const uint4& w, uint16_t) {
-  constexpr uint32_t kTwo = 0xf180f180u;  // -2^100 twice
-  return make_uint4(max_bf16x2(w.x, kTwo), max_bf16x2(w.y, kTwo), max_bf16x2(w.z, kTwo), max_bf16x2(w.w, kTwo));
+__device__ __forceinline__ uint4 at_least(const uint4& w, uint16_t, uint32_t least) {
+  return make_uint4(max_bf16x2(w.x, least), max_bf16x2(w.y, least), max_bf16x2(w.z, least),
+                    max_bf16x2(w.w, least));
 }
 // A vector of -inf: what a place past the end of a row counts as.
 template <typename T>
@@ -313,7 +316,6 @@ __device__ __forceinline__ void soft_raise(SoftState& st, float m, float c) {
   st.m = m;
 }
 
-constexpr float kWide = 4194304.0f;  // 2^22
 // 2^n for a whole n <= 0.
 __device__ __forceinline__ float pow2(float n) {
   return n < -126.0f ? 0.0f : __int_as_float((static_cast<int>(n) + 127) << 23);
@@ -347,18 +349,18 @@ struct SoftSums {
     m = largest;
     limit = largest + slack;
   }
-  // N vectors whose largest element is `largest`; of a row's last ones, `fill` of them. taken(u): vector
-  // u is out of its register.
+  // N vectors whose largest element is `largest`; of a row's last ones, `fill` of them. `least`: see
+  // at_least. taken(u): vector u is out of its register.
   template <typename T, int N, typename Fill, typename Taken>
-  __device__ __forceinline__ void add(const uint4 (&w)[N], float largest, float c, float slack, Fill fill,
-                                      Taken taken) {
+  __device__ __forceinline__ void add(const uint4 (&w)[N], float largest, float c, float slack, uint32_t least,
+                                      Fill fill, Taken taken) {
     if (!(largest <= limit)) raise(largest, c, slack);  // a NaN too
     const bool sum = !wide && m != neg_inf();
     float ps[2] = {0.0f, 0.0f}, pa[2] = {0.0f, 0.0f};  // (a batch's own sums: fewer terms in a row)
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       float x[kVec<T>];
-      unpack(ENTROPY ? at_least(w[u], T()) : w[u], x);
+      unpack(ENTROPY ? at_least(w[u], T(), least) : w[u], x);
       taken(u);
       if (u > 0 && u >= fill) continue;
 #pragma unroll

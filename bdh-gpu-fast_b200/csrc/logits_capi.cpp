@@ -35,6 +35,15 @@ int check_rows(const char* what, int dtype, int64_t outer, int64_t inner, int64_
   return BDH_OK;
 }
 
+// The bits of -2 kWide / c, cut to bf16 (twice) where the logits are: within the range of both types for
+// every temperature that check_rows lets through.
+uint32_t least_logit(float c, int dtype) {
+  const float least = -2.0f * kWide / c;
+  uint32_t bits;
+  std::memcpy(&bits, &least, sizeof(bits));
+  return dtype == BDH_DTYPE_F32 ? bits : (bits & 0xffff0000u) | bits >> 16;
+}
+
 RowGrad row_grad(const float* p, const int64_t strides[2]) {
   RowGrad g;
   g.p = p;
@@ -71,6 +80,7 @@ int bdh_token_logprobs(const void* logits, int dtype, const int64_t l_strides[2]
   a.ignore_index = ignore_index;
   a.outer = outer; a.inner = inner; a.V = V; a.K = K;
   a.inv_t = 1.0f / temperature; a.c = kLog2eHost * a.inv_t;
+  a.least = least_logit(a.c, dtype);
   a.logprob = logprob; a.lse = lse; a.entropy = entropy; a.stats = stats;
   a.top_logprob = top_logprob; a.top_index = top_index;
   return launch_token_logprobs(a, static_cast<cudaStream_t>(stream));

@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(cta_threads<G>, (TOP && G > 32 ? 1280 : 1024) 
         }
       }
     }
-    sums.template add<T>(w, largest, c, slack, fill, refill);
+    sums.template add<T>(w, largest, c, slack, a.least, fill, refill);
   });
   SoftState st = sums.wide ? soft_slowly<T, G>(vec, v0, v1, tid, c) : sums.state(c);
   if (edge >= 0) soft_add(st, edge_x, c);
