@@ -10,7 +10,8 @@
 // A slot with token < 0 is empty; a repeated token's masses add; a row of weight 0 counts for nothing,
 // whatever it holds.
 // The unlisted tokens are summed by themselves, so that s keeps its digits when the list holds
-// nearly everything.
+// nearly everything. Where the student masks all of them there is no class beside the list as long as r may
+// be the list's rounding.
 //
 // A row that a warp takes passes through shared memory: the listed tokens are struck out there (-inf),
 // the rest is summed from it and turned into the gradient from it. Repeated tokens are found on the
@@ -109,6 +110,17 @@ __device__ __forceinline__ RowGradient row_gradient(const RowStats& st, int tail
   if (g.none) g.m = g.l2 = 0.0f;
   return g;
 }
+// ln of the student's probability outside the list.
+__device__ __forceinline__ float ln_rest_mass(const RowStats& st, float inv_t) {
+  return st.rest_m == neg_inf() ? neg_inf() : (st.rest_m - st.m) * inv_t + st.ln_rest - st.ln_s;
+}
+// A list of all that a teacher allows has a mass of 1 up to its rounding: r is then noise (K 2^-23, or a log
+// softmax's 2^-24 of logits up to 256), which a student that masks everything else (-inf, or so low that no
+// model's logits go there) would pay for with an infinite loss, or one of the mask's size.
+constexpr float kListRounding = 1.0f / 65536.0f, kMaskedMass = -1000.0f;
+__device__ __forceinline__ void settle_rest(RowStats& st, float inv_t) {
+  if (st.r <= kListRounding && ln_rest_mass(st, inv_t) < kMaskedMass) st.r = 0.0f;
+}
 // Loss of a row from its list (L lanes; `slots(f)` calls f(ln q, q, z) for the lane's slots).
 template <int L, typename Slots>
 __device__ __forceinline__ float row_loss(const RowStats& st, float inv_t, Slots slots) {
@@ -119,11 +131,7 @@ __device__ __forceinline__ float row_loss(const RowStats& st, float inv_t, Slots
     if (!(q <= 0.0f)) loss = fmaf(q, lnq - lp, loss);
   });
   loss = warp_sum<L>(loss);
-  if (st.r > 0.0f) {
-    const float ls = st.rest_m == neg_inf() ? neg_inf()
-                                            : (st.rest_m - st.m) * inv_t + st.ln_rest - st.ln_s;
-    loss = fmaf(st.r, logf(st.r) - ls, loss);
-  }
+  if (st.r > 0.0f) loss = fmaf(st.r, logf(st.r) - ln_rest_mass(st, inv_t), loss);
   return st.total != st.total ? quiet_nan() : loss;
 }
 
@@ -308,6 +316,7 @@ __global__ void __launch_bounds__(kThreads) distill_short_kernel(DistillTopkArgs
   st.ln_s = all.m == neg_inf() ? neg_inf() : logf(all.s);
   st.rest_m = rest.m;
   st.ln_rest = rest.m == neg_inf() ? neg_inf() : logf(rest.s);
+  settle_rest(st, inv_t);
   const float loss = row_loss<L>(st, inv_t, [&](auto f) {
 #pragma unroll
     for (int s = 0; s < S; ++s) f(lnq[s], q[s], z[s]);
@@ -433,7 +442,7 @@ __device__ __forceinline__ void list_state(RowShared& sh, const List& l, int K, 
 }
 // The row's statistics from the unlisted tokens' state.
 __device__ __forceinline__ RowStats row_stats(const RowShared& sh, const SoftState& rest, bool repeated,
-                                              float c) {
+                                              float inv_t, float c) {
   const SoftState all = soft_merge(rest, {sh.top.m, sh.top.s, 0.0f}, c);
   RowStats st;
   st.m = all.m;
@@ -444,6 +453,7 @@ __device__ __forceinline__ RowStats row_stats(const RowShared& sh, const SoftSta
   st.r = sh.r;
   st.shift = sh.shift;
   st.repeated = repeated ? 1.0f : 0.0f;
+  settle_rest(st, inv_t);
   return st;
 }
 __device__ __forceinline__ void write_loss(const DistillTopkArgs& a, const RowStats& st, const List& l,
@@ -543,7 +553,7 @@ __global__ void __launch_bounds__(32 * kWarpsHeld, 10) distill_warp_kernel(Disti
   SoftState rest = sums.wide ? soft_slowly<T, 32>(hvec, 0, span.vecs, lane, c) : sums.state(c);
   if (edge >= 0) soft_add(rest, logit_at<T>(held, edge), c);
   rest = soft_join(rest, c);
-  const RowStats st = row_stats(sh, rest, repeated, c);
+  const RowStats st = row_stats(sh, rest, repeated, inv_t, c);
   write_loss(a, st, l, row, w, inv_t, lane);
   if (d == nullptr) return;
 
@@ -763,7 +773,7 @@ __global__ void __launch_bounds__(G + 32, G == kThreads ? 4 : 7)
       rest = soft_merge(rest, {sh.part[k].x, sh.part[k].y, 0.0f}, c);
     rest = soft_join(rest, c);
     __syncwarp();
-    const RowStats st = row_stats(sh.row, rest, repeated, c);
+    const RowStats st = row_stats(sh.row, rest, repeated, inv_t, c);
     const RowGradient g = row_gradient(st, a.tail, inv_t, w);
     if (d != nullptr) {
       if (lane == 0) sh.gradient = g;

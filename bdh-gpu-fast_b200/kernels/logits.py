@@ -145,8 +145,10 @@ def distill_topk_loss(logits: torch.Tensor, teacher_index: torch.Tensor,
     teacher's top tokens and their log probabilities at the temperature of the loss, as
     ``token_logprobs(..., top_k=k)`` gives them. ``tail=False`` renormalises them over the list
     (logits / temperature do as well then); ``tail=True`` takes them as they are and makes "every
-    other token" one more class, with the probability the list leaves over. An index below 0 is an
-    empty slot, one past the vocabulary makes the position NaN, the masses of a repeated one add.
+    other token" one more class, with the probability the list leaves over (up to 2^-16 of it, an
+    fp32 list's rounding, counts as none where the student masks every other token; more costs an
+    infinite loss there). An index below 0 is an empty slot, one past the vocabulary makes the
+    position NaN, the masses of a repeated one add.
     ``weight``: a tensor of the leading shape or with no dimension; a position of weight 0 gives
     exactly 0, whatever it holds. Multiply by temperature ** 2 in the weight where that
     convention is wanted. Differentiable with respect to the logits.

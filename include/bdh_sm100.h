@@ -426,8 +426,9 @@ int bdh_token_logprobs_bwd(const void* logits, int dtype, const int64_t l_stride
  *   dx_i = w/temperature [ p_i (sum_j q_j + r) - r p_i / s [i unlisted] - sum_j q_j [i = index_j] ]
  * index < 0: an empty slot; index >= V: the row's loss and gradient are NaN; a repeated token's
  * masses add. weight null: 1; a row of weight 0 gives exact zeros, whatever its logits and list hold.
- * When the list holds every token there is no other class (r = 0). A row with no logit above -inf
- * has loss +inf and gradient 0.
+ * When the list holds every token there is no other class (r = 0); nor is there one when the student's
+ * probability outside the list is below e^-1000 (a mask) and r is at most 2^-16, which the rounding of an
+ * fp32 list may leave of a whole. A row with no logit above -inf has loss +inf and gradient 0.
  * bdh_distill_topk writes the loss per row and, with dlogits, the gradient of the sum of the losses
  * in the same call (a second look at a row is served by the caches as far as they reach); stats (8
  * floats per row, 16-byte aligned, may be null) is what bdh_distill_topk_bwd reads, which multiplies the

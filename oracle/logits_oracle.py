@@ -92,6 +92,12 @@ def _list(index, teacher, tail, V):
     return t, q, mass[..., :V], listed, r
 
 
+def _settled(r, rest):
+    """A list's remainder that may be its fp32 rounding, where the student's tokens outside the list are
+    masked: there is no other class."""
+    return torch.where((r <= 2.0 ** -16) & (rest < -1000.0), 0.0, r)
+
+
 def distill(x, index, teacher, weight=None, temperature=1.0, tail=False):
     V = x.size(-1)
     logp, lse, none = _softmax(x, temperature)
@@ -99,6 +105,7 @@ def distill(x, index, teacher, weight=None, temperature=1.0, tail=False):
     lp = logp.gather(-1, index.clamp_min(0))
     loss = torch.where(q > 0, q * (torch.where(q > 0, t, 0.0) - lp), 0.0).sum(-1)
     rest = torch.logsumexp(torch.where(listed, NEG, logp), dim=-1)
+    r = _settled(r, rest)
     loss = loss + torch.where(r > 0, r * (torch.log(torch.where(r > 0, r, 1.0)) - rest), 0.0)
     w = torch.ones_like(loss) if weight is None else weight.double().expand(loss.shape)
     return torch.where(w == 0, 0.0, w * loss)
@@ -111,6 +118,7 @@ def distill_grad(x, index, teacher, weight=None, temperature=1.0, tail=False):
     p = torch.exp(logp)
     rest_logp = torch.where(listed, NEG, logp)
     rest = torch.logsumexp(rest_logp, dim=-1, keepdim=True)
+    r = _settled(r, rest.squeeze(-1))
     cond = torch.where(listed | (rest == NEG), 0.0, torch.exp(rest_logp - rest))
     d = p * (q.sum(-1) + r).unsqueeze(-1) - r.unsqueeze(-1) * cond - mass
     w = torch.ones_like(lse) if weight is None else weight.double().expand(lse.shape)

@@ -98,3 +98,62 @@ def test_distillation_at_the_ends_of_the_temperatures(rows, V, T, dtype):
         close(loss.detach(), want, bound)
         (d,) = torch.autograd.grad(loss.sum(), z)
         check_grad(d, dwant, torch.full((rows,), 2 / T), V, DT[dtype])
+
+
+# ---------------------------------------------------------- a list of all that a mask leaves
+def masked_to(index, V, dtype, mask, seed):
+    """Students that allow the listed tokens alone."""
+    x = torch.full((index.size(0), V), mask, dtype=dtype)
+    g = torch.Generator().manual_seed(seed)
+    return x.scatter_(1, index, (torch.randn(index.shape, generator=g) * 2).to(dtype))
+
+
+MASKED = [("f32", -math.inf), ("bf16", -math.inf), ("f32", torch.finfo(torch.float32).min), ("bf16", -1e9),
+          ("f32", -1e4)]
+
+
+@pytest.mark.parametrize("dtype,mask", MASKED)
+@pytest.mark.parametrize("rows,V,k", [(40, 200, 12), (40, 500, 30), (40, 1000, 60), (0, 1100, 12), (40, 5000, 100),
+                                      (300, 20011, 20), (40, 131072, 12)])
+def test_a_list_of_every_allowed_token_has_no_rest(rows, V, k, dtype, mask):
+    """The list's mass is 1 but for its rounding in fp32, and the student has nothing else to give."""
+    rows = rows or many_rows()
+    index, lp = lists((rows,), V, k, seed=V, empty=False, outside=0.0)
+    assert 0 < ((1 - lp.exp().sum(-1)) > 0).sum() < rows  # (rounded to either side)
+    x = masked_to(index, V, DT[dtype], mask, 1)
+    want = L.distill(x.float(), index, lp, None, 1.0, True)
+    p = torch.log_softmax(x.gather(1, index).double(), -1)  # the definition over the allowed tokens alone
+    assert torch.allclose(want, (lp.double().exp() * (lp.double() - p)).sum(-1), rtol=0, atol=2e-5)
+    bound = (2 * rel(V) + 1e-6 * (1 + 2 * 10)) * 1.2
+    dwant = L.distill_grad(x.float(), index, lp, None, 1.0, True)
+    loss, d = kernels.distill_topk_loss_grad(x.cuda(), index.cuda(), lp.cuda(), tail=True)
+    close(loss, want, bound)
+    check_grad(d, dwant, torch.full((rows,), 2.0), V, DT[dtype])
+    z = x.cuda().requires_grad_(True)
+    loss = kernels.distill_topk_loss(z, index.cuda(), lp.cuda(), tail=True)
+    close(loss.detach(), want, bound)
+    (d,) = torch.autograd.grad(loss.sum(), z)
+    check_grad(d, dwant, torch.full((rows,), 2.0), V, DT[dtype])
+    close(kernels.distill_topk_loss(x.cuda(), index.cuda(), lp.cuda(), tail=True), want, bound)
+
+
+@pytest.mark.parametrize("V", [256, 3000, 70001])
+def test_a_constrained_teacher_and_its_student(V):
+    """A teacher's lists as token_logprobs makes them, longer than what the teacher allows (the places after
+    its last token hold log probabilities of -inf): a student equal to it has no loss and no gradient."""
+    x = masked_to(torch.stack([torch.randperm(V)[:9] for _ in range(200)]), V, torch.float32, -math.inf, 2).cuda()
+    for T in (1.0, 1.7):
+        top = kernels.token_logprobs(x, top_k=16, temperature=T)
+        assert (top.top_logprob[:, 9:] == -math.inf).all()
+        loss, d = kernels.distill_topk_loss_grad(x, top.top_index, top.top_logprob, temperature=T, tail=True)
+        assert loss.abs().max().item() < 4 * rel(V) and d.abs().max().item() < 4 * rel(V)
+
+
+@pytest.mark.parametrize("rows,V", [(5, 300), (0, 1100), (5, 30000)])
+def test_a_rest_beyond_rounding_that_the_student_forbids_costs_infinitely(rows, V):
+    rows = rows or many_rows()
+    index, lp = lists((rows,), V, 10, empty=False, outside=1e-4)
+    x = masked_to(index, V, torch.float32, -math.inf, 3)
+    loss, d = kernels.distill_topk_loss_grad(x.cuda(), index.cuda(), lp.cuda(), tail=True)
+    assert (loss == math.inf).all() and torch.isfinite(d).all()
+    check_grad(d, L.distill_grad(x, index, lp, None, 1.0, True), torch.full((rows,), 2.0), V, torch.float32)
