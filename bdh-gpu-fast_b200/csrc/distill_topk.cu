@@ -596,6 +596,12 @@ __host__ __device__ constexpr int slice_batches(int64_t V, int cluster) {
   return static_cast<int>(((V / kVec<T> + cluster - 1) / cluster + G * kUnroll - 1) / (G * kUnroll));
 }
 static_assert(kUnroll == 4, "a batch's bytes make a word");
+template <typename T, int G>
+__host__ __device__ constexpr size_t cta_smem(int K, int64_t V, int cluster) {
+  return bits_at(K) + static_cast<size_t>(slice_batches<T, G>(V, cluster)) * G * kUnroll;
+}
+static_assert(cta_smem<float, kThreads>(kTopMax, BDH_DISTILL_VOCAB_MAX, kMaxCluster) <= 128 * 1024,
+              "the widest row's bits have room in the largest cluster");
 
 // -inf in the places of a vector that the bits name.
 __device__ __forceinline__ void strike(uint4& w, uint32_t bits, float) {
@@ -916,8 +922,7 @@ int allow_smem(const void* kern, size_t smem) {
 template <typename T, int G>
 int launch_cta(const DistillTopkArgs& a, int cluster, const FastDiv& inner, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
-  const size_t smem =
-      bits_at(static_cast<int>(a.K)) + static_cast<size_t>(slice_batches<T, G>(a.V, cluster)) * G * kUnroll;
+  const size_t smem = cta_smem<T, G>(static_cast<int>(a.K), a.V, cluster);
   auto* kern = distill_cta_kernel<T, G>;
   if (int rc = allow_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -955,8 +960,11 @@ int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
     return launch_check("distill_topk launch", cudaSuccess);
   }
   int cluster = 1;
+  // (a loss alone is split for its bits' room from some 900 thousand tokens in fp32 or 1.8 million in bf16)
+  const size_t most = static_cast<size_t>(shared_memory_limit(dev));
   while (cluster < kMaxCluster &&
-         ((a.dlogits != nullptr && bytes > static_cast<int64_t>(cluster) * kSliceBytes) ||
+         (cta_smem<T, kThreads>(K, a.V, cluster) > most ||
+          (a.dlogits != nullptr && bytes > static_cast<int64_t>(cluster) * kSliceBytes) ||
           (2 * rows * cluster <= 3 * sm_count(dev) && bytes >= cluster * int64_t(32768))))
     cluster *= 2;
   if (rows * cluster >= int64_t(1) << 31) {

@@ -44,6 +44,19 @@ int sm_count(int device) {
   return cache[device];
 }
 
+int shared_memory_limit(int device) {
+  constexpr int kB200 = 227 * 1024;
+  static int cache[64] = {0};
+  if (device < 0 || device >= 64) return kB200;
+  if (cache[device] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMaxSharedMemoryPerBlockOptin, device) != cudaSuccess || n <= 0)
+      n = kB200;
+    cache[device] = n;
+  }
+  return cache[device];
+}
+
 bool make_map_4d(CUtensorMap* map, const void* base, int elem_bytes, const int64_t dims[4],
                  const int64_t strides_bytes[3], int box0, int box1, const char* what) {
   const int box[4] = {box0, box1, 1, 1};

@@ -16,6 +16,8 @@ void set_error(const std::string& msg);
 const char* last_error();
 
 int sm_count(int device);
+// The most dynamic shared memory that a CTA may ask for.
+int shared_memory_limit(int device);
 
 // 4-D tiled tensor map over a strided tensor whose innermost dimension is contiguous.
 //   dims    : extents innermost first (d0 is the contiguous one)

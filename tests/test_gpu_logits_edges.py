@@ -157,3 +157,28 @@ def test_a_rest_beyond_rounding_that_the_student_forbids_costs_infinitely(rows, 
     loss, d = kernels.distill_topk_loss_grad(x.cuda(), index.cuda(), lp.cuda(), tail=True)
     assert (loss == math.inf).all() and torch.isfinite(d).all()
     check_grad(d, L.distill_grad(x, index, lp, None, 1.0, True), torch.full((rows,), 2.0), V, torch.float32)
+
+
+# ------------------------------------------------------------------------ wide vocabularies
+@pytest.mark.parametrize("rows,V,dtype", [(230, 1000003, "f32"), (230, 2097152, "f32"), (230, 2097152, "bf16"),
+                                          (230, 1900001, "bf16"), (130, 2097152, "f32"), (3, 2097152, "f32")])
+def test_distillation_over_the_widest_vocabularies(rows, V, dtype):
+    """One row of logits seen many times, each with a list of its own."""
+    x = make((1,), V, DT[dtype], seed=1).expand(rows, V)
+    at = torch.randint(V, (rows, 7), generator=torch.Generator().manual_seed(2))
+    at[0, :3] = torch.tensor([0, V - 1, V // 2])
+    _, lp = lists((rows,), 100, 7, empty=False)
+    loss = kernels.distill_topk_loss(x, at.cuda(), lp.cuda(), tail=True)
+    z = x.detach().requires_grad_(True)
+    loss2 = kernels.distill_topk_loss(z, at.cuda(), lp.cuda(), tail=True)
+    assert torch.equal(loss, loss2.detach())
+    (d,) = torch.autograd.grad(loss2.sum(), z)
+    look = [0, rows // 2, rows - 1]
+    xc = x[look].float().cpu()
+    want, dwant = (f(xc, at[look], lp[look], None, 1.0, True) for f in (L.distill, L.distill_grad))
+    close(loss[look], want, (2 * rel(V) + 1e-6 * (1 + 2 * 20)) * 1.2)
+    check_grad(d[look], dwant, torch.full((3,), 2.0), V, DT[dtype])
+    del d
+    loss3, d = kernels.distill_topk_loss_grad(x, at.cuda(), lp.cuda(), tail=True)
+    close(loss3[look], want, (2 * rel(V) + 1e-6 * (1 + 2 * 20)) * 1.2)
+    check_grad(d[look], dwant, torch.full((3,), 2.0), V, DT[dtype])
