@@ -895,28 +895,19 @@ __global__ void __launch_bounds__(kThreads) distill_topk_bwd_kernel(DistillTopkA
   }
 }
 
-int launch_check(const char* what, cudaError_t e) {
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) {
-    set_error(std::string(what) + ": " + cudaGetErrorString(e));
-    return BDH_ERR_CUDA;
-  }
-  return BDH_OK;
-}
-
 template <typename T, int L, int E, int S>
 int launch_short(const DistillTopkArgs& a, const FastDiv& inner, cudaStream_t stream) {
   constexpr int kRows = kThreads / L;
   const unsigned grid = static_cast<unsigned>((a.outer * a.inner + kRows - 1) / kRows);
   distill_short_kernel<T, L, E, S><<<grid, kThreads, 0, stream>>>(a, inner);
-  return launch_check("distill_topk launch", cudaSuccess);
+  return cuda_status("distill_topk launch");
 }
 
 int allow_smem(const void* kern, size_t smem) {
   if (smem <= 48 * 1024) return BDH_OK;
   const cudaError_t e =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  return e == cudaSuccess ? BDH_OK : launch_check("distill_topk shared memory", e);
+  return e == cudaSuccess ? BDH_OK : cuda_status("distill_topk shared memory", e);
 }
 
 template <typename T, int G>
@@ -936,7 +927,7 @@ int launch_cta(const DistillTopkArgs& a, int cluster, const FastDiv& inner, cuda
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return launch_check("distill_topk launch", cudaLaunchKernelEx(&cfg, kern, a, cluster, inner));
+  return cuda_status("distill_topk launch", cudaLaunchKernelEx(&cfg, kern, a, cluster, inner));
 }
 
 template <typename T>
@@ -957,7 +948,7 @@ int forward_by_size(const DistillTopkArgs& a, cudaStream_t stream) {
     if (int rc = allow_smem(reinterpret_cast<const void*>(distill_warp_kernel<T>), smem)) return rc;
     distill_warp_kernel<T><<<static_cast<unsigned>((rows + kWarpsHeld - 1) / kWarpsHeld), 32 * kWarpsHeld, smem,
                              stream>>>(a, inner);
-    return launch_check("distill_topk launch", cudaSuccess);
+    return cuda_status("distill_topk launch");
   }
   int cluster = 1;
   // (a loss alone is split for its bits' room from some 900 thousand tokens in fp32 or 1.8 million in bf16)
@@ -986,7 +977,7 @@ int launch_backward(const DistillTopkArgs& a, int64_t pieces, int piece, cudaStr
   }
   distill_topk_bwd_kernel<T, G><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
       a, FastDiv(static_cast<uint32_t>(pieces)), piece, FastDiv(static_cast<uint32_t>(a.inner)));
-  return launch_check("distill_topk_bwd launch", cudaSuccess);
+  return cuda_status("distill_topk_bwd launch");
 }
 
 template <typename T>

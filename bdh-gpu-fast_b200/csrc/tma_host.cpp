@@ -1,5 +1,7 @@
 #include "tma_host.h"
 
+#include "bdh_sm100.h"
+
 #include <mutex>
 #include <sstream>
 
@@ -31,6 +33,14 @@ EncodeTiledFn encode_fn() {
 
 void set_error(const std::string& msg) { g_last_error = msg; }
 const char* last_error() { return g_last_error.c_str(); }
+
+int cuda_status(const char* what, cudaError_t e) {
+  const cudaError_t last = cudaGetLastError();
+  if (e == cudaSuccess) e = last;
+  if (e == cudaSuccess) return BDH_OK;
+  set_error(std::string(what) + ": " + cudaGetErrorString(e));
+  return BDH_ERR_CUDA;
+}
 
 int sm_count(int device) {
   static int cache[64] = {0};

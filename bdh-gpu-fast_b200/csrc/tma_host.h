@@ -15,6 +15,11 @@ namespace bdh {
 void set_error(const std::string& msg);
 const char* last_error();
 
+// BDH_OK, or BDH_ERR_CUDA with the message "<what>: <the error>" for the error of a runtime call or (when
+// that had none) of the launches before it. The runtime's own record of it is taken away, so that the next
+// call does not read it as its own.
+int cuda_status(const char* what, cudaError_t e = cudaSuccess);
+
 int sm_count(int device);
 // The most dynamic shared memory that a CTA may ask for.
 int shared_memory_limit(int device);

@@ -1073,15 +1073,6 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(TokenLogpr
   }
 }
 
-int launch_check(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) {
-    set_error(std::string(what) + ": " + cudaGetErrorString(e));
-    return BDH_ERR_CUDA;
-  }
-  return BDH_OK;
-}
-
 int sm_count_here() {
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1107,10 +1098,7 @@ int launch_forward(const TokenLogprobsArgs& a, int cluster, cudaStream_t stream)
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                static_cast<int>(smem));
-    if (e != cudaSuccess) {
-      set_error(std::string("token_logprobs shared memory: ") + cudaGetErrorString(e));
-      return BDH_ERR_CUDA;
-    }
+    if (e != cudaSuccess) return cuda_status("token_logprobs shared memory", e);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(G == 32 ? (rows + kGroups - 1) / kGroups : rows * cluster));
@@ -1123,8 +1111,8 @@ int launch_forward(const TokenLogprobsArgs& a, int cluster, cudaStream_t stream)
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, kern, a, plan, FastDiv(static_cast<uint32_t>(a.inner)));
-  return launch_check("token_logprobs launch");
+  return cuda_status("token_logprobs launch",
+                     cudaLaunchKernelEx(&cfg, kern, a, plan, FastDiv(static_cast<uint32_t>(a.inner))));
 }
 
 template <typename T, int L, int E>
@@ -1137,7 +1125,7 @@ int launch_short(const TokenLogprobsArgs& a, const FastDiv& inner, cudaStream_t 
   if (a.K == 0) token_logprobs_short_kernel<T, L, E><<<grid, kThreads, 0, stream>>>(a, inner);
   else if (lanes) token_list_lanes_kernel<T, L < 32 ? L : 16, E><<<grid, kThreads, 0, stream>>>(a, inner);
   else token_list_short_kernel<T, L * E / 32><<<grid, kThreads, 0, stream>>>(a, inner);
-  return launch_check("token_logprobs launch");
+  return cuda_status("token_logprobs launch");
 }
 
 template <typename T>
@@ -1173,7 +1161,7 @@ int launch_backward(const TokenLogprobsBwdArgs& a, int64_t pieces, int piece, cu
   const size_t lists = a.g_top != nullptr && a.f.K > 0 ? kGroups * sizeof(GradShared) : 0;
   token_logprobs_bwd_kernel<T, G><<<static_cast<unsigned>(grid), kThreads, lists, stream>>>(
       a, FastDiv(static_cast<uint32_t>(pieces)), piece, FastDiv(static_cast<uint32_t>(a.f.inner)));
-  return launch_check("token_logprobs_bwd launch");
+  return cuda_status("token_logprobs_bwd launch");
 }
 
 template <typename T>

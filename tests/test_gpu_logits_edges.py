@@ -182,3 +182,56 @@ def test_distillation_over_the_widest_vocabularies(rows, V, dtype):
     loss3, d = kernels.distill_topk_loss_grad(x, at.cuda(), lp.cuda(), tail=True)
     close(loss3[look], want, (2 * rel(V) + 1e-6 * (1 + 2 * 20)) * 1.2)
     check_grad(d[look], dwant, torch.full((3,), 2.0), V, DT[dtype])
+
+
+# ------------------------------------------------------------------- errors left behind
+def _distill_by_c(x, index, lp, loss, stream):
+    rows, V = x.shape
+    k = index.size(-1)
+    s2, s3 = (ctypes.c_int64 * 2)(0, V), (ctypes.c_int64 * 3)(0, k, 1)
+    return sm100_logits._lib().bdh_distill_topk(
+        x.data_ptr(), 0, s2, index.data_ptr(), s3, lp.data_ptr(), s3, None, s2, loss.data_ptr(), None, None, s2, 1,
+        rows, V, k, 1.0, 0, stream)
+
+
+def _logprobs_by_c(x, lse, stream, stats=None, k=0, top=None, index=None):
+    rows, V = x.shape
+    s2 = (ctypes.c_int64 * 2)(0, V)
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    return sm100_logits._lib().bdh_token_logprobs(
+        x.data_ptr(), 0, s2, None, s2, -100, None, lse.data_ptr(), None, ptr(stats), ptr(top), ptr(index), 1, rows, V,
+        k, 1.0, stream)
+
+
+@pytest.mark.parametrize("rows,V", [(4, 300), (0, 1100), (300, 20011), (2, 70001)])
+def test_a_refused_launch_leaves_the_next_call_alone(rows, V):
+    """The runtime refuses a launch on the legacy stream while a blocking stream records a graph. The call
+    says so, and the next one, which is valid, goes through."""
+    rows = rows or many_rows()
+    x = make((rows,), V, torch.float32)
+    index, lp = (t.cuda() for t in lists((rows,), 40, 5, empty=False))
+    wants = kernels.distill_topk_loss(x, index, lp), kernels.token_logprobs(x).lse
+    out = torch.zeros(rows, device="cuda")
+    side = torch.cuda.Stream()  # (neither blocks the recording nor is blocked by it)
+    rt = ctypes.CDLL("libcudart.so.12")
+    rt.cudaStreamBeginCapture.argtypes = [ctypes.c_void_p, ctypes.c_int]
+    rt.cudaStreamEndCapture.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    rt.cudaStreamDestroy.argtypes = [ctypes.c_void_p]
+    error = sm100_logits._lib().bdh_last_error
+    for call, want in ((lambda s: _distill_by_c(x, index, lp, out, s), wants[0]), (lambda s: _logprobs_by_c(x, out, s), wants[1])):
+        stream, graph = ctypes.c_void_p(), ctypes.c_void_p()
+        assert rt.cudaStreamCreate(ctypes.byref(stream)) == 0
+        torch.cuda.synchronize()
+        assert rt.cudaStreamBeginCapture(stream, 2) == 0  # relaxed: what else this thread does is its own affair
+        try:
+            rc, message = call(None), error()
+        finally:
+            rt.cudaStreamEndCapture(stream, ctypes.byref(graph))  # (invalid by now: no graph)
+            rt.cudaGetLastError()
+            rt.cudaStreamDestroy(stream)
+        assert rc == 2 and b"captur" in message, (rc, message)
+        out.zero_()
+        torch.cuda.synchronize()
+        assert call(side.cuda_stream) == 0, error()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
