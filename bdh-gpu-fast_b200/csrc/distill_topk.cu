@@ -904,10 +904,7 @@ int launch_short(const DistillTopkArgs& a, const FastDiv& inner, cudaStream_t st
 }
 
 int allow_smem(const void* kern, size_t smem) {
-  if (smem <= 48 * 1024) return BDH_OK;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  return e == cudaSuccess ? BDH_OK : cuda_status("distill_topk shared memory", e);
+  return allow_shared_memory("distill_topk shared memory", kern, smem);
 }
 
 template <typename T, int G>

@@ -67,6 +67,15 @@ int shared_memory_limit(int device) {
   return cache[device];
 }
 
+int allow_shared_memory(const char* what, const void* kernel, size_t bytes) {
+  if (bytes <= 48 * 1024) return BDH_OK;  // every kernel may
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_memory_limit(dev));
+  return e == cudaSuccess ? BDH_OK : cuda_status(what, e);
+}
+
 bool make_map_4d(CUtensorMap* map, const void* base, int elem_bytes, const int64_t dims[4],
                  const int64_t strides_bytes[3], int box0, int box1, const char* what) {
   const int box[4] = {box0, box1, 1, 1};

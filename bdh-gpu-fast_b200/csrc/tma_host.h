@@ -23,6 +23,9 @@ int cuda_status(const char* what, cudaError_t e = cudaSuccess);
 int sm_count(int device);
 // The most dynamic shared memory that a CTA may ask for.
 int shared_memory_limit(int device);
+// Lets a kernel of the current device ask for `bytes` of dynamic shared memory. Always up to the device's
+// limit: a limit of this call's own size could be lowered by another thread's before the launch.
+int allow_shared_memory(const char* what, const void* kernel, size_t bytes);
 
 // 4-D tiled tensor map over a strided tensor whose innermost dimension is contiguous.
 //   dims    : extents innermost first (d0 is the contiguous one)

@@ -1095,11 +1095,8 @@ int launch_forward(const TokenLogprobsArgs& a, int cluster, cudaStream_t stream)
   constexpr int kGroups = cta_threads<G> / G;
   const size_t smem = kGroups * group_smem<T, G>(static_cast<int>(a.K), plan.cells, cluster);
   auto* kern = a.K > 0 ? token_logprobs_kernel<T, G, true> : token_logprobs_kernel<T, G, false>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem));
-    if (e != cudaSuccess) return cuda_status("token_logprobs shared memory", e);
-  }
+  if (int rc = allow_shared_memory("token_logprobs shared memory", reinterpret_cast<const void*>(kern), smem))
+    return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(G == 32 ? (rows + kGroups - 1) / kGroups : rows * cluster));
   cfg.blockDim = dim3(cta_threads<G>);

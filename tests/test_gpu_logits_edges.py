@@ -235,3 +235,38 @@ def test_a_refused_launch_leaves_the_next_call_alone(rows, V):
         assert call(side.cuda_stream) == 0, error()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------------- host threads
+@pytest.mark.parametrize("op", ["token_logprobs", "distill_topk"])
+def test_calls_of_several_threads_do_not_limit_one_another(op):
+    """The same kernel with more and with less shared memory, from host threads at once (the C entries: a
+    binding's own time would keep them apart)."""
+    if op == "token_logprobs":
+        x = make((1,), 1500000, torch.float32)
+        tops = {k: (torch.zeros(1, k, device="cuda"), torch.zeros(1, k, dtype=torch.long, device="cuda")) for k in (128, 1)}
+        calls = [(lambda s, k=k, out=torch.zeros(1, device="cuda"): _logprobs_by_c(x, out, s, None, k, *tops[k]))
+                 for k in (128, 1, 128, 1)]
+    else:
+        index, lp = (t.cuda() for t in lists((1,), 1000, 9, empty=False))
+        xs = [make((1,), V, torch.float32) for V in (2097152, 1700000)]
+        calls = [(lambda s, x=x, out=torch.zeros(1, device="cuda"): _distill_by_c(x, index, lp, out, s)) for x in xs + xs]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    failed, gate = [], threading.Barrier(len(calls))
+
+    def work(n):
+        s = streams[n].cuda_stream
+        gate.wait(60)
+        for _ in range(10000):
+            if calls[n](s) != 0:
+                failed.append(sm100_logits._lib().bdh_last_error())
+                return
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(300)
+    torch.cuda.synchronize()
+    assert not failed, failed
