@@ -14,9 +14,10 @@
 // can be captured in CUDA graphs). Differences on purpose: CUDA tensors only (no CPU path: a CPU
 // tensor raises), fp32 and bf16 only, and scratch memory comes from the PyTorch caching
 // allocator (the library itself never allocates).
+#include <ATen/EmptyTensor.h>
 #include <ATen/MemoryOverlap.h>
-#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/stl.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -598,37 +599,32 @@ std::optional<BesideRows> token_rows(const LogitRows& x, const std::optional<at:
   return BesideRows(x, *tokens, at::kLong, -1, "tokens");
 }
 
-// The outputs of one call in one allocation: a small call spends most of its host time on them.
-// Each is a tensor of its own (not a view of another) at a 16-byte boundary of the shared storage.
-class Outputs {
- public:
-  void add(at::Tensor* out, at::IntArrayRef shape, at::ScalarType dtype) {
-    int64_t n = 1;
-    for (int64_t d : shape) n *= d;
-    parts_.push_back({out, at::DimVector(shape), dtype, bytes_});
-    bytes_ += (n * static_cast<int64_t>(c10::elementSize(dtype)) + 15) / 16 * 16;
-  }
-  void make(const c10::Device& device) {
-    const at::Tensor slab = at::detail::empty_cuda({bytes_}, at::kByte, device, std::nullopt);
-    for (const Part& p : parts_) {
-      at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
-          c10::Storage(slab.storage()), slab.key_set(), c10::scalarTypeToTypeMeta(p.dtype));
-      t.unsafeGetTensorImpl()->set_sizes_contiguous(p.shape);
-      t.unsafeGetTensorImpl()->set_storage_offset(p.at / static_cast<int64_t>(c10::elementSize(p.dtype)));
-      *p.out = std::move(t);
-    }
-  }
+// A new tensor on the logits' device from the caching allocator (of the current device and stream), without
+// at::empty's dispatch: a small call spends most of its host time on its outputs.
+at::Tensor fresh(at::IntArrayRef shape, at::ScalarType dtype) {
+  at::globalContext().lazyInitDevice(c10::DeviceType::CUDA);
+  return at::detail::empty_generic(shape, c10::cuda::CUDACachingAllocator::get(),
+                                   c10::DispatchKeySet(c10::DispatchKey::CUDA), dtype, std::nullopt);
+}
 
- private:
-  struct Part {
-    at::Tensor* out;
-    at::DimVector shape;
-    at::ScalarType dtype;
-    int64_t at;
-  };
-  c10::SmallVector<Part, 6> parts_;
-  int64_t bytes_ = 0;
-};
+// The fp32 figures of a call, one a row and of one shape, in one allocation (three would be a tenth of a
+// small call). Each is a tensor of its own (not a view of another) at a 16-byte boundary of the shared
+// storage. Nothing else shares one: lists outlive the figures and are saved, which a storage of two types
+// cannot be.
+void fresh_figures(std::initializer_list<at::Tensor*> figures, at::IntArrayRef shape) {
+  int64_t each = 1;
+  for (int64_t d : shape) each *= d;
+  each = (each + 3) / 4 * 4;
+  const at::Tensor slab = fresh({each * static_cast<int64_t>(figures.size())}, at::kFloat);
+  int64_t at = 0;
+  for (at::Tensor* figure : figures) {
+    *figure = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(slab.storage()), slab.key_set(),
+                                                       slab.dtype());
+    figure->unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+    figure->unsafeGetTensorImpl()->set_storage_offset(at);
+    at += each;
+  }
+}
 
 void check_temperature(double temperature, const char* what) {
   if (!(temperature > 0.0) || !(temperature < 1e30) || !(temperature > 1e-30))
@@ -645,12 +641,6 @@ at::DimVector with_entries(const LogitRows& x, int64_t k) {
 using MaybeTensor = std::optional<at::Tensor>;
 MaybeTensor maybe(const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : std::nullopt; }
 
-// A new tensor on the logits' device from the caching allocator (of the current stream), without
-// at::empty's dispatch: a small call spends most of its host time on its outputs.
-at::Tensor fresh(const LogitRows& x, at::IntArrayRef shape, at::ScalarType dtype) {
-  return at::detail::empty_cuda(shape, dtype, x.t.device(), std::nullopt);
-}
-
 // (logprob, entropy, lse, top_logprob, top_index, stats) per row; None where not asked for.
 std::tuple<MaybeTensor, at::Tensor, at::Tensor, MaybeTensor, MaybeTensor, MaybeTensor>
 token_logprobs(const at::Tensor& logits, const MaybeTensor& tokens, int64_t top_k,
@@ -663,16 +653,14 @@ token_logprobs(const at::Tensor& logits, const MaybeTensor& tokens, int64_t top_
   const std::optional<BesideRows> tok = token_rows(x, tokens, "token_logprobs");
   const c10::cuda::CUDAGuard guard(x.t.device());
   at::Tensor logprob, entropy, lse, top_logprob, top_index, stats;
-  Outputs outputs;
-  if (tok.has_value()) outputs.add(&logprob, x.lead, at::kFloat);
-  outputs.add(&entropy, x.lead, at::kFloat);
-  outputs.add(&lse, x.lead, at::kFloat);
+  if (tok.has_value()) fresh_figures({&logprob, &entropy, &lse}, x.lead);
+  else fresh_figures({&entropy, &lse}, x.lead);
   if (top_k > 0) {
-    outputs.add(&top_logprob, with_entries(x, top_k), at::kFloat);
-    outputs.add(&top_index, with_entries(x, top_k), at::kLong);
+    const at::DimVector entries = with_entries(x, top_k);
+    top_logprob = fresh(entries, at::kFloat);
+    top_index = fresh(entries, at::kLong);
   }
-  if (want_stats) outputs.add(&stats, {x.rows(), 2}, at::kFloat);
-  outputs.make(x.t.device());
+  if (want_stats) stats = fresh({x.rows(), 2}, at::kFloat);
   auto fp = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
   check_rc(bdh_token_logprobs(
                x.t.data_ptr(), dtype_code(x.t), x.strides,
@@ -715,7 +703,7 @@ at::Tensor token_logprobs_bwd(const at::Tensor& logits, const MaybeTensor& token
     ti = rowmajor(top_index, at::kLong, k * x.rows(), "top_index");
     gt = rowmajor(g_top, at::kFloat, k * x.rows(), "g_top");
   }
-  at::Tensor d = fresh(x, logits.sizes(), x.t.scalar_type());
+  at::Tensor d = fresh(logits.sizes(), x.t.scalar_type());
   const int64_t ds[2] = {x.inner * x.V, x.V};
   check_rc(bdh_token_logprobs_bwd(
                x.t.data_ptr(), dtype_code(x.t), x.strides,
@@ -755,10 +743,10 @@ std::tuple<at::Tensor, MaybeTensor, MaybeTensor> distill_topk(
   const LogitRows x(logits, "distill_topk");
   const c10::cuda::CUDAGuard guard(x.t.device());
   const DistillList l = distill_list(x, index, teacher, weight, temperature);
-  at::Tensor loss = fresh(x, x.lead, at::kFloat);
+  at::Tensor loss = fresh(x.lead, at::kFloat);
   MaybeTensor d, stats;
-  if (want_grad) d = fresh(x, logits.sizes(), x.t.scalar_type());
-  if (want_stats) stats = fresh(x, {x.rows(), 8}, at::kFloat);
+  if (want_grad) d = fresh(logits.sizes(), x.t.scalar_type());
+  if (want_stats) stats = fresh({x.rows(), 8}, at::kFloat);
   const int64_t ds[2] = {x.inner * x.V, x.V};
   check_rc(bdh_distill_topk(x.t.data_ptr(), dtype_code(x.t), x.strides,
                             l.index.t.data_ptr<int64_t>(), l.index.strides,
@@ -783,7 +771,7 @@ at::Tensor distill_topk_bwd(const at::Tensor& logits, const at::Tensor& index,
       stats.numel() != 8 * x.rows())
     TORCH_CHECK_VALUE(false, "distill_topk_bwd: bad stats");
   const at::Tensor st = stats.contiguous();
-  at::Tensor d = fresh(x, logits.sizes(), x.t.scalar_type());
+  at::Tensor d = fresh(logits.sizes(), x.t.scalar_type());
   const int64_t ds[2] = {x.inner * x.V, x.V};
   check_rc(bdh_distill_topk_bwd(x.t.data_ptr(), dtype_code(x.t), x.strides,
                                 l.index.t.data_ptr<int64_t>(), l.index.strides,

@@ -23,7 +23,8 @@ from . import sm100_attn, sm100_ext, sm100_logits
 
 
 class TokenLogprobs(NamedTuple):
-    """Per position; ``logprob`` is None without tokens, the two lists without ``top_k``."""
+    """Per position; ``logprob`` is None without tokens, the two lists without ``top_k``. The lists
+    have a storage each; the three figures may share one."""
 
     logprob: Optional[torch.Tensor]      # (...,) fp32: log p[token]
     entropy: torch.Tensor                # (...,) fp32: -sum p log p
@@ -34,6 +35,9 @@ class TokenLogprobs(NamedTuple):
 
 def _ops():
     """The extension's functions when it is built, else the ctypes binding of the same library."""
+    ext = sm100_ext._ext
+    if ext is not None and ext.in_use():
+        return ext
     ops = sm100_ext.model_ops()
     return sm100_logits if ops is sm100_attn else ops
 
@@ -101,8 +105,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     """
     ops = _ops()
     if ops is not sm100_logits:
-        return TokenLogprobs._make(ops.token_logprobs_autograd(logits, tokens, top_k, temperature,
-                                                               ignore_index))
+        return tuple.__new__(TokenLogprobs, ops.token_logprobs_autograd(
+            logits, tokens, top_k, temperature, ignore_index))
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobsFn.apply(logits, tokens, top_k, temperature,
                                                      ignore_index))

@@ -184,6 +184,29 @@ def test_distillation_over_the_widest_vocabularies(rows, V, dtype):
     check_grad(d[look], dwant, torch.full((3,), 2.0), V, DT[dtype])
 
 
+# ------------------------------------------------------------------- results kept and saved
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("binding", BINDINGS)
+def test_results_can_be_saved_and_do_not_hold_the_lists(binding, grad, monkeypatch):
+    use(binding, monkeypatch)
+    x = make((4, 5), 300, torch.float32).requires_grad_(grad)
+    r = kernels.token_logprobs(x, tokens((4, 5), 300).cuda(), top_k=6)
+    kept = {name: t.detach() for name, t in r._asdict().items()}
+    f = io.BytesIO()
+    torch.save(kept, f)
+    f.seek(0)
+    back = torch.load(f)
+    assert back.keys() == kept.keys()
+    figures = ("logprob", "entropy", "lse")  # (these three may share a storage)
+    for name, t in kept.items():
+        assert torch.equal(back[name], t)
+        own = t.numel() * t.element_size()
+        assert t.untyped_storage().nbytes() <= (3 * (own + 12) if name in figures else own), name
+    shared = {kept[name].untyped_storage().data_ptr() for name in figures}
+    lists_ = {kept[name].untyped_storage().data_ptr() for name in ("top_logprob", "top_index")}
+    assert len(lists_) == 2 and not lists_ & shared
+
+
 # ------------------------------------------------------------------- errors left behind
 def _distill_by_c(x, index, lp, loss, stream):
     rows, V = x.shape
