@@ -516,6 +516,13 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> residual_layer_norm(const at::
 }
 
 // ------------------------------------------------------------------ operators on logits ----
+// The operators have no forward-mode form: a tangent is refused where it would otherwise be dropped.
+void check_no_tangent(const at::Tensor& t, const char* what) {
+  if (t._fw_grad(0).defined())
+    TORCH_CHECK_NOT_IMPLEMENTED(false, std::string(what) +
+                                           ": forward-mode derivatives are not implemented");
+}
+
 // Logits (..., V) as (outer, inner) rows of V with unit stride: the last leading dimension is
 // the inner one and the rest the outer, in place for up to two leading dimensions (and for more
 // where they flatten), else a copy.
@@ -528,6 +535,7 @@ struct LogitRows {
   LogitRows(const at::Tensor& x, const char* what) : t(x) {
     if (x.dim() < 1) TORCH_CHECK_VALUE(false, std::string(what) + ": logits must be (..., V)");
     require_cuda({&x});
+    check_no_tangent(x, what);
     if (x.scalar_type() != at::kFloat && x.scalar_type() != at::kBFloat16)
       TORCH_CHECK_TYPE(false, std::string(what) + ": logits must be float32 or bfloat16, got " +
                                   c10::toString(x.scalar_type()));
@@ -555,6 +563,7 @@ struct BesideRows {
       : t(v) {
     if (!t.is_cuda() || t.device() != x.t.device())
       TORCH_CHECK(false, std::string(what) + " must be on the logits' device");
+    check_no_tangent(t, what);
     const int64_t lists = extra >= 0 ? 1 : 0;
     const int64_t n = static_cast<int64_t>(x.lead.size());
     bool ok = t.dim() == n + lists && (lists == 0 || t.size(-1) == extra);
@@ -691,6 +700,7 @@ at::Tensor token_logprobs_bwd(const at::Tensor& logits, const MaybeTensor& token
   auto rowmajor = [&](const MaybeTensor& v, at::ScalarType dtype, int64_t n, const char* what) {
     if (!v->is_cuda() || v->device() != x.t.device() || v->scalar_type() != dtype || v->numel() != n)
       TORCH_CHECK_VALUE(false, std::string("token_logprobs_bwd: bad ") + what);
+    check_no_tangent(*v, what);
     return v->contiguous();
   };
   const at::Tensor st = rowmajor(stats, at::kFloat, 2 * x.rows(), "stats");

@@ -10,7 +10,7 @@ have no counterpart there. Logits are ``(..., V)`` float32 or bfloat16 with any 
 strides (a shifted view ``[:, :-1]`` is read in place, the vocabulary needs no particular size);
 statistics are float32. CUDA tensors only (no CPU fallback). Work is queued on the current stream
 and can be captured in a CUDA graph. Both operators are differentiable with respect to the logits
-(once); a gradient comes in the logits' dtype.
+(once, in reverse mode; a tangent raises); a gradient comes in the logits' dtype.
 """
 
 from __future__ import annotations
@@ -176,6 +176,7 @@ def distill_topk_loss_grad(logits: torch.Tensor, teacher_index: torch.Tensor,
     one call that reads the logits from memory once (through autograd they are read twice). A
     training step goes on with ``logits.backward(dlogits)``."""
     _constant_teacher(teacher_logprob, weight)
+    sm100_logits.check_no_tangent(logits, "distill_topk")  # (detach drops it)
     loss, d, _ = _ops().distill_topk(logits.detach(), teacher_index, teacher_logprob, weight,
                                      temperature, tail, True)
     return loss, d

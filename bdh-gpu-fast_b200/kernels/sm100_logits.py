@@ -9,6 +9,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .sm100_attn import _check, _code, _require_cuda, _require_lib, _stream
 
@@ -39,6 +40,13 @@ def _lib() -> ctypes.CDLL:
     return lib
 
 
+def check_no_tangent(t: torch.Tensor, what: str) -> None:
+    """The operators have no forward-mode form: a tangent is refused where it would otherwise be
+    dropped."""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented")
+
+
 class _Rows:
     """Logits (..., V) as (outer, inner) rows of V with unit stride, in place for up to two
     leading dimensions (and for more where they flatten)."""
@@ -47,6 +55,7 @@ class _Rows:
         if x.dim() < 1:
             raise ValueError(f"{what}: logits must be (..., V)")
         _require_cuda(x)
+        check_no_tangent(x, what)
         if x.dtype not in (torch.float32, torch.bfloat16):
             raise TypeError(f"{what}: logits must be float32 or bfloat16, got {x.dtype}")
         self.lead, self.V = tuple(x.shape[:-1]), x.size(-1)
@@ -70,6 +79,7 @@ class _Rows:
         """(tensor, strides) of one value (or ``extra`` values) per row."""
         if v.device != self.t.device:
             raise RuntimeError(f"{what} must be on the logits' device")
+        check_no_tangent(v, what)
         want = self.lead + (() if extra is None else (extra,))
         if tuple(v.shape) != want:
             raise ValueError(f"{what} has shape {tuple(v.shape)}, which does not go with logits of "
@@ -150,6 +160,7 @@ def token_logprobs_bwd(logits, tokens, stats, entropy=None, top_index=None, g_lo
     def rowmajor(v, dtype, n, name):
         if v is None or v.device != x.t.device or v.dtype != dtype or v.numel() != n:
             raise ValueError(f"{what}: bad {name}")
+        check_no_tangent(v, name)
         return v.contiguous()
 
     stats = rowmajor(stats, torch.float32, 2 * x.rows, "stats")

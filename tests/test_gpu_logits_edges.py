@@ -207,6 +207,48 @@ def test_results_can_be_saved_and_do_not_hold_the_lists(binding, grad, monkeypat
     assert len(lists_) == 2 and not lists_ & shared
 
 
+# -------------------------------------------------------------------- forward-mode derivatives
+@pytest.mark.parametrize("binding", BINDINGS)
+def test_forward_mode_derivatives_are_refused(binding, monkeypatch):
+    use(binding, monkeypatch)
+    from torch.autograd import forward_ad as fw
+
+    x, tok = make((3,), 50, torch.float32), tokens((3,), 50).cuda()
+    index, lp = (t.cuda() for t in lists((3,), 50, 4))
+    w = torch.rand(3, device="cuda")
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: kernels.token_logprobs(dual(x), tok, top_k=2),
+                     lambda: kernels.token_logprobs(dual(x)[:, 1:]),
+                     lambda: kernels.distill_topk_loss(dual(x), index, lp),
+                     lambda: kernels.distill_topk_loss(x, index, dual(lp)),
+                     lambda: kernels.distill_topk_loss(x, index, lp, weight=dual(w)),
+                     lambda: kernels.distill_topk_loss_grad(dual(x), index, lp),
+                     lambda: kernels.distill_topk_loss_grad(x, index, dual(lp)),
+                     lambda: kernels.distill_topk_loss_grad(x, index, lp, weight=dual(w))):
+            with pytest.raises(RuntimeError, match="forward"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
+                call()
+        z = x.clone().requires_grad_(True)
+        for call in (lambda: kernels.token_logprobs(dual(z), tok), lambda: kernels.distill_topk_loss(dual(z), index, lp)):
+            with pytest.raises(RuntimeError):
+                call()
+        # a tangent that comes with the upstream gradient
+        r = kernels.token_logprobs(z, tok, top_k=2)
+        for y in (r.logprob, r.entropy, r.lse, r.top_logprob, kernels.distill_topk_loss(z, index, lp)):
+            with pytest.raises(RuntimeError, match="forward"):
+                torch.autograd.grad(y, z, dual(torch.ones_like(y.detach())))
+        # torch.func's wrappers have no memory to read
+        for y in (lambda z: kernels.token_logprobs(z, tok).logprob, lambda z: kernels.distill_topk_loss_grad(z, index, lp)[0]):
+            with pytest.raises(RuntimeError):
+                torch.func.jvp(y, (x,), (x,))
+        # nothing else is refused there
+        r = kernels.token_logprobs(x, tok, top_k=2)
+    for a, b in zip(r, kernels.token_logprobs(x, tok, top_k=2)):
+        assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------- errors left behind
 def _distill_by_c(x, index, lp, loss, stream):
     rows, V = x.shape
