@@ -160,7 +160,10 @@ __device__ __forceinline__ void write_figures(const TokenLogprobsArgs& a, int64_
   const bool none = st.m == neg_inf();
   if (a.lse != nullptr) a.lse[row] = none ? neg_inf() : fmaf(st.m, inv_t, ln_s);
   if (a.entropy != nullptr) a.entropy[row] = none ? 0.0f : ln_s - kLn2 * st.a / st.s;
-  if (a.stats != nullptr) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(st.m, ln_s);
+  if (a.stats != nullptr) {  // (at any float: a caller's own allocation)
+    a.stats[2 * row] = st.m;
+    a.stats[2 * row + 1] = ln_s;
+  }
   if (a.tokens != nullptr)
     a.logprob[row] = t.left_out ? 0.0f : t.given ? logprob_of(t.z, st, ln_s, inv_t) : quiet_nan();
 }

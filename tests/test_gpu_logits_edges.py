@@ -335,3 +335,19 @@ def test_calls_of_several_threads_do_not_limit_one_another(op):
         t.join(300)
     torch.cuda.synchronize()
     assert not failed, failed
+
+
+# ---------------------------------------------------------------------------- alignment
+@pytest.mark.parametrize("rows,V,k", [(5, 200, 0), (5, 200, 4), (5, 1000, 3), (0, 1100, 0), (0, 1100, 5), (300, 20011, 0),
+                                      (2, 70001, 6)])
+def test_statistics_at_any_float(rows, V, k):
+    """The C entry writes a row's statistics wherever a float may lie."""
+    rows = rows or many_rows()
+    x = make((rows,), V, torch.float32)
+    top, index = torch.empty(rows, max(k, 1), device="cuda"), torch.empty(rows, max(k, 1), dtype=torch.long, device="cuda")
+    want = sm100_logits.token_logprobs(x, None, k, 1.0, -100, True)[5]
+    room = torch.full((2 * rows + 2,), 7.0, device="cuda")
+    lse = torch.empty(rows, device="cuda")
+    rc = _logprobs_by_c(x, lse, torch.cuda.current_stream().cuda_stream, room[1:], k, top, index)
+    torch.cuda.synchronize()
+    assert rc == 0 and torch.equal(room[1:-1].view(rows, 2), want) and room[0] == 7.0 and room[-1] == 7.0
