@@ -18,7 +18,8 @@
 // way: every slot writes its number in place of its token's logit and reads it back.
 // A longer row is streamed by a CTA of 128 or 256 threads, or by a cluster whose CTAs take a slice each and
 // exchange their sums through distributed shared memory; a bit per element in shared memory says what is
-// listed (and was set twice for a repeated token). For the gradient the slice is streamed again, from L2.
+// listed (and was set twice for a repeated token); a row whose bits have no room in one CTA is split over
+// more. For the gradient the slice is streamed again, from L2.
 // Where a token is repeated its masses are added up by a search (K^2 comparisons, seldom needed).
 // The backward from stored statistics has nothing to sum.
 //

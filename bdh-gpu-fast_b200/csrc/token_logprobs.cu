@@ -12,13 +12,17 @@
 // the K-th largest of the threads' own maxima bounds the K-th largest logit from below, so that only cells
 // above it are looked at again, a few cache lines, and the few candidates are put in order by counting.
 //
-// What bounds it: without a list, memory, with the exponentials close behind. 4096 rows of 131072 in bf16
-// take 162 us, 6.6 TB/s; the exponential's unit is then busy 76% of the time and 0.67 of the issue slots
-// are used (7.2 instructions an element; run for seconds, at the clocks that the power limit leaves, 173).
-// With a list the issue slots (0.75 used): 2048 rows of 65536 with K = 64 take 66 us, 4.1 TB/s, of which
-// the search after the stream is 13, half of it the second look at the cells above the bound. A single
-// row of 131072 with K = 20 takes 8.2 us (with K = 128 13), the latencies of some ten steps that wait for
-// one another. The backward reads and writes at 6.2 to 6.6 TB/s: 81 us for 1024 rows of 131072 in bf16.
+// What bounds it (times here and beside the constants: the kernels alone, from a CUDA graph): without a
+// list, memory, with the exponentials close behind. 4096 rows of 131072 in bf16 take 162 us, 6.6 TB/s; the
+// exponential's unit is then busy 76% of the time and 0.67 of the issue slots are used (7.2 instructions an
+// element; run for seconds, at the clocks that the power limit leaves, 186). With a list the issue slots
+// (0.75 used): 2048 rows of 65536 with K = 64 take 67 us, 4.0 TB/s, of which the search after the stream is
+// 13, half of it the second look at the cells above the bound. A single row of 131072 with K = 20 takes 8.3
+// us (with K = 128 13), the latencies of some ten steps that wait for one another (0.16 of the issue slots of
+// its 8 CTAs). The backward reads and writes at 6.2 to 6.6 TB/s: 81 us for 1024 rows of 131072 in bf16.
+// Through a list it is further off, since every thread adds a row's K upstream gradients and every entry
+// looks for itself among the others: 16384 rows of 256 in bf16 4.7 us without, with K = 16 11.3, with
+// K = 64 65; 2048 rows of 65536 83, with K = 64 125.
 #include <algorithm>
 #include <string>
 
@@ -33,7 +37,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kWarpTop = 16;     // longest list that a warp bounds by its lanes' largest
+// Longest list that a warp bounds by its lanes' largest, one each; longer ones by each element of a short
+// row, by 4 items a lane of a middling one. By lanes and otherwise, bf16: 1200 rows of 256 with K = 16 5.0
+// and 5.3 us, 16384 rows of 1000 with K = 4 29 and 48, with K = 16 33 and 50, with K = 20 36 and 51; 8192 rows
+// of 4096 with K = 4 20.7 and 21.2, with K = 16 24.7 and 24.0, with K = 20 27.3 and 25.7.
+constexpr int kWarpTop = 16;
 // Steps that bring the bound close where the list is more than a quarter of the items that it is searched
 // among: with 24 of 32 lanes' largest above it 45 of 256 elements are, with 16 of them 22. 16384 rows of
 // 256 with K = 16, a warp each: 18.9 us, 21 without; with K = 5 16 and 15.5. 8192 rows of 4096 with
@@ -61,14 +69,21 @@ constexpr int kHalfBytes = 112 * 1024;
 // What a warp's bound is searched among, of a lane: its cells' largest in so many groups. (8192 rows of
 // 2048 with K = 32: 24.5 us, with every cell by itself 28.)
 constexpr int kLaneItems = 4;
-constexpr int kMaxCells = 48;    // cells per thread; longer rows put more batches into a cell
+// Cells per thread; longer rows put more batches into a cell. With up to 24, 48 and 96 cells: 300 rows of
+// 500000 in fp32 with K = 20 120, 120 and 159 us (96: two CTAs an SM), in bf16 with K = 64 83,
+// 100 and 100; 300 rows of 1000000 in bf16 with K = 20 146, 146 and 162; one row of 4000000 in fp32 46, 47
+// and 52.
+constexpr int kMaxCells = 48;
 constexpr int kMaxCluster = 8;
 // A row by itself is split over a cluster in slices of at least 16 KB, but not one of 32 KB or less, which
 // a CTA has read before a cluster has met: one row of 16384 in bf16 3.3 us whole and 3.5 split, of 65536
 // 4.8 whole, 3.7 split, of 131072 8.2 and 4.1.
 constexpr int kUnsplitBytes = 32 * 1024, kSliceBytes = 16 * 1024;
 
-// Threads' maxima that may lie above the bound besides the K wanted: the search for it ends early.
+// Threads' maxima that may lie above the bound besides the K wanted: the search for it ends early. With
+// K / 8 + 2, K / 4 + 4 and K / 2 + 8: 16384 rows of 256 in bf16 with K = 5 12.8, 11.6 and 12.3 us, with K = 16
+// 14.8, 15.7 and 19.3; 8192 rows of 4096 with K = 20 27.1, 25.7 and 28.9; 2048 rows of 65536 with K = 64 67.0,
+// 67.3 and 69.5, with K = 8 61.0, 60.2 and 60.8; a row of 131072 in fp32 with K = 20 8.3, 8.5 and 8.7.
 __host__ __device__ constexpr int top_slack(int K) { return K / 4 + 4; }
 // Room for candidates: every element of the vectors that hold the maxima (a row of equal values),
 // and of the row's ends.
@@ -377,8 +392,10 @@ __device__ __forceinline__ int lanes_before(int v, int lane) {
 
 // Many short rows with a short list: L lanes a row, as without a list. The bound is searched among the
 // largest of every four of a lane's elements, for the warp's rows in step; what is not below it goes to
-// the row's places in shared memory, where counting puts it in order. Bound by the issue slots. 16384 rows
-// of 256 in bf16: K = 1 10.8 us, K = 5 11.8, K = 16 16.3; with a warp a row 15.4, 16.0 and 19.1; but 1200
+// the row's places in shared memory, where counting puts it in order. Bound by its instructions and by
+// how few warps there are to hide their latencies (74 registers: 3 CTAs an SM): with K = 16 16384 rows take
+// 593 instructions each, at 0.65 of the issue slots, in 512 CTAs of which 444 run at a time. 16384 rows
+// of 256 in bf16: K = 1 10.8 us, K = 5 11.6, K = 16 15.7; with a warp a row 15.4, 16.0 and 19.1; but 1200
 // rows with K = 5 5.8 against 4.4 (K = 16: 8.1 and 5.1), and where a list is more than a sixteenth of the
 // row, so that the bound lets much of it through, 25 against 22 (16384 rows of 100 with K = 16).
 constexpr int kLanesRoom = 64;

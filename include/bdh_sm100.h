@@ -428,7 +428,8 @@ int bdh_token_logprobs_bwd(const void* logits, int dtype, const int64_t l_stride
  * masses add. weight null: 1; a row of weight 0 gives exact zeros, whatever its logits and list hold.
  * When the list holds every token there is no other class (r = 0); nor is there one when the student's
  * probability outside the list is below e^-1000 (a mask) and r is at most 2^-16, which the rounding of an
- * fp32 list may leave of a whole. A row with no logit above -inf has loss +inf and gradient 0.
+ * fp32 list may leave of a whole. A row with no logit above -inf has loss +inf (0 where its list has no
+ * mass either) and gradient 0.
  * bdh_distill_topk writes the loss per row and, with dlogits, the gradient of the sum of the losses
  * in the same call (a second look at a row is served by the caches as far as they reach); stats (8
  * floats per row, 16-byte aligned, may be null) is what bdh_distill_topk_bwd reads, which multiplies the
